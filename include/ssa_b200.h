@@ -135,6 +135,57 @@ int ssa_attn_bwd_noalloc(const ssa_problem_t* prob,
                          ssa_tensor_t dq, ssa_tensor_t dk, ssa_tensor_t dv,
                          float* dn, float* db, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Operators of a decoder's training step around the attention. They follow the conventions above
+ * (device pointers, asynchronous on `stream`, caller workspaces, no allocation, status codes);
+ * workspaces are 256-byte aligned. No reference counterpart: its model takes them from NeMo. */
+
+/* Linear cross entropy: loss of the logits x W^T against targets, without keeping the logits.
+ * x [rows, hidden] and w [vocab, hidden] are fp16 or bf16 with unit column stride and 16-byte
+ * aligned rows; hidden is a multiple of 8. targets: int64, a row whose target equals ignore_index
+ * has loss 0 and no gradient, and one outside [0, vocab) gives NaN. */
+typedef struct {
+  int32_t dtype; /* ssa_dtype_t */
+  int32_t rows, hidden, vocab;
+  const void* x;
+  int64_t x_stride; /* elements */
+  const void* w;
+  int64_t w_stride;
+  const int64_t* targets;
+  int64_t ignore_index;
+  int32_t reduction; /* 0 none, 1 mean over the rows that are not ignored, 2 sum */
+} ssa_linear_ce_t;
+
+/* loss: `rows` floats (reduction 0) or 1; lse: rows floats (natural log of the sum of exponentials,
+ * the backward's input); count: 1 float, the rows not ignored (reduction 1 or 2, else unused). */
+int ssa_linear_ce_fwd(const ssa_linear_ce_t* prob, float* loss, float* lse, float* count,
+                      void* workspace, size_t workspace_bytes, void* stream);
+size_t ssa_linear_ce_fwd_workspace_size(const ssa_linear_ce_t* prob);
+/* grad_loss: rows floats (reduction 0) or 1. dx [rows, hidden] and dw [vocab, hidden], contiguous,
+ * in the inputs' dtype; either may be NULL. Deterministic. */
+int ssa_linear_ce_bwd(const ssa_linear_ce_t* prob, const float* lse, const float* count,
+                      const float* grad_loss, void* dx, void* dw, void* workspace,
+                      size_t workspace_bytes, void* stream);
+size_t ssa_linear_ce_bwd_workspace_size(const ssa_linear_ce_t* prob);
+
+/* Gated feed-forward: h = silu(x Wg^T) * (x Wu^T) with w = [Wg; Wu] of [2 ffn, hidden] (the layout
+ * and alignment rules of the linear cross entropy). h and dh are [rows, ffn] with unit column
+ * stride and any row stride of at least ffn. */
+typedef struct {
+  int32_t dtype;
+  int32_t rows, hidden, ffn;
+  const void* x;
+  int64_t x_stride;
+  const void* w;
+  int64_t w_stride;
+} ssa_gated_ffn_t;
+
+int ssa_gated_ffn_fwd(const ssa_gated_ffn_t* prob, void* h, int64_t h_stride, void* stream);
+/* dx [rows, hidden] and dw [2 ffn, hidden], contiguous; either may be NULL. Deterministic. */
+int ssa_gated_ffn_bwd(const ssa_gated_ffn_t* prob, const void* dh, int64_t dh_stride, void* dx,
+                      void* dw, void* workspace, size_t workspace_bytes, void* stream);
+size_t ssa_gated_ffn_bwd_workspace_size(const ssa_gated_ffn_t* prob);
+
 /* Which kernel family serves this problem: 0 = generic (fp32-compute SIMT: fp32 inputs or
  * D = 16, which has no tensor-core kernel), 1 = sm_100a tcgen05/TMA kernels (bf16/fp16 with
  * D in {32, 64, 128}; D = 32 runs the D = 64 kernels). */

@@ -33,7 +33,9 @@ EXPORTED_SYMBOLS = (
     "ssa_attn_fwd", "ssa_attn_fwd_workspace_size", "ssa_attn_bwd_preprocess", "ssa_attn_bwd",
     "ssa_attn_bwd_workspace_size", "ssa_attn_kernel_family", "ssa_device_status",
     "ssa_last_error", "ssa_version", "ssa_kernel_launch_count", "ssa_attn_bwd_noalloc",
-    "ssa_selftest_device_timeout",
+    "ssa_selftest_device_timeout", "ssa_linear_ce_fwd", "ssa_linear_ce_fwd_workspace_size",
+    "ssa_linear_ce_bwd", "ssa_linear_ce_bwd_workspace_size", "ssa_gated_ffn_fwd",
+    "ssa_gated_ffn_bwd", "ssa_gated_ffn_bwd_workspace_size",
 )
 
 
@@ -51,6 +53,20 @@ class SsaProblem(ctypes.Structure):
                 ("max_seqlen", ctypes.c_int32), ("cu_seqlens_padded", ctypes.c_void_p),
                 ("deterministic", ctypes.c_int32), ("dropout_p", ctypes.c_float),
                 ("dropout_seed", ctypes.c_void_p)]
+
+
+class SsaLinearCe(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("rows", ctypes.c_int32), ("hidden", ctypes.c_int32),
+                ("vocab", ctypes.c_int32), ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64),
+                ("w", ctypes.c_void_p), ("w_stride", ctypes.c_int64),
+                ("targets", ctypes.c_void_p), ("ignore_index", ctypes.c_int64),
+                ("reduction", ctypes.c_int32)]
+
+
+class SsaGatedFfn(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("rows", ctypes.c_int32), ("hidden", ctypes.c_int32),
+                ("ffn", ctypes.c_int32), ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64),
+                ("w", ctypes.c_void_p), ("w_stride", ctypes.c_int64)]
 
 
 def deterministic_default() -> bool:
@@ -101,6 +117,19 @@ def load() -> ctypes.CDLL:
         lib.ssa_attn_bwd_workspace_size.restype = sz
         lib.ssa_attn_kernel_family.argtypes = [P]
         lib.ssa_attn_kernel_family.restype = ctypes.c_int
+        CE, FF, i64 = ctypes.POINTER(SsaLinearCe), ctypes.POINTER(SsaGatedFfn), ctypes.c_int64
+        lib.ssa_linear_ce_fwd.argtypes = [CE, vp, vp, vp, vp, sz, vp]
+        lib.ssa_linear_ce_bwd.argtypes = [CE, vp, vp, vp, vp, vp, vp, sz, vp]
+        lib.ssa_gated_ffn_fwd.argtypes = [FF, vp, i64, vp]
+        lib.ssa_gated_ffn_bwd.argtypes = [FF, vp, i64, vp, vp, vp, sz, vp]
+        for fn in (lib.ssa_linear_ce_fwd, lib.ssa_linear_ce_bwd, lib.ssa_gated_ffn_fwd,
+                   lib.ssa_gated_ffn_bwd):
+            fn.restype = ctypes.c_int
+        for fn, prob in ((lib.ssa_linear_ce_fwd_workspace_size, CE),
+                         (lib.ssa_linear_ce_bwd_workspace_size, CE),
+                         (lib.ssa_gated_ffn_bwd_workspace_size, FF)):
+            fn.argtypes = [prob]
+            fn.restype = sz
         lib.ssa_selftest_device_timeout.argtypes = [ctypes.c_uint64, vp]
         lib.ssa_selftest_device_timeout.restype = ctypes.c_int
         lib.ssa_device_status.argtypes = [vp]
@@ -133,6 +162,23 @@ def tensor_thd(t: torch.Tensor) -> SsaTensor:
     """[T, H, D] packed view, expressed as B = 1 (sB = 0), N = T."""
     assert t.dim() == 3 and t.stride(2) == 1
     return SsaTensor(t.data_ptr(), 0, t.stride(1), t.stride(0))
+
+
+def tma_matrix(t: torch.Tensor) -> torch.Tensor:
+    """A 2-D 16-bit matrix the TMA path can address (unit column stride, 16-byte aligned base and
+    row stride, rows that do not overlap): `t` itself, or a copy in fresh storage."""
+    ok = t.stride(1) == 1 and t.data_ptr() % 16 == 0 and (
+        t.shape[0] <= 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1]))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def row_stride(t: torch.Tensor) -> int:
+    """Row stride of a 2-D matrix; a single row's stride is never used and reads as its length."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def workspace(size: int, device: torch.device) -> torch.Tensor:
+    return torch.empty(max(int(size), 1), device=device, dtype=torch.uint8)
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)

@@ -247,6 +247,7 @@ int abi_validate_problem(const ssa_problem_t* pr) {
   g_err[0] = 0;
   return check_problem(pr);
 }
+void abi_clear_error() { g_err[0] = 0; }
 int abi_check_tensor(const ssa_tensor_t& t, const char* name) { return check_tensor(t, name); }
 Problem abi_to_problem(const ssa_problem_t* pr) { return to_problem(pr); }
 int abi_bind_device(const void* ptr, const char* name) { return bind_device(ptr, name); }

@@ -67,6 +67,7 @@ int abi_validate_problem(const ssa_problem_t* pr);
 int abi_check_tensor(const ssa_tensor_t& t, const char* name);
 Problem abi_to_problem(const ssa_problem_t* pr);
 int abi_error(int code, const char* fmt, ...);
+void abi_clear_error();
 // One CTA waiting on an mbarrier nobody completes, with a bounded wait of `cycles` (self-test of
 // the device-timeout path; ssa_sm100_fwd.cu).
 int launch_selftest_timeout(unsigned int* status, long long cycles, cudaStream_t st);

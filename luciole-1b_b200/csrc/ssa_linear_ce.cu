@@ -1,0 +1,459 @@
+// ssa_linear_ce.cu — cross entropy of a linear head, without its logits:
+//     l = x W^T,  lse_r = log sum_v exp(l_rv),  loss_r = lse_r - l_r,t(r)
+//     d_rv = g_r (exp(l_rv - lse_r) - [v = t(r)]),  dx = d W,  dW = d^T x
+// for x [rows, hidden], W [vocab, hidden] in bf16 or fp16, fp32 logits that never leave the chip.
+//
+// Forward: one tensor-core product whose epilogue reduces each row of a tile to a running maximum
+// and sum of exponentials (and picks the target's logit); a second kernel joins the tiles' pairs.
+// Backward: the vocabulary is walked in pieces that fit the workspace. Per piece the logits are
+// formed again and leave as d in 16 bits, then two products read that piece: dx is summed over the
+// pieces in fp32, dW's rows of the piece are final. Bound: the tensor cores, 8 rows hidden vocab
+// operations for forward and backward against the 6 that a kept logit matrix would need.
+#include <atomic>
+#include <cmath>
+
+#include "ssa_gemm.cuh"
+
+namespace ssa {
+namespace sm100 {
+
+int device_sm_count() {
+  static std::atomic<int> counts[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return kPlanSms;
+  if ((n = counts[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1)
+    return kPlanSms;
+  counts[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+constexpr float kLowest = -3.0e38f;  // start of a running maximum: finite, so that max - max is 0
+
+struct CeFwdArgs {
+  const int64_t* targets;
+  float2* part;   // [tiles_n][rows]: (maximum, sum of exp(l - maximum)) of a tile's columns
+  float* target_logit;
+  int rows, vocab;
+};
+
+template <int BN>
+struct EpiCeFwd {
+  using Args = CeFwdArgs;
+  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, int r,
+                                              const AccReader& rd) {
+    const int row = w.mt * 128 + r;
+    const int col0 = w.nt * BN;
+    const bool ok = row < a.rows;
+    const int64_t t = ok ? __ldg(a.targets + row) : -1;
+    float m = kLowest, s = 0.f;
+#pragma unroll 1
+    for (int c = 0; c < BN; c += 32) {
+      if (col0 + c >= a.vocab) break;
+      float v[32];
+      rd(c, v);
+      if (col0 + c + 32 > a.vocab) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (col0 + c + i >= a.vocab) v[i] = -INFINITY;
+      }
+      float m4[4] = {m, m, m, m};
+#pragma unroll
+      for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], v[i]);
+      const float mn = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+      const float b = -mn * kLog2e;
+      float s4[4] = {s * ex2_approx((m - mn) * kLog2e), 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 32; ++i) s4[i & 3] += ex2_approx(fmaf(v[i], kLog2e, b));
+      s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+      m = mn;
+      const int64_t at = t - (col0 + c);
+      if (at >= 0 && at < 32 && t < a.vocab) {
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x = at == i ? v[i] : x;
+        a.target_logit[row] = x;
+      }
+    }
+    if (ok) a.part[(int64_t)w.nt * a.rows + row] = make_float2(m, s);
+  }
+};
+
+// Joins the tiles' pairs: 32 rows per block (one per lane), 32 warps that each walk every 32nd
+// tile. lse in natural units; loss 0 where the target is ignored, NaN where it is out of range.
+__global__ void __launch_bounds__(1024)
+    ce_join_kernel(const float2* part, const float* target_logit, const int64_t* targets,
+                   int64_t ignore_index, int rows, int vocab, int tiles, float* lse, float* loss) {
+  __shared__ float2 sh[32][33];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int lane = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int row = blockIdx.x * 32 + lane;
+  float m = kLowest, s = 0.f;
+  if (row < rows)
+    for (int i = y; i < tiles; i += 32) {
+      const float2 p = part[(int64_t)i * rows + row];
+      const float mn = fmaxf(m, p.x);
+      s = s * ex2_approx((m - mn) * kLog2e) + p.y * ex2_approx((p.x - mn) * kLog2e);
+      m = mn;
+    }
+  sh[y][lane] = make_float2(m, s);
+  __syncthreads();
+  if (y == 0 && row < rows) {
+    for (int i = 1; i < 32; ++i) {
+      const float2 p = sh[i][lane];
+      const float mn = fmaxf(m, p.x);
+      s = s * ex2_approx((m - mn) * kLog2e) + p.y * ex2_approx((p.x - mn) * kLog2e);
+      m = mn;
+    }
+    const float ls = logf(s);
+    lse[row] = m + ls;
+    const int64_t t = targets[row];
+    // (m - l_t) + log s: no cancellation between a large lse and a large logit
+    loss[row] = t == ignore_index ? 0.f
+                : (t < 0 || t >= vocab) ? nan_f32()
+                                        : (m - target_logit[row]) + ls;
+  }
+}
+
+// Sum over a block of 1024 threads in a fixed order.
+__device__ __forceinline__ double block_sum_1024(double v, double* red) {
+  red[threadIdx.x] = v;
+  __syncthreads();
+  for (int o = 512; o > 0; o >>= 1) {
+    if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
+    __syncthreads();
+  }
+  const double t = red[0];
+  __syncthreads();
+  return t;
+}
+
+// Sum of the rows' losses in 64 bits (mean: over the rows that are not ignored), and that count.
+__global__ void __launch_bounds__(1024)
+    ce_total_kernel(const float* loss_rows, const int64_t* targets, int64_t ignore_index, int rows,
+                    int mean, float* loss, float* count) {
+  __shared__ double red[1024];
+  griddep_wait();
+  griddep_launch_dependents();
+  double s = 0.0, n = 0.0;
+  for (int i = threadIdx.x; i < rows; i += 1024) {
+    s += (double)loss_rows[i];
+    n += targets[i] != ignore_index ? 1.0 : 0.0;
+  }
+  s = block_sum_1024(s, red);
+  n = block_sum_1024(n, red);
+  if (threadIdx.x == 0) {
+    *loss = (float)(mean ? s / n : s);
+    *count = (float)n;
+  }
+}
+
+// Row weights of the backward, g_r = grad (1 value or one per row) / count, 0 for ignored rows,
+// multiplied by the power of two that brings the largest to [2^11, 2^12): d is held in 16 bits,
+// and in fp16 the small probabilities of a large vocabulary would be subnormal without it. The
+// products' epilogues multiply by *inv, its exact inverse.
+__global__ void __launch_bounds__(1024)
+    ce_row_weights_kernel(const float* grad, int per_row, const int64_t* targets,
+                          int64_t ignore_index, int rows, int vocab, const float* count, int mean,
+                          float* weight, float* inv) {
+  __shared__ float red[32];
+  griddep_wait();
+  griddep_launch_dependents();
+  const float n = mean ? *count : 1.f;
+  float top = 0.f;
+  for (int i = threadIdx.x; i < rows; i += 1024)
+    if (targets[i] != ignore_index) top = fmaxf(top, fabsf(grad[per_row ? i : 0] / n));
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+  __syncthreads();
+  top = red[threadIdx.x & 31];
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  int e = 0;
+  if (top > 0.f && top < INFINITY) e = max(-126, min(126, 11 - ilogbf(top)));
+  const float up = ldexpf(1.f, e);
+  for (int i = threadIdx.x; i < rows; i += 1024) {
+    const int64_t t = targets[i];
+    float g = grad[per_row ? i : 0] / n * up;
+    if (t == ignore_index) g = 0.f;
+    else if (t < 0 || t >= vocab) g = nan_f32();
+    weight[i] = g;
+  }
+  if (threadIdx.x == 0) *inv = ldexpf(1.f, -e);
+}
+
+struct CeBwdArgs {
+  const int64_t* targets;
+  const float* lse;
+  const float* weight;
+  void* d;         // 16-bit [rows][ldd], this piece's columns; columns past the vocabulary are 0
+  int64_t ldd;
+  int rows, piece0, vocab;
+};
+
+template <int BN, bool BF16>
+struct EpiCeBwd {
+  using Args = CeBwdArgs;
+  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, int r,
+                                              const AccReader& rd) {
+    const int row = w.mt * 128 + r;
+    const bool ok = row < a.rows;
+    const float g = ok ? __ldg(a.weight + row) : 0.f;
+    const float b = ok ? -__ldg(a.lse + row) * kLog2e : 0.f;
+    const int64_t t = ok ? __ldg(a.targets + row) : -1;
+    uint16_t* drow = reinterpret_cast<uint16_t*>(a.d) + (int64_t)row * a.ldd + w.nt * BN;
+#pragma unroll 1
+    for (int c = 0; c < BN; c += 32) {
+      const int col = a.piece0 + w.nt * BN + c;
+      float v[32];
+      rd(c, v);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = ex2_approx(fmaf(v[i], kLog2e, b)) * g;
+      const int64_t at = t - col;
+      if (at >= 0 && at < 32) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = at == i ? v[i] - g : v[i];
+      }
+      if (g == 0.f || col + 32 > a.vocab) {  // an ignored row adds nothing, whatever its logits
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (g == 0.f || col + i >= a.vocab) v[i] = 0.f;
+      }
+      if (ok) {
+        uint4* o = reinterpret_cast<uint4*>(drow + c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          o[i] = make_uint4(pack2<BF16>(v[8 * i], v[8 * i + 1]), pack2<BF16>(v[8 * i + 2], v[8 * i + 3]),
+                            pack2<BF16>(v[8 * i + 4], v[8 * i + 5]),
+                            pack2<BF16>(v[8 * i + 6], v[8 * i + 7]));
+      }
+    }
+  }
+};
+
+}  // namespace sm100
+
+namespace {
+
+using namespace sm100;
+
+// d of one piece; the larger, the fewer passes over the fp32 sums of dx
+constexpr int64_t kPieceBytes = (int64_t)256 << 20;
+
+struct CePlan {
+  int tiles_n;                 // forward column tiles
+  int64_t ldd;                 // columns of a piece (a multiple of 256)
+  int pieces;
+  int dx_bn, dx_splits;
+  size_t off_target, off_rows, fwd_bytes;
+  size_t off_inv, off_d, off_sum, bwd_bytes;
+};
+
+CePlan ce_plan(const ssa_linear_ce_t* p) {
+  CePlan q{};
+  const int64_t rows = p->rows;
+  q.tiles_n = cdiv(p->vocab, 256);
+  q.off_target = up256(sizeof(float2) * (size_t)q.tiles_n * rows);
+  q.off_rows = q.off_target + up256(sizeof(float) * rows);
+  q.fwd_bytes = q.off_rows + up256(sizeof(float) * rows);
+
+  int64_t cols = kPieceBytes / (2 * rows) / 256 * 256;
+  if (cols < 1024) cols = 1024;
+  const int64_t all = (int64_t)cdiv(p->vocab, 256) * 256;
+  if (cols > all) cols = all;
+  q.pieces = cdiv(all, cols);
+  q.ldd = (int64_t)cdiv(all / 256, q.pieces) * 256;  // pieces of about equal width
+  q.pieces = cdiv(all, q.ldd);
+  const int tm = cdiv(rows, 128);
+  // dx: [rows, hidden] tiles that contract over the vocabulary. Too few of them for the
+  // multiprocessors: narrower tiles, then each tile's contraction in splits.
+  q.dx_bn = (int64_t)tm * cdiv(p->hidden, 256) >= kPlanSms ? 256 : 128;
+  const int tiles = tm * cdiv(p->hidden, q.dx_bn);
+  const int kblocks = (int)(q.ldd / 64);
+  q.dx_splits = split_count(tiles, kblocks);
+  q.off_inv = up256(sizeof(float) * rows);
+  q.off_d = q.off_inv + 256;
+  q.off_sum = q.off_d + up256(2 * (size_t)rows * q.ldd);
+  q.bwd_bytes = q.off_sum;
+  if (q.pieces > 1 || q.dx_splits > 1)
+    q.bwd_bytes += up256(sizeof(float) * (size_t)q.dx_splits * rows * p->hidden);
+  return q;
+}
+
+int ce_check(const ssa_linear_ce_t* p) {
+  if (!p) return abi_error(SSA_ERR_NULL, "problem is NULL");
+  if (p->dtype != SSA_DTYPE_F16 && p->dtype != SSA_DTYPE_BF16)
+    return abi_error(SSA_ERR_UNSUPPORTED, "linear_ce: dtype %d not supported (fp16, bf16)", p->dtype);
+  if (p->rows <= 0 || p->hidden <= 0 || p->vocab <= 0)
+    return abi_error(SSA_ERR_BAD_SHAPE, "linear_ce: non-positive shape rows=%d hidden=%d vocab=%d",
+                     p->rows, p->hidden, p->vocab);
+  if (p->hidden % 8)
+    return abi_error(SSA_ERR_BAD_SHAPE, "linear_ce: hidden=%d must be a multiple of 8", p->hidden);
+  if (p->rows > (1 << 24) || p->vocab > (1 << 24))
+    return abi_error(SSA_ERR_BAD_SHAPE, "linear_ce: rows and vocab must not exceed 2^24");
+  if (p->reduction < 0 || p->reduction > 2)
+    return abi_error(SSA_ERR_UNSUPPORTED, "linear_ce: reduction %d (0 none, 1 mean, 2 sum)",
+                     p->reduction);
+  if (!p->x || !p->w || !p->targets)
+    return abi_error(SSA_ERR_NULL, "linear_ce: x, w or targets is NULL");
+  if (((uintptr_t)p->x | (uintptr_t)p->w) % 16 || p->x_stride % 8 || p->w_stride % 8 ||
+      p->x_stride < p->hidden || p->w_stride < p->hidden)
+    return abi_error(SSA_ERR_BAD_STRIDE, "linear_ce: x and w need 16-byte aligned rows of at least "
+                     "hidden elements");
+  return SSA_OK;
+}
+
+template <bool BF16>
+int ce_fwd(const ssa_linear_ce_t* p, const CePlan& q, float* loss, float* lse, float* count,
+           uint8_t* ws, cudaStream_t st) {
+  CeFwdArgs a{p->targets, reinterpret_cast<float2*>(ws),
+              reinterpret_cast<float*>(ws + q.off_target), p->rows, p->vocab};
+  const GemmShape g = plain_shape(cdiv(p->rows, 128), q.tiles_n, cdiv(p->hidden, 64),
+                                  2 * (int64_t)p->rows * p->hidden);
+  int rc = launch_gemm<EpiCeFwd<256>, 256, false, false, BF16>(
+      GemmOperand{p->x, p->rows, p->hidden, p->x_stride, "x"},
+      GemmOperand{p->w, p->vocab, p->hidden, p->w_stride, "w"}, g, a, st);
+  if (rc != SSA_OK) return rc;
+  float* rows_loss = p->reduction ? reinterpret_cast<float*>(ws + q.off_rows) : loss;
+  cudaError_t e = launch_pdl(ce_join_kernel, dim3((unsigned)cdiv(p->rows, 32)), dim3(1024), 0, st,
+                             (const float2*)a.part, (const float*)a.target_logit, p->targets,
+                             p->ignore_index, p->rows, p->vocab, q.tiles_n, lse, rows_loss);
+  if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "ce_join: %s", cudaGetErrorString(e));
+  note_launches(1);
+  if (p->reduction) {
+    e = launch_pdl(ce_total_kernel, dim3(1), dim3(1024), 0, st, (const float*)rows_loss, p->targets,
+                   p->ignore_index, p->rows, (int)(p->reduction == 1), loss, count);
+    if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "ce_total: %s", cudaGetErrorString(e));
+    note_launches(1);
+  }
+  return SSA_OK;
+}
+
+template <bool BF16>
+int ce_bwd(const ssa_linear_ce_t* p, const CePlan& q, const float* lse, const float* count,
+           const float* grad, void* dx, void* dw, uint8_t* ws, cudaStream_t st) {
+  float* weight = reinterpret_cast<float*>(ws);
+  float* inv = reinterpret_cast<float*>(ws + q.off_inv);
+  uint8_t* d = ws + q.off_d;
+  float* sum = reinterpret_cast<float*>(ws + q.off_sum);
+  const cudaError_t e = launch_pdl(ce_row_weights_kernel, dim3(1), dim3(1024), 0, st, grad,
+                                   (int)(p->reduction == 0), p->targets, p->ignore_index, p->rows,
+                                   p->vocab, count, (int)(p->reduction == 1), weight, inv);
+  if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "ce_row_weights: %s", cudaGetErrorString(e));
+  note_launches(1);
+  const int tm = cdiv(p->rows, 128);
+  for (int i = 0; i < q.pieces; ++i) {
+    const int64_t v0 = (int64_t)i * q.ldd;
+    const int64_t cols = p->vocab - v0 < q.ldd ? p->vocab - v0 : q.ldd;  // of the vocabulary
+    const int64_t wide = (int64_t)cdiv(cols, 256) * 256;                 // written to d
+    const uint8_t* w0 = static_cast<const uint8_t*>(p->w) + 2 * v0 * p->w_stride;
+    CeBwdArgs a{p->targets, lse, weight, d, q.ldd, p->rows, (int)v0, p->vocab};
+    int rc = launch_gemm<EpiCeBwd<256, BF16>, 256, false, false, BF16>(
+        GemmOperand{p->x, p->rows, p->hidden, p->x_stride, "x"},
+        GemmOperand{w0, cols, p->hidden, p->w_stride, "w"},
+        plain_shape(tm, (int)(wide / 256), cdiv(p->hidden, 64), 2 * (int64_t)p->rows * p->hidden), a,
+        st);
+    if (rc != SSA_OK) return rc;
+    if (dx) {
+      const bool direct = q.dx_splits == 1 && i == q.pieces - 1;
+      StoreArgs s{};
+      s.out = direct ? dx : nullptr;
+      s.sum = sum;
+      s.scale = inv;
+      s.rows = p->rows;
+      s.ldo = p->hidden;
+      s.cols = p->hidden;
+      s.add_prev = i > 0;
+      const int kblocks = (int)(wide / 64);
+      GemmShape g = plain_shape(tm, cdiv(p->hidden, q.dx_bn), kblocks,
+                                2 * (int64_t)p->rows * q.ldd);
+      // every piece fills the same split planes: a narrower last piece takes thinner splits
+      g.kb_split = cdiv(kblocks, q.dx_splits);
+      g.splits = cdiv(kblocks, g.kb_split);
+      const GemmOperand A{d, p->rows, wide, q.ldd, "d"};
+      const GemmOperand B{w0, p->hidden, cols, p->w_stride, "w"};
+      rc = q.dx_bn == 256 ? launch_gemm<EpiStore<256, BF16>, 256, false, true, BF16>(A, B, g, s, st)
+                          : launch_gemm<EpiStore<128, BF16>, 128, false, true, BF16>(A, B, g, s, st);
+      if (rc != SSA_OK) return rc;
+    }
+    if (dw) {
+      StoreArgs s{};
+      s.out = static_cast<uint8_t*>(dw) + 2 * v0 * p->hidden;
+      s.scale = inv;
+      s.rows = cols;
+      s.ldo = p->hidden;
+      s.cols = p->hidden;
+      rc = launch_gemm<EpiStore<256, BF16>, 256, true, true, BF16>(
+          GemmOperand{d, wide, p->rows, q.ldd, "d"},
+          GemmOperand{p->x, p->hidden, p->rows, p->x_stride, "x"},
+          plain_shape((int)cdiv(cols, 128), cdiv(p->hidden, 256), cdiv(p->rows, 64),
+                      2 * (int64_t)p->rows * q.ldd), s, st);
+      if (rc != SSA_OK) return rc;
+    }
+  }
+  if (dx && q.dx_splits > 1)
+    return launch_sum_splits<BF16>(sum, dx, inv, p->rows, p->hidden, p->hidden, q.dx_splits, st);
+  return SSA_OK;
+}
+
+}  // namespace
+}  // namespace ssa
+
+using namespace ssa;
+
+extern "C" {
+
+size_t ssa_linear_ce_fwd_workspace_size(const ssa_linear_ce_t* p) {
+  abi_clear_error();
+  if (ce_check(p) != SSA_OK) return 0;
+  return ce_plan(p).fwd_bytes;
+}
+
+size_t ssa_linear_ce_bwd_workspace_size(const ssa_linear_ce_t* p) {
+  abi_clear_error();
+  if (ce_check(p) != SSA_OK) return 0;
+  return ce_plan(p).bwd_bytes;
+}
+
+int ssa_linear_ce_fwd(const ssa_linear_ce_t* p, float* loss, float* lse, float* count,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+  abi_clear_error();
+  int rc = ce_check(p);
+  if (rc != SSA_OK) return rc;
+  if (!loss || !lse || (p->reduction && !count))
+    return abi_error(SSA_ERR_NULL, "linear_ce: loss, lse or count is NULL");
+  if ((rc = abi_bind_device(p->x, "x")) != SSA_OK) return rc;
+  const CePlan q = ce_plan(p);
+  if (!workspace || workspace_bytes < q.fwd_bytes || (uintptr_t)workspace % 256)
+    return abi_error(SSA_ERR_WORKSPACE, "workspace needs %zu bytes (256-byte aligned), got %zu", q.fwd_bytes,
+                     workspace_bytes);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return p->dtype == SSA_DTYPE_BF16 ? ce_fwd<true>(p, q, loss, lse, count, ws, st)
+                                    : ce_fwd<false>(p, q, loss, lse, count, ws, st);
+}
+
+int ssa_linear_ce_bwd(const ssa_linear_ce_t* p, const float* lse, const float* count,
+                      const float* grad_loss, void* dx, void* dw, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  abi_clear_error();
+  int rc = ce_check(p);
+  if (rc != SSA_OK) return rc;
+  if (!lse || !grad_loss || (p->reduction == 1 && !count))
+    return abi_error(SSA_ERR_NULL, "linear_ce: lse, grad_loss or count is NULL");
+  if (((uintptr_t)dx | (uintptr_t)dw) % 16)
+    return abi_error(SSA_ERR_BAD_STRIDE, "linear_ce: dx and dw must be 16-byte aligned");
+  if (!dx && !dw) return SSA_OK;
+  if ((rc = abi_bind_device(p->x, "x")) != SSA_OK) return rc;
+  const CePlan q = ce_plan(p);
+  if (!workspace || workspace_bytes < q.bwd_bytes || (uintptr_t)workspace % 256)
+    return abi_error(SSA_ERR_WORKSPACE, "workspace needs %zu bytes (256-byte aligned), got %zu", q.bwd_bytes,
+                     workspace_bytes);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return p->dtype == SSA_DTYPE_BF16
+             ? ce_bwd<true>(p, q, lse, count, grad_loss, dx, dw, ws, st)
+             : ce_bwd<false>(p, q, lse, count, grad_loss, dx, dw, ws, st);
+}
+
+}  // extern "C"
