@@ -186,6 +186,58 @@ int ssa_gated_ffn_bwd(const ssa_gated_ffn_t* prob, const void* dh, int64_t dh_st
                       void* dw, void* workspace, size_t workspace_bytes, void* stream);
 size_t ssa_gated_ffn_bwd_workspace_size(const ssa_gated_ffn_t* prob);
 
+/* Queries and keys out of a packed qkv projection: per-head RMS norm (with q_weight / k_weight, both
+ * or neither) and rotate-half position rotation, y = n cos + rot(n) sin, in one pass. qkv is a
+ * strided [B, Hq + 2 Hkv, S, D] view (sN the row stride, sH the head stride), queries first, then
+ * keys, then values; 16-byte aligned base and strides; D 16, 32, 64 or 128; fp32, fp16 or bf16.
+ * cos / sin: fp32 [table_rows, D]. positions: NULL (row s of a sequence has position s), or int32 /
+ * int64 values, positions_stride apart per sequence (0: one row for all); a position outside the
+ * tables gives NaN. */
+typedef struct {
+  int32_t dtype;
+  int32_t B, S, Hq, Hkv, D;
+  ssa_tensor_t qkv;
+  const float* cos;
+  const float* sin;
+  int32_t table_rows;
+  const void* positions;
+  int32_t positions_64; /* positions are int64 */
+  int64_t positions_stride;
+  const void* q_weight;
+  const void* k_weight;
+  int32_t weight_dtype; /* dtype, or SSA_DTYPE_F32 */
+  float eps;
+} ssa_qk_rope_t;
+
+/* q [B, S, Hq, D] and k [B, S, Hkv, D], contiguous. */
+int ssa_qk_rope_fwd(const ssa_qk_rope_t* prob, void* q, void* k, void* stream);
+/* dq, dk, dv: strided [B, H, S, D]. dqkv: contiguous [B, S, (Hq + 2 Hkv) D], with dv copied into
+ * its place; dq_weight, dk_weight: D values of weight_dtype, or NULL. Deterministic. */
+int ssa_qk_rope_bwd(const ssa_qk_rope_t* prob, ssa_tensor_t dq, ssa_tensor_t dk, ssa_tensor_t dv,
+                    void* dqkv, void* dq_weight, void* dk_weight, void* workspace,
+                    size_t workspace_bytes, void* stream);
+size_t ssa_qk_rope_bwd_workspace_size(const ssa_qk_rope_t* prob);
+
+/* A list of gradient tensors (host arrays of device pointers and element counts), each contiguous.
+ * outs NULL: in place. out_dtype: dtype or SSA_DTYPE_F32. */
+typedef struct {
+  int32_t dtype;
+  int32_t count;
+  const void* const* grads;
+  const int64_t* sizes;
+  void* const* outs;
+  int32_t out_dtype;
+} ssa_grad_list_t;
+
+/* 2-norm over the list (1 float, device). Deterministic. */
+int ssa_grad_norm(const ssa_grad_list_t* list, float* norm, void* workspace, size_t workspace_bytes,
+                  void* stream);
+/* The same, then every element times min(1, max_norm / (norm + 1e-6)). Written tensors must not
+ * share memory. */
+int ssa_grad_clip(const ssa_grad_list_t* list, float max_norm, float* norm, void* workspace,
+                  size_t workspace_bytes, void* stream);
+size_t ssa_grad_clip_workspace_size(const ssa_grad_list_t* list);
+
 /* Which kernel family serves this problem: 0 = generic (fp32-compute SIMT: fp32 inputs or
  * D = 16, which has no tensor-core kernel), 1 = sm_100a tcgen05/TMA kernels (bf16/fp16 with
  * D in {32, 64, 128}; D = 32 runs the D = 64 kernels). */

@@ -35,7 +35,9 @@ EXPORTED_SYMBOLS = (
     "ssa_last_error", "ssa_version", "ssa_kernel_launch_count", "ssa_attn_bwd_noalloc",
     "ssa_selftest_device_timeout", "ssa_linear_ce_fwd", "ssa_linear_ce_fwd_workspace_size",
     "ssa_linear_ce_bwd", "ssa_linear_ce_bwd_workspace_size", "ssa_gated_ffn_fwd",
-    "ssa_gated_ffn_bwd", "ssa_gated_ffn_bwd_workspace_size",
+    "ssa_gated_ffn_bwd", "ssa_gated_ffn_bwd_workspace_size", "ssa_qk_rope_fwd", "ssa_qk_rope_bwd",
+    "ssa_qk_rope_bwd_workspace_size", "ssa_grad_norm", "ssa_grad_clip",
+    "ssa_grad_clip_workspace_size",
 )
 
 
@@ -67,6 +69,22 @@ class SsaGatedFfn(ctypes.Structure):
     _fields_ = [("dtype", ctypes.c_int32), ("rows", ctypes.c_int32), ("hidden", ctypes.c_int32),
                 ("ffn", ctypes.c_int32), ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64),
                 ("w", ctypes.c_void_p), ("w_stride", ctypes.c_int64)]
+
+
+class SsaQkRope(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("B", ctypes.c_int32), ("S", ctypes.c_int32),
+                ("Hq", ctypes.c_int32), ("Hkv", ctypes.c_int32), ("D", ctypes.c_int32),
+                ("qkv", SsaTensor), ("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p),
+                ("table_rows", ctypes.c_int32), ("positions", ctypes.c_void_p),
+                ("positions_64", ctypes.c_int32), ("positions_stride", ctypes.c_int64),
+                ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p),
+                ("weight_dtype", ctypes.c_int32), ("eps", ctypes.c_float)]
+
+
+class SsaGradList(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("count", ctypes.c_int32), ("grads", ctypes.c_void_p),
+                ("sizes", ctypes.c_void_p), ("outs", ctypes.c_void_p),
+                ("out_dtype", ctypes.c_int32)]
 
 
 def deterministic_default() -> bool:
@@ -122,12 +140,20 @@ def load() -> ctypes.CDLL:
         lib.ssa_linear_ce_bwd.argtypes = [CE, vp, vp, vp, vp, vp, vp, sz, vp]
         lib.ssa_gated_ffn_fwd.argtypes = [FF, vp, i64, vp]
         lib.ssa_gated_ffn_bwd.argtypes = [FF, vp, i64, vp, vp, vp, sz, vp]
+        QK, GL = ctypes.POINTER(SsaQkRope), ctypes.POINTER(SsaGradList)
+        lib.ssa_qk_rope_fwd.argtypes = [QK, vp, vp, vp]
+        lib.ssa_qk_rope_bwd.argtypes = [QK, T, T, T, vp, vp, vp, vp, sz, vp]
+        lib.ssa_grad_norm.argtypes = [GL, vp, vp, sz, vp]
+        lib.ssa_grad_clip.argtypes = [GL, ctypes.c_float, vp, vp, sz, vp]
         for fn in (lib.ssa_linear_ce_fwd, lib.ssa_linear_ce_bwd, lib.ssa_gated_ffn_fwd,
-                   lib.ssa_gated_ffn_bwd):
+                   lib.ssa_gated_ffn_bwd, lib.ssa_qk_rope_fwd, lib.ssa_qk_rope_bwd,
+                   lib.ssa_grad_norm, lib.ssa_grad_clip):
             fn.restype = ctypes.c_int
         for fn, prob in ((lib.ssa_linear_ce_fwd_workspace_size, CE),
                          (lib.ssa_linear_ce_bwd_workspace_size, CE),
-                         (lib.ssa_gated_ffn_bwd_workspace_size, FF)):
+                         (lib.ssa_gated_ffn_bwd_workspace_size, FF),
+                         (lib.ssa_qk_rope_bwd_workspace_size, QK),
+                         (lib.ssa_grad_clip_workspace_size, GL)):
             fn.argtypes = [prob]
             fn.restype = sz
         lib.ssa_selftest_device_timeout.argtypes = [ctypes.c_uint64, vp]
@@ -175,6 +201,12 @@ def tma_matrix(t: torch.Tensor) -> torch.Tensor:
 def row_stride(t: torch.Tensor) -> int:
     """Row stride of a 2-D matrix; a single row's stride is never used and reads as its length."""
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def table(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous, 16-byte aligned table: `t` itself, or a copy in fresh storage."""
+    ok = t.is_contiguous() and t.data_ptr() % 16 == 0
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 def workspace(size: int, device: torch.device) -> torch.Tensor:

@@ -1,0 +1,368 @@
+// ssa_grad_clip.cu — the 2-norm over a list of gradient tensors, and the gradients scaled by
+// min(1, max_norm / (norm + 1e-6)), in place or into fp32 tensors (an optimizer's master
+// gradients, which saves their separate conversion).
+//
+// Bound: memory. The norm reads every gradient once; the scaling needs the norm, so it reads them
+// again and writes once. The tensors' addresses and sizes travel in the kernels' parameter block
+// (no table copy to the device, nothing to keep alive, capturable as it is), up to kTable tensors
+// per launch. Work is cut into chunks of kChunk elements, one block each; the second pass walks the
+// chunks from the last to the first, so that what the first pass read last is still in L2.
+//
+// Squares are added in fp32 over a thread's few elements of a chunk and in fp64 from there on, in
+// a fixed order: the norm is the same from run to run. A thread whose fp32 sum overflowed, or is so
+// small that squares may have been lost, adds its elements again in fp64.
+#include <cmath>
+
+#include "ssa_internal.h"
+#include "ssa_sm100.cuh"
+
+namespace ssa {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kUnit = 8;                          // elements a thread takes at a time
+constexpr int kUnits = 4;                         // times it does so per chunk
+constexpr int kChunk = kThreads * kUnit * kUnits;
+
+struct TableEntry {
+  const void* in;
+  void* out;
+  int64_t n;
+  int32_t first;     // index of the tensor's first chunk among the launch's chunks
+  int32_t vec;       // 16-byte accesses are aligned on both sides
+};
+
+template <int kTable>
+struct Table {
+  int32_t tensors;
+  int32_t chunks;
+  TableEntry t[kTable];
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else {
+    const uint4 x = *reinterpret_cast<const uint4*>(p);
+    const T* h = reinterpret_cast<const T*>(&x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(h[i]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    uint4 x;
+    T* h = reinterpret_cast<T*>(&x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = from_f32<T>(v[i]);
+    *reinterpret_cast<uint4*>(p) = x;
+  }
+}
+
+// The tensor of a chunk: the last entry whose first chunk is not past it.
+template <int kTable>
+__device__ __forceinline__ int find_tensor(const Table<kTable>& t, int chunk) {
+  int lo = 0, hi = t.tensors - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.t[mid].first <= chunk) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+template <typename T, int kTable>
+__global__ void __launch_bounds__(kThreads)
+    sum_squares_kernel(const __grid_constant__ Table<kTable> tab, double* part) {
+  __shared__ double red[kThreads / 32];
+  sm100::griddep_wait();
+  sm100::griddep_launch_dependents();
+  const TableEntry& e = tab.t[find_tensor(tab, (int)blockIdx.x)];
+  const int64_t base = (int64_t)((int)blockIdx.x - e.first) * kChunk;
+  const T* in = reinterpret_cast<const T*>(e.in);
+  float v[kUnits][kUnit];
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    const int64_t at = base + ((int64_t)u * kThreads + threadIdx.x) * kUnit;
+    if (e.vec && at + kUnit <= e.n) {
+      load8(in + at, v[u]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kUnit; ++i) v[u][i] = at + i < e.n ? to_f32<T>(in[at + i]) : 0.f;
+    }
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i) s = fmaf(v[u][i], v[u][i], s);
+  double d = (double)s;
+  // fp32 squares overflow above 1.8e19 and lose digits below 1e-18 or so
+  if (!(s < 3.0e38f) || s < 1.0e-30f) {
+    d = 0.0;
+    float top = 0.f;  // all zero (rows of an embedding that no token reached): nothing to redo
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+      for (int i = 0; i < kUnit; ++i) top = v[u][i] == 0.f ? top : 1.f;
+    if (top != 0.f) {
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i) d = fma((double)v[u][i], (double)v[u][i], d);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = d;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < kThreads / 32; ++i) d += red[i];
+    part[blockIdx.x] = d;
+  }
+}
+
+// norm = sqrt of the chunks' sums, coef = min(1, max_norm / (norm + 1e-6)); NaN stays NaN.
+__global__ void __launch_bounds__(1024) norm_kernel(const double* part, int64_t n, float max_norm,
+                                                    float* norm, float* coef) {
+  __shared__ double red[1024];
+  sm100::griddep_wait();
+  sm100::griddep_launch_dependents();
+  double s[4] = {0.0, 0.0, 0.0, 0.0};
+  int64_t i = threadIdx.x;
+  for (; i + 3 * 1024 < n; i += 4 * 1024) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s[k] += part[i + k * 1024];
+  }
+  for (; i < n; i += 1024) s[0] += part[i];
+  red[threadIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
+  __syncthreads();
+  for (int o = 512; o > 0; o >>= 1) {
+    if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    const float r = (float)sqrt(red[0]);
+    *norm = r;
+    if (coef) {
+      const float c = max_norm / (r + 1e-6f);
+      *coef = c > 1.f ? 1.f : c;
+    }
+  }
+}
+
+template <typename T, typename O, int kTable>
+__global__ void __launch_bounds__(kThreads)
+    scale_kernel(const __grid_constant__ Table<kTable> tab, const float* coef) {
+  sm100::griddep_wait();
+  sm100::griddep_launch_dependents();
+  const float c = __ldg(coef);
+  const int chunk = tab.chunks - 1 - (int)blockIdx.x;  // last chunk first: its data is still in L2
+  const TableEntry& e = tab.t[find_tensor(tab, chunk)];
+  if (c == 1.f && e.in == e.out) return;  // in place and nothing to scale
+  const int64_t base = (int64_t)(chunk - e.first) * kChunk;
+  const T* in = reinterpret_cast<const T*>(e.in);
+  O* out = reinterpret_cast<O*>(e.out);
+  float v[kUnits][kUnit];
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    const int64_t at = base + ((int64_t)u * kThreads + threadIdx.x) * kUnit;
+    if (e.vec && at + kUnit <= e.n) {
+      load8(in + at, v[u]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kUnit; ++i) v[u][i] = at + i < e.n ? to_f32<T>(in[at + i]) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    const int64_t at = base + ((int64_t)u * kThreads + threadIdx.x) * kUnit;
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i) v[u][i] *= c;
+    if (e.vec && at + kUnit <= e.n) {
+      store8(out + at, v[u]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kUnit; ++i)
+        if (at + i < e.n) out[at + i] = from_f32<O>(v[u][i]);
+    }
+  }
+}
+
+int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
+
+// One launch for tensors [i0, i1) of the list.
+template <typename T, typename O, int kTable, bool SCALE>
+int launch_table(const ssa_grad_list_t* l, int i0, int i1, double* part, const float* coef,
+                 cudaStream_t st) {
+  Table<kTable> tab;
+  tab.tensors = 0;
+  int64_t chunks = 0;
+  for (int i = i0; i < i1; ++i) {
+    if (l->sizes[i] == 0) continue;
+    TableEntry& e = tab.t[tab.tensors++];
+    e.in = l->grads[i];
+    e.out = l->outs ? l->outs[i] : const_cast<void*>(l->grads[i]);
+    e.n = l->sizes[i];
+    e.first = (int32_t)chunks;
+    e.vec = ((uintptr_t)e.in | (SCALE ? (uintptr_t)e.out : 0)) % 16 == 0;
+    chunks += chunks_of(e.n);
+  }
+  if (!chunks) return SSA_OK;
+  tab.chunks = (int32_t)chunks;
+  cudaError_t err;
+  if constexpr (SCALE)
+    err = sm100::launch_pdl(scale_kernel<T, O, kTable>, dim3((unsigned)chunks), dim3(kThreads), 0,
+                            st, tab, coef);
+  else
+    err = sm100::launch_pdl(sum_squares_kernel<T, kTable>, dim3((unsigned)chunks), dim3(kThreads), 0,
+                            st, tab, part);
+  if (err != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "grad_clip: %s", cudaGetErrorString(err));
+  note_launches(1);
+  return SSA_OK;
+}
+
+// Walks the list in launches of at most 64 or 768 tensors (the parameter block is copied with
+// every launch: a short list takes the short one).
+template <typename T, typename O, bool SCALE>
+int walk(const ssa_grad_list_t* l, double* part, const float* coef, cudaStream_t st) {
+  const int step = l->count <= 64 ? 64 : 768;
+  int64_t done = 0;
+  const int groups = (l->count + step - 1) / step;
+  for (int k = 0; k < groups; ++k) {
+    const int g = SCALE ? groups - 1 - k : k;
+    const int i0 = g * step, i1 = i0 + step < l->count ? i0 + step : l->count;
+    const int rc = step == 64
+                       ? launch_table<T, O, 64, SCALE>(l, i0, i1, part + done, coef, st)
+                       : launch_table<T, O, 768, SCALE>(l, i0, i1, part + done, coef, st);
+    if (rc != SSA_OK) return rc;
+    if (!SCALE)
+      for (int i = i0; i < i1; ++i) done += chunks_of(l->sizes[i]);
+  }
+  return SSA_OK;
+}
+
+template <bool SCALE>
+int walk_types(const ssa_grad_list_t* l, double* part, const float* coef, cudaStream_t st) {
+  const bool f32 = SCALE && l->out_dtype == SSA_DTYPE_F32;
+  switch (l->dtype) {
+    case SSA_DTYPE_F32:
+      return walk<float, float, SCALE>(l, part, coef, st);
+    case SSA_DTYPE_F16:
+      return f32 ? walk<__half, float, SCALE>(l, part, coef, st)
+                 : walk<__half, __half, SCALE>(l, part, coef, st);
+    default:
+      return f32 ? walk<__nv_bfloat16, float, SCALE>(l, part, coef, st)
+                 : walk<__nv_bfloat16, __nv_bfloat16, SCALE>(l, part, coef, st);
+  }
+}
+
+int64_t total_chunks(const ssa_grad_list_t* l) {
+  int64_t n = 0;
+  for (int i = 0; i < l->count; ++i) n += chunks_of(l->sizes[i]);
+  return n;
+}
+
+int list_check(const ssa_grad_list_t* l, bool outs) {
+  if (!l) return abi_error(SSA_ERR_NULL, "list is NULL");
+  if (l->dtype < SSA_DTYPE_F32 || l->dtype > SSA_DTYPE_BF16)
+    return abi_error(SSA_ERR_UNSUPPORTED, "grad_clip: unsupported dtype %d", l->dtype);
+  if (l->count < 1) return abi_error(SSA_ERR_BAD_SHAPE, "grad_clip: empty list");
+  if (!l->grads || !l->sizes) return abi_error(SSA_ERR_NULL, "grad_clip: grads or sizes is NULL");
+  const uintptr_t es = l->dtype == SSA_DTYPE_F32 ? 4 : 2;
+  for (int i = 0; i < l->count; ++i) {
+    if (l->sizes[i] < 0 || l->sizes[i] > ((int64_t)1 << 40))
+      return abi_error(SSA_ERR_BAD_SHAPE, "grad_clip: tensor %d has %lld elements", i,
+                       (long long)l->sizes[i]);
+    if (l->sizes[i] && !l->grads[i])
+      return abi_error(SSA_ERR_NULL, "grad_clip: tensor %d is NULL", i);
+    if ((uintptr_t)l->grads[i] % es)
+      return abi_error(SSA_ERR_BAD_STRIDE, "grad_clip: tensor %d is not aligned to its type", i);
+  }
+  if (total_chunks(l) > INT32_MAX)
+    return abi_error(SSA_ERR_BAD_SHAPE, "grad_clip: too many elements");
+  if (!outs || !l->outs) return SSA_OK;
+  if (l->out_dtype != l->dtype && l->out_dtype != SSA_DTYPE_F32)
+    return abi_error(SSA_ERR_UNSUPPORTED, "grad_clip: outputs are fp32 or of the gradients' dtype");
+  const uintptr_t eo = l->out_dtype == SSA_DTYPE_F32 ? 4 : 2;
+  for (int i = 0; i < l->count; ++i)
+    if (l->sizes[i] && (!l->outs[i] || (uintptr_t)l->outs[i] % eo))
+      return abi_error(SSA_ERR_NULL, "grad_clip: output %d is NULL or not aligned to its type", i);
+  return SSA_OK;
+}
+
+int first_tensor(const ssa_grad_list_t* l) {
+  for (int i = 0; i < l->count; ++i)
+    if (l->sizes[i]) return i;
+  return -1;
+}
+
+int norm_into(const ssa_grad_list_t* l, double* part, float max_norm, float* norm, float* coef,
+              cudaStream_t st) {
+  int rc = walk_types<false>(l, part, nullptr, st);
+  if (rc != SSA_OK) return rc;
+  const cudaError_t e = sm100::launch_pdl(norm_kernel, dim3(1), dim3(1024), 0, st,
+                                          (const double*)part, total_chunks(l), max_norm, norm, coef);
+  if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "grad_norm: %s", cudaGetErrorString(e));
+  note_launches(1);
+  return SSA_OK;
+}
+
+}  // namespace
+}  // namespace ssa
+
+using namespace ssa;
+
+extern "C" {
+
+size_t ssa_grad_clip_workspace_size(const ssa_grad_list_t* list) {
+  abi_clear_error();
+  if (list_check(list, false) != SSA_OK) return 0;
+  return 256 + sizeof(double) * (size_t)(total_chunks(list) + 1);
+}
+
+int ssa_grad_norm(const ssa_grad_list_t* list, float* norm, void* workspace, size_t workspace_bytes,
+                  void* stream) {
+  abi_clear_error();
+  int rc = list_check(list, false);
+  if (rc != SSA_OK) return rc;
+  if (!norm) return abi_error(SSA_ERR_NULL, "grad_norm: norm is NULL");
+  const size_t need = 256 + sizeof(double) * (size_t)(total_chunks(list) + 1);
+  if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256)
+    return abi_error(SSA_ERR_WORKSPACE, "workspace needs %zu bytes (256-byte aligned), got %zu",
+                     need, workspace_bytes);
+  if ((rc = abi_bind_device(norm, "norm")) != SSA_OK) return rc;
+  return norm_into(list, reinterpret_cast<double*>(static_cast<uint8_t*>(workspace) + 256), 0.f,
+                   norm, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+int ssa_grad_clip(const ssa_grad_list_t* list, float max_norm, float* norm, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+  abi_clear_error();
+  int rc = list_check(list, true);
+  if (rc != SSA_OK) return rc;
+  if (!norm) return abi_error(SSA_ERR_NULL, "grad_clip: norm is NULL");
+  if (!(max_norm >= 0.f))
+    return abi_error(SSA_ERR_BAD_SHAPE, "grad_clip: max_norm must not be negative or NaN");
+  const size_t need = 256 + sizeof(double) * (size_t)(total_chunks(list) + 1);
+  if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256)
+    return abi_error(SSA_ERR_WORKSPACE, "workspace needs %zu bytes (256-byte aligned), got %zu",
+                     need, workspace_bytes);
+  if ((rc = abi_bind_device(norm, "norm")) != SSA_OK) return rc;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  float* coef = reinterpret_cast<float*>(ws);
+  double* part = reinterpret_cast<double*>(ws + 256);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((rc = norm_into(list, part, max_norm, norm, coef, st)) != SSA_OK) return rc;
+  if (first_tensor(list) < 0) return SSA_OK;
+  return walk_types<true>(list, part, coef, st);
+}
+
+}  // extern "C"
