@@ -370,7 +370,7 @@ def run_train(args):
     world, rank, local = dist_setup(args)
     dev = torch.device("cuda", local)
     torch.cuda.set_device(dev)
-    cfg = LT.LucioleConfig()
+    cfg = LT.LucioleConfig(fused=args.fused_ops)
     mbs, seq = 4, 2048
     model = LT.build(cfg, dev, torch.bfloat16, seed=0)
     net = model
@@ -439,7 +439,9 @@ def run_train(args):
             "scaling": "weak", "vs_baseline": None, "dtype": "bf16", "data": "synthetic",
             "config": {"workload": "config5: Llama-style decoder 16 x 2048, 32/8 heads (D=64), "
                                    "SwiGLU 5632, RMSNorm, RoPE 1e4, vocab 65536, SSA attention "
-                                   "kernels; random-init weights, uniform random token ids",
+                                   "kernels; random-init weights, uniform random token ids"
+                                   + ("; rotation, gated feed-forward and loss in the library's "
+                                      "kernels" if cfg.fused else ""),
                        "global_batch": mbs * world, "seq_len": seq,
                        "params": LT.param_count(cfg),
                        "parallelism": f"DDP x{world} (NCCL all-reduce of bf16 grads)"},
@@ -469,6 +471,9 @@ def main():
     ap.add_argument("--config", default="c2", choices=sorted(CONFIGS) + ["c5"],
                     help="c2 (headline), c3, c4: attention workloads; c5: the Luciole-1B "
                          "training step (tokens/s)")
+    ap.add_argument("--fused-ops", action="store_true",
+                    help="c5: rotation, gated feed-forward and LM-head loss through the library's "
+                         "kernels too (LucioleConfig.fused)")
     ap.add_argument("--cp", action="store_true",
                     help="context-parallel ring over the ranks (strong scaling of one sequence; "
                          "use with --config c4 under torchrun)")

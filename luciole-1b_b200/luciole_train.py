@@ -10,9 +10,15 @@ module restates that decoder in plain PyTorch with the same shapes and the same 
     ``SSA.ssa_flash_attention`` (the tcgen05 kernels) with a learnable per-head n and fixed b.
 
 Weights are bf16 for compute with fp32 master copies updated by AdamW (``MasterWeightAdamW``);
-data parallelism is torch DDP over NCCL, one process per GPU. Everything here except the
-attention is ordinary PyTorch (cuBLAS GEMMs, eager elementwise ops): this module is the
+data parallelism is torch DDP over NCCL, one process per GPU. By default everything here except
+the attention is ordinary PyTorch (cuBLAS GEMMs, eager elementwise ops): this module is the
 workload that measures the attention path inside a training step, not a training framework.
+
+``LucioleConfig(fused=True)`` takes the rest of the step's hot operators from the library as well:
+the per-head norm (``qk_norm=True``) and rotation of queries and keys (``SSA.ssa_qk_norm_rope``), the
+gated feed-forward (``SSA.ssa_gated_ffn``) and the LM head with its cross entropy
+(``SSA.ssa_linear_cross_entropy``, which keeps no logits); ``train_step(..., max_grad_norm=...)``
+clips the gradients into the fp32 masters (``SSA.ssa_clip_grad_norm``).
 """
 
 from __future__ import annotations
@@ -39,6 +45,8 @@ class LucioleConfig:
     ssa_n: float = 0.43   # initial per-head n (learnable)
     ssa_b: float = 0.8    # fixed b
     init_std: float = 0.02
+    qk_norm: bool = False  # RMS norm of each query and key head before the rotation
+    fused: bool = False    # rotation, feed-forward and loss through the library's kernels
 
     @property
     def head_dim(self) -> int:
@@ -81,23 +89,43 @@ class DecoderLayer(nn.Module):
         self.down = nn.Linear(cfg.ffn, cfg.hidden, bias=False)
         self.ssa_n = nn.Parameter(torch.full((cfg.heads,), cfg.ssa_n))
         self.register_buffer("ssa_b", torch.tensor(cfg.ssa_b), persistent=True)
+        if cfg.qk_norm:
+            self.q_norm = nn.RMSNorm(D, eps=cfg.norm_eps)
+            self.k_norm = nn.RMSNorm(D, eps=cfg.norm_eps)
         self.attn_fn = attn_fn
 
-    def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+    def project(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> tuple:
+        """Normed (with qk_norm) and rotated queries and keys, and values: [B, S, H, D] each."""
         cfg = self.cfg
-        Bsz, S, _ = x.shape
         D, H, Hkv = cfg.head_dim, cfg.heads, cfg.kv_heads
-        qkv = self.qkv(self.attn_norm(x)).view(Bsz, S, H + 2 * Hkv, D)
-        q = apply_rope(qkv[:, :, :H], cos, sin)
-        k = apply_rope(qkv[:, :, H:H + Hkv], cos, sin)
-        v = qkv[:, :, H + Hkv:]
+        qkv = self.qkv(self.attn_norm(x))
+        if cfg.fused:
+            from SSA.ssa_qk_norm_rope import ssa_qk_norm_rope
+            wq, wk = (self.q_norm.weight, self.k_norm.weight) if cfg.qk_norm else (None, None)
+            return ssa_qk_norm_rope(qkv, H, Hkv, cos, sin, wq, wk, cfg.norm_eps)
+        qkv = qkv.view(*x.shape[:2], H + 2 * Hkv, D)
+        q, k, v = qkv[:, :, :H], qkv[:, :, H:H + Hkv], qkv[:, :, H + Hkv:]
+        if cfg.qk_norm:
+            q, k = self.q_norm(q), self.k_norm(k)
+        return apply_rope(q, cos, sin), apply_rope(k, cos, sin), v
+
+    def feed_forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.cfg.fused:
+            from SSA.ssa_gated_ffn import ssa_gated_ffn
+            return self.down(ssa_gated_ffn(self.mlp_norm(x), self.gate_up.weight))
+        g, u = self.gate_up(self.mlp_norm(x)).chunk(2, dim=-1)
+        return self.down(F.silu(g) * u)
+
+    def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+        Bsz, S, _ = x.shape
+        D, H = self.cfg.head_dim, self.cfg.heads
+        q, k, v = self.project(x, cos, sin)
         # [B, S, H, D] -> [B, H, S, D] views: the kernels read the strides, and the output
         # keeps q's layout, so the permute back below is free.
         o = self.attn_fn(q.permute(0, 2, 1, 3), k.permute(0, 2, 1, 3), v.permute(0, 2, 1, 3),
                          D ** -0.5, self.ssa_n, self.ssa_b)
         x = x + self.o_proj(o.permute(0, 2, 1, 3).reshape(Bsz, S, H * D))
-        g, u = self.gate_up(self.mlp_norm(x)).chunk(2, dim=-1)
-        return x + self.down(F.silu(g) * u)
+        return x + self.feed_forward(x)
 
 
 class LucioleDecoder(nn.Module):
@@ -127,15 +155,25 @@ class LucioleDecoder(nn.Module):
             self._rope[key] = rope_tables(seq, self.cfg.head_dim, self.cfg.rope_theta, device)
         return self._rope[key]
 
-    def forward(self, tokens: torch.Tensor) -> torch.Tensor:
-        """tokens [B, S] int64 -> logits [B, S, vocab] (in the weights' dtype)."""
+    def hidden(self, tokens: torch.Tensor) -> torch.Tensor:
+        """tokens [B, S] int64 -> the LM head's input [B, S, hidden]."""
         cos, sin = self.rope(tokens.shape[1], tokens.device)
         x = self.embed(tokens)
         for layer in self.layers:
             x = layer(x, cos, sin)
-        return self.lm_head(self.norm(x))
+        return self.norm(x)
+
+    def forward(self, tokens: torch.Tensor, targets: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """tokens [B, S] int64 -> logits [B, S, vocab] (in the weights' dtype), or with targets
+        [B, S] the mean cross entropy."""
+        if targets is not None:
+            return self.loss(tokens, targets)
+        return self.lm_head(self.hidden(tokens))
 
     def loss(self, tokens: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+        if self.cfg.fused:
+            from SSA.ssa_cross_entropy import ssa_linear_cross_entropy
+            return ssa_linear_cross_entropy(self.hidden(tokens), self.lm_head.weight, targets)
         logits = self(tokens)
         return F.cross_entropy(logits.float().view(-1, logits.shape[-1]), targets.reshape(-1))
 
@@ -153,17 +191,27 @@ class MasterWeightAdamW:
                                      weight_decay=weight_decay, fused=fused)
 
     @torch.no_grad()
-    def step(self) -> None:
+    def step(self, max_grad_norm: Optional[float] = None) -> Optional[torch.Tensor]:
+        """One update. With max_grad_norm the gradients are clipped to that global 2-norm on their
+        way into the fp32 masters, and the norm before clipping is returned (on the device)."""
+        have = [(p, m) for p, m in zip(self.params, self.master) if p.grad is not None]
         for p, m in zip(self.params, self.master):
             if p.grad is None:
                 m.grad = None
-                continue
-            if m.grad is None:
+            elif m.grad is None:
                 m.grad = torch.empty_like(m)
-            m.grad.copy_(p.grad)
+        norm = None
+        if max_grad_norm is None:
+            for p, m in have:
+                m.grad.copy_(p.grad)
+        else:
+            from SSA.ssa_grad_clip import ssa_clip_grad_norm
+            norm = ssa_clip_grad_norm([p.grad for p, _ in have], max_grad_norm,
+                                      out=[m.grad for _, m in have])
         self.opt.step()
         for p, m in zip(self.params, self.master):
             p.copy_(m)
+        return norm
 
     def zero_grad(self) -> None:
         for p in self.params:
@@ -182,13 +230,17 @@ def build(cfg: LucioleConfig, device, dtype=torch.bfloat16, seed: int = 0,
 
 
 def train_step(model: nn.Module, opt: MasterWeightAdamW, tokens: torch.Tensor,
-               targets: torch.Tensor) -> torch.Tensor:
+               targets: torch.Tensor, max_grad_norm: Optional[float] = None) -> torch.Tensor:
     """One optimizer step on one micro-batch: forward, loss, backward (DDP all-reduces the
-    gradients when `model` is wrapped), AdamW on the fp32 masters. Returns the loss (device)."""
-    logits = model(tokens)
-    loss = F.cross_entropy(logits.float().view(-1, logits.shape[-1]), targets.reshape(-1))
+    gradients when `model` is wrapped), AdamW on the fp32 masters, with max_grad_norm on gradients
+    clipped to that global norm. Returns the loss (device)."""
+    if getattr(model, "module", model).cfg.fused:
+        loss = model(tokens, targets)
+    else:
+        logits = model(tokens)
+        loss = F.cross_entropy(logits.float().view(-1, logits.shape[-1]), targets.reshape(-1))
     loss.backward()
-    opt.step()
+    opt.step(max_grad_norm)
     opt.zero_grad()
     return loss.detach()
 
@@ -196,7 +248,8 @@ def train_step(model: nn.Module, opt: MasterWeightAdamW, tokens: torch.Tensor,
 def param_count(cfg: LucioleConfig) -> int:
     D = cfg.head_dim
     per_layer = (cfg.hidden * (cfg.heads + 2 * cfg.kv_heads) * D + cfg.heads * D * cfg.hidden
-                 + 3 * cfg.hidden * cfg.ffn + 2 * cfg.hidden + cfg.heads)
+                 + 3 * cfg.hidden * cfg.ffn + 2 * cfg.hidden + cfg.heads
+                 + (2 * D if cfg.qk_norm else 0))
     return cfg.vocab * cfg.hidden * 2 + cfg.layers * per_layer + cfg.hidden
 
 
