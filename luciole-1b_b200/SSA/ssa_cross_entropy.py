@@ -27,40 +27,45 @@ def _problem(x, w, t, ignore_index, reduction):
                             t.data_ptr(), ignore_index, reduction)
 
 
+def _forward(hidden, weight, targets, ignore_index, code):
+    """The loss, and what the backward needs: x, w, targets, the rows' lse, the rows counted."""
+    dev = hidden.device
+    x = _lib.tma_matrix(hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1]))
+    w = _lib.tma_matrix(weight)
+    t = targets.reshape(-1).to(torch.int64).contiguous()
+    n = x.shape[0]
+    stats = torch.empty(n + 1, device=dev, dtype=torch.float32)  # lse of the rows, their count
+    if n == 0:
+        loss = stats.new_empty(targets.shape) if code == 0 else \
+            stats.new_full((), float("nan") if code == 1 else 0.0)
+    else:
+        loss = torch.empty(targets.shape if code == 0 else (), device=dev, dtype=torch.float32)
+        lib = _lib.load()
+        prob = _problem(x, w, t, ignore_index, code)
+        ws = _lib.workspace(lib.ssa_linear_ce_fwd_workspace_size(ctypes.byref(prob)), dev)
+        lse = stats.data_ptr()
+        with _lib.device_guard(dev):
+            rc = lib.ssa_linear_ce_fwd(ctypes.byref(prob), loss.data_ptr(), lse, lse + 4 * n,
+                                       ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev))
+        _lib.check(rc)
+    return loss, x, w, t, stats
+
+
 class SSALinearCrossEntropyFunc(Function):
     """loss = reduce(logsumexp(x W^T) - (x W^T)[target]); gradients of x and W."""
 
     @staticmethod
     def forward(ctx, hidden, weight, targets, ignore_index, reduction):
         code = _REDUCTIONS[reduction]
-        dev = hidden.device
-        x = _lib.tma_matrix(hidden.reshape(-1, hidden.shape[-1]))
-        w = _lib.tma_matrix(weight)
-        t = targets.reshape(-1).to(torch.int64).contiguous()
-        n = x.shape[0]
-        lse = torch.empty(n, device=dev, dtype=torch.float32)
-        count = torch.empty((), device=dev, dtype=torch.float32)
-        if n == 0:
-            loss = lse.new_empty(targets.shape) if code == 0 else \
-                lse.new_full((), float("nan") if code == 1 else 0.0)
-        else:
-            loss = torch.empty(targets.shape if code == 0 else (), device=dev, dtype=torch.float32)
-            lib = _lib.load()
-            prob = _problem(x, w, t, ignore_index, code)
-            ws = _lib.workspace(lib.ssa_linear_ce_fwd_workspace_size(ctypes.byref(prob)), dev)
-            with _lib.device_guard(dev):
-                rc = lib.ssa_linear_ce_fwd(ctypes.byref(prob), loss.data_ptr(), lse.data_ptr(),
-                                           count.data_ptr(), ws.data_ptr(), ws.numel(),
-                                           _lib.stream_ptr(dev))
-            _lib.check(rc)
-        ctx.save_for_backward(x, w, t, lse, count)
+        loss, *saved = _forward(hidden, weight, targets, ignore_index, code)
+        ctx.save_for_backward(*saved)
         ctx.args = (ignore_index, code, hidden.shape)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_loss):
-        x, w, t, lse, count = ctx.saved_tensors
+        x, w, t, stats = ctx.saved_tensors
         ignore_index, code, shape = ctx.args
         need_x, need_w = ctx.needs_input_grad[:2]
         dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need_x else None
@@ -73,9 +78,10 @@ class SSALinearCrossEntropyFunc(Function):
             g = grad_loss.reshape(-1).to(torch.float32).contiguous()
             prob = _problem(x, w, t, ignore_index, code)
             ws = _lib.workspace(lib.ssa_linear_ce_bwd_workspace_size(ctypes.byref(prob)), x.device)
+            lse = stats.data_ptr()
             with _lib.device_guard(x.device):
                 rc = lib.ssa_linear_ce_bwd(
-                    ctypes.byref(prob), lse.data_ptr(), count.data_ptr(), g.data_ptr(),
+                    ctypes.byref(prob), lse, lse + 4 * x.shape[0], g.data_ptr(),
                     dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None,
                     ws.data_ptr(), ws.numel(), _lib.stream_ptr(x.device))
             _lib.check(rc)
@@ -113,4 +119,6 @@ def ssa_linear_cross_entropy(hidden, weight, targets, ignore_index=-100, reducti
         raise ValueError(f"targets must be int64 or int32, got {targets.dtype}")
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
-    return SSALinearCrossEntropyFunc.apply(hidden, weight, targets, int(ignore_index), reduction)
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return SSALinearCrossEntropyFunc.apply(hidden, weight, targets, int(ignore_index), reduction)
+    return _forward(hidden, weight, targets, int(ignore_index), _REDUCTIONS[reduction])[0]

@@ -23,23 +23,28 @@ def _problem(x, w):
                             x.data_ptr(), _lib.row_stride(x), w.data_ptr(), _lib.row_stride(w))
 
 
+def _forward(inp, weight):
+    """h and the matrices it was computed from."""
+    dev = inp.device
+    x = _lib.tma_matrix(inp if inp.dim() == 2 else inp.reshape(-1, inp.shape[-1]))
+    w = _lib.tma_matrix(weight)
+    f = w.shape[0] // 2
+    h = torch.empty(*inp.shape[:-1], f, device=dev, dtype=inp.dtype)
+    if x.shape[0]:
+        prob = _problem(x, w)
+        with _lib.device_guard(dev):
+            rc = _lib.load().ssa_gated_ffn_fwd(ctypes.byref(prob), h.data_ptr(), f,
+                                               _lib.stream_ptr(dev))
+        _lib.check(rc)
+    return h, x, w
+
+
 class SSAGatedFFNFunc(Function):
     """h = silu(x Wg^T) * (x Wu^T); gradients of x and [Wg; Wu]."""
 
     @staticmethod
     def forward(ctx, inp, weight):
-        dev = inp.device
-        x = _lib.tma_matrix(inp.reshape(-1, inp.shape[-1]))
-        w = _lib.tma_matrix(weight)
-        f = w.shape[0] // 2
-        h = torch.empty(*inp.shape[:-1], f, device=dev, dtype=inp.dtype)
-        if x.shape[0]:
-            lib = _lib.load()
-            prob = _problem(x, w)
-            with _lib.device_guard(dev):
-                rc = lib.ssa_gated_ffn_fwd(ctypes.byref(prob), h.data_ptr(), f,
-                                           _lib.stream_ptr(dev))
-            _lib.check(rc)
+        h, x, w = _forward(inp, weight)
         ctx.save_for_backward(x, w)
         ctx.shape = inp.shape
         return h
@@ -56,7 +61,7 @@ class SSAGatedFFNFunc(Function):
                 dw.zero_()
         elif need_x or need_w:
             lib = _lib.load()
-            dh = grad.reshape(-1, w.shape[0] // 2).to(x.dtype)
+            dh = grad.reshape(-1, w.shape[0] // 2)
             if dh.stride(1) != 1 or _lib.row_stride(dh) < dh.shape[1]:
                 dh = dh.contiguous()
             prob = _problem(x, w)
@@ -93,4 +98,6 @@ def ssa_gated_ffn(x, weight_gate_up):
                          f"{tuple(x.shape)}")
     if x.shape[-1] < 8 or x.shape[-1] % 8:
         raise ValueError(f"hidden size {x.shape[-1]} must be a positive multiple of 8")
-    return SSAGatedFFNFunc.apply(x, w)
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+        return SSAGatedFFNFunc.apply(x, w)
+    return _forward(x, w)[0]

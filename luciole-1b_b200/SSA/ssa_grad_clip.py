@@ -9,9 +9,9 @@ Neither synchronises with the host.
 from __future__ import annotations
 
 import ctypes
+from array import array
 from typing import Optional, Sequence
 
-import numpy as np
 import torch
 
 from . import _lib
@@ -19,43 +19,56 @@ from . import _lib
 __all__ = ["ssa_grad_norm", "ssa_clip_grad_norm"]
 
 
-def _check_list(ts, what, device=None, dtype=None):
-    """A list of CUDA tensors of one device and one floating dtype."""
+def _check_list(ts, what, device=None):
+    """A list of dense CUDA tensors of one device and one floating dtype."""
     ts = list(ts)
     for t in ts:
-        if not isinstance(t, torch.Tensor) or t.layout != torch.strided:
+        if not isinstance(t, torch.Tensor) or t.layout is not torch.strided:
             raise ValueError(f"{what} must be dense tensors")
-        device = t.device if device is None else device
-        dtype = t.dtype if dtype is None else dtype
-        if t.device != device or t.dtype != dtype:
-            raise ValueError(f"{what} must be on one device and of one dtype, got {t.dtype} on "
-                             f"{t.device} beside {dtype} on {device}")
-    if ts and device.type != "cuda":
+    dtypes = {t.dtype for t in ts}
+    devices = {t.device for t in ts}
+    if device is not None and ts:
+        devices.add(device)
+    if len(dtypes) > 1 or len(devices) > 1:
+        raise ValueError(f"{what} must be on one device and of one dtype, got {dtypes} on {devices}")
+    if ts and not ts[0].is_cuda:
         raise ValueError(f"{what} must be CUDA tensors (there is no CPU path)")
-    if ts and dtype not in _lib.DTYPE_CODES:
-        raise ValueError(f"{what} must be fp32, fp16 or bf16, got {dtype}")
+    if ts and ts[0].dtype not in _lib.DTYPE_CODES:
+        raise ValueError(f"{what} must be fp32, fp16 or bf16, got {ts[0].dtype}")
     return ts
 
 
-def _overlap(ptrs, sizes, item):
-    """Whether two of the (contiguous) tensors share memory."""
-    used = sizes > 0
-    order = np.argsort(ptrs[used], kind="stable")
-    start, nbytes = ptrs[used][order], sizes[used][order] * item
-    return bool((start[1:] < start[:-1] + nbytes[:-1]).any())
+def _pointers(ts):
+    return array("q", [t.data_ptr() for t in ts])
 
 
-def _arrays(ts):
-    n = len(ts)
-    return (np.fromiter((t.data_ptr() for t in ts), np.int64, n),
-            np.fromiter((t.numel() for t in ts), np.int64, n))
+def _run(grads, held, max_norm=None, out=None):
+    """The norm (max_norm None) or the clipping of the contiguous tensors `held`."""
+    dev = grads[0].device
+    ptrs, sizes = _pointers(held), array("q", [t.numel() for t in held])
+    optrs = _pointers(out) if out is not None else None
+    lst = _lib.SsaGradList(
+        _lib.DTYPE_CODES[grads[0].dtype], len(sizes), ptrs.buffer_info()[0], sizes.buffer_info()[0],
+        optrs.buffer_info()[0] if out is not None else None,
+        _lib.DTYPE_CODES[(out or grads)[0].dtype])
+    lib = _lib.load()
+    norm = torch.empty((), device=dev, dtype=torch.float32)
+    ws = _lib.workspace(lib.ssa_grad_clip_workspace_size(ctypes.byref(lst)), dev)
+    with _lib.device_guard(dev):
+        st = _lib.stream_ptr(dev)
+        if max_norm is None:
+            rc = lib.ssa_grad_norm(ctypes.byref(lst), norm.data_ptr(), ws.data_ptr(), ws.numel(), st)
+        else:
+            rc = lib.ssa_grad_clip(ctypes.byref(lst), max_norm, norm.data_ptr(), ws.data_ptr(),
+                                   ws.numel(), st)
+    _lib.check(rc)
+    return norm
 
 
-def _list(ptrs, sizes, dtype, outs=None, out_dtype=None):
-    return _lib.SsaGradList(
-        _lib.DTYPE_CODES[dtype], len(sizes), ptrs.ctypes.data, sizes.ctypes.data,
-        outs.ctypes.data if outs is not None else None,
-        _lib.DTYPE_CODES[out_dtype if out_dtype is not None else dtype])
+def _contiguous(grads):
+    if all([t.is_contiguous() for t in grads]):
+        return grads
+    return [t if t.is_contiguous() else t.detach().contiguous() for t in grads]
 
 
 def ssa_grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
@@ -63,23 +76,9 @@ def ssa_grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
     device), as an fp32 scalar on their device. Squares are summed in 64 bits in a fixed order;
     infinities and NaN in a gradient come through. An empty list gives 0 on the current device."""
     grads = _check_list(grads, "grads")
-    if not grads:
-        return torch.zeros((), device="cuda")
-    dev = grads[0].device
-    held = [t if t.is_contiguous() else t.contiguous() for t in grads]
-    ptrs, sizes = _arrays(held)
-    lib = _lib.load()
-    lst = _list(ptrs, sizes, grads[0].dtype)
-    norm = torch.empty((), device=dev, dtype=torch.float32)
-    ws = _lib.workspace(lib.ssa_grad_clip_workspace_size(ctypes.byref(lst)), dev)
-    with _lib.device_guard(dev):
-        rc = lib.ssa_grad_norm(ctypes.byref(lst), norm.data_ptr(), ws.data_ptr(), ws.numel(),
-                               _lib.stream_ptr(dev))
-    _lib.check(rc)
-    return norm
+    return _run(grads, _contiguous(grads)) if grads else torch.zeros((), device="cuda")
 
 
-@torch.no_grad()
 def ssa_clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float,
                        out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """Scale ``grads`` so that their 2-norm is at most ``max_norm``; returns the norm before that
@@ -89,7 +88,8 @@ def ssa_clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float,
     place, or, with ``out``, into contiguous tensors of the same sizes that are fp32 or of the
     gradients' dtype (``grads`` then stay as they are). As with torch's clipping, a NaN norm makes
     every gradient NaN and an infinite one makes the finite ones 0. grads: one dtype (fp32, fp16,
-    bf16), one CUDA device; tensors that are written must not share memory."""
+    bf16), one CUDA device; tensors that are written must not share memory, with one another or
+    with gradients that are read."""
     grads = _check_list(grads, "grads")
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
@@ -108,47 +108,16 @@ def ssa_clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float,
             raise ValueError(f"out must be fp32 or of the gradients' dtype, got {out[0].dtype}")
     if not grads:
         return torch.zeros((), device="cuda")
-    dev, dtype = grads[0].device, grads[0].dtype
-    held = [t if t.is_contiguous() else t.contiguous() for t in grads]
-    ptrs, sizes = _arrays(held)
-    optrs, out_dtype = None, dtype
-    if out is None:
-        strided = [(g, h) for g, h in zip(grads, held) if g is not h]
-        item = held[0].element_size()
-        if _overlap(ptrs, sizes, item) or any(n > 1 and s == 0 for g, _ in strided
-                                              for n, s in zip(g.shape, g.stride())):
-            raise ValueError("gradients that are scaled in place must not share memory")
-    else:
-        strided = []
-        optrs, _ = _arrays(out)
-        out_dtype = out[0].dtype
-        item = out[0].element_size()
-        both = np.concatenate([ptrs, optrs])
-        nbytes = np.concatenate([sizes * held[0].element_size(), sizes * item])
-        same = item == held[0].element_size() and bool((ptrs == optrs).all())
-        if _overlap(optrs, sizes, item) or (not same and _overlap_between(both, nbytes, len(out))):
-            raise ValueError("out must not share memory, neither within itself nor with grads")
-    lib = _lib.load()
-    lst = _list(ptrs, sizes, dtype, optrs, out_dtype)
-    norm = torch.empty((), device=dev, dtype=torch.float32)
-    ws = _lib.workspace(lib.ssa_grad_clip_workspace_size(ctypes.byref(lst)), dev)
-    with _lib.device_guard(dev):
-        rc = lib.ssa_grad_clip(ctypes.byref(lst), max_norm, norm.data_ptr(), ws.data_ptr(),
-                               ws.numel(), _lib.stream_ptr(dev))
-    _lib.check(rc)
+    held = _contiguous(grads)
+    back = [] if out is not None or held is grads else \
+        [(g, h) for g, h in zip(grads, held) if g is not h]
+    if any(n > 1 and s == 0 for g, _ in back for n, s in zip(g.shape, g.stride())):
+        raise ValueError("gradients that are scaled in place must not share memory")
+    norm = _run(grads, held, max_norm, out)
     torch.autograd.graph.increment_version(
         [t for t in (held if out is None else out) if not t.is_inference()])
-    for g, h in strided:
-        g.copy_(h)
+    if back:
+        with torch.no_grad():
+            for g, h in back:
+                g.copy_(h)
     return norm
-
-
-def _overlap_between(ptrs, nbytes, n):
-    """Whether one of the last n ranges meets one of the others (which may share among themselves)."""
-    start, end = ptrs[:-n], ptrs[:-n] + nbytes[:-n]
-    used = nbytes[-n:] > 0
-    order = np.argsort(ptrs[-n:][used], kind="stable")
-    os_, oe = ptrs[-n:][used][order], (ptrs[-n:] + nbytes[-n:])[used][order]
-    at = np.searchsorted(os_, end, side="left")  # outputs that begin before a gradient ends
-    top = np.concatenate([[0], np.maximum.accumulate(oe)])
-    return bool(((top[at] > start) & (nbytes[:-n] > 0)).any())

@@ -40,35 +40,40 @@ def _problem(x, hq, hkv, cos, sin, pos, pos_stride, wq, wk, eps):
         _lib.DTYPE_CODES[wq.dtype if wq is not None else x.dtype], eps)
 
 
+def _forward(qkv, q_weight, k_weight, cos, sin, positions, hq, hkv, eps):
+    """q, k, v, the tensors the backward needs, and the stride between sequences' positions."""
+    d = cos.shape[1]
+    lead = qkv.shape[:-1]
+    heads = qkv.unflatten(-1, (hq + 2 * hkv, d))
+    x = _aligned(heads if len(lead) == 2 else heads.unsqueeze(0))
+    cos, sin = _lib.table(cos), _lib.table(sin)
+    pos, pos_stride = positions, 0
+    if pos is not None:
+        pos = pos.contiguous()
+        pos_stride = lead[1] if pos.dim() == 2 else 0
+    wq = q_weight.contiguous() if q_weight is not None else None
+    wk = k_weight.contiguous() if k_weight is not None else None
+    q = torch.empty(*lead, hq, d, device=qkv.device, dtype=qkv.dtype)
+    k = torch.empty(*lead, hkv, d, device=qkv.device, dtype=qkv.dtype)
+    if q.numel():
+        prob = _problem(x, hq, hkv, cos, sin, pos, pos_stride, wq, wk, eps)
+        with _lib.device_guard(qkv.device):
+            rc = _lib.load().ssa_qk_rope_fwd(ctypes.byref(prob), q.data_ptr(), k.data_ptr(),
+                                             _lib.stream_ptr(qkv.device))
+        _lib.check(rc)
+    return (q, k, heads[..., hq + hkv:, :]), (x, cos, sin, pos, wq, wk), pos_stride
+
+
 class SSAQKNormRopeFunc(Function):
     """(q, k, v) of a packed qkv projection; gradients of qkv and the norm weights."""
 
     @staticmethod
     def forward(ctx, qkv, q_weight, k_weight, cos, sin, positions, hq, hkv, eps):
-        d = cos.shape[1]
-        lead = qkv.shape[:-1]
-        heads = qkv.unflatten(-1, (hq + 2 * hkv, d))
-        x = _aligned(heads if len(lead) == 2 else heads.unsqueeze(0))
-        cos, sin = _lib.table(cos), _lib.table(sin)
-        pos, pos_stride = positions, 0
-        if pos is not None:
-            pos = pos.contiguous()
-            pos_stride = lead[1] if pos.dim() == 2 else 0
-        wq = q_weight.contiguous() if q_weight is not None else None
-        wk = k_weight.contiguous() if k_weight is not None else None
-        q = torch.empty(*lead, hq, d, device=qkv.device, dtype=qkv.dtype)
-        k = torch.empty(*lead, hkv, d, device=qkv.device, dtype=qkv.dtype)
-        if q.numel():
-            lib = _lib.load()
-            prob = _problem(x, hq, hkv, cos, sin, pos, pos_stride, wq, wk, eps)
-            with _lib.device_guard(qkv.device):
-                rc = lib.ssa_qk_rope_fwd(ctypes.byref(prob), q.data_ptr(), k.data_ptr(),
-                                         _lib.stream_ptr(qkv.device))
-            _lib.check(rc)
+        out, saved, pos_stride = _forward(qkv, q_weight, k_weight, cos, sin, positions, hq, hkv, eps)
         # without the norm the rotation's gradient needs no x
-        ctx.save_for_backward(x if wq is not None else None, cos, sin, pos, wq, wk)
+        ctx.save_for_backward(saved[0] if q_weight is not None else None, *saved[1:])
         ctx.args = (hq, hkv, eps, pos_stride, qkv.shape)
-        return q, k, heads[..., hq + hkv:, :]
+        return out
 
     @staticmethod
     @once_differentiable
@@ -110,13 +115,16 @@ def ssa_qk_norm_rope(qkv, num_heads, num_kv_heads, cos, sin, q_weight=None, k_we
     sequence has position s), or int32 / int64 of shape [S], [B, S] or [T], an index into the tables;
     one outside them gives NaN (nothing is read out of range). Returns q [..., Hq, D], k [..., Hkv, D]
     and v [..., Hkv, D], the last a view of qkv. Layouts the kernels cannot address are copied."""
-    tensors = [t for t in (qkv, cos, sin, q_weight, k_weight, positions) if t is not None]
-    if not all(isinstance(t, torch.Tensor) for t in tensors):
-        raise ValueError("qkv, cos, sin, the weights and positions must be tensors")
-    if not all(t.is_cuda for t in tensors):
-        raise ValueError("all tensors must be CUDA tensors (there is no CPU path)")
-    if any(t.device != qkv.device for t in tensors):
-        raise ValueError("all tensors must be on one device")
+    dev = qkv.device if isinstance(qkv, torch.Tensor) else None
+    for t in (qkv, cos, sin, q_weight, k_weight, positions):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise ValueError("qkv, cos, sin, the weights and positions must be tensors")
+        if not t.is_cuda or t.device != dev:
+            raise ValueError("all tensors must be CUDA tensors (there is no CPU path) on one device")
+    if qkv is None or cos is None or sin is None:
+        raise ValueError("qkv, cos and sin are required")
     if qkv.dtype not in _lib.DTYPE_CODES:
         raise ValueError(f"unsupported dtype {qkv.dtype}")
     hq, hkv = int(num_heads), int(num_kv_heads)
@@ -146,4 +154,8 @@ def ssa_qk_norm_rope(qkv, num_heads, num_kv_heads, cos, sin, q_weight=None, k_we
             raise ValueError(f"positions {tuple(positions.shape)} do not fit rows {tuple(lead)}")
         if cos.shape[0] < 1:
             raise ValueError("empty cos / sin tables")
-    return SSAQKNormRopeFunc.apply(qkv, q_weight, k_weight, cos, sin, positions, hq, hkv, float(eps))
+    if torch.is_grad_enabled() and (qkv.requires_grad or (
+            q_weight is not None and (q_weight.requires_grad or k_weight.requires_grad))):
+        return SSAQKNormRopeFunc.apply(qkv, q_weight, k_weight, cos, sin, positions, hq, hkv,
+                                       float(eps))
+    return _forward(qkv, q_weight, k_weight, cos, sin, positions, hq, hkv, float(eps))[0]

@@ -11,7 +11,10 @@
 // Squares are added in fp32 over a thread's few elements of a chunk and in fp64 from there on, in
 // a fixed order: the norm is the same from run to run. A thread whose fp32 sum overflowed, or is so
 // small that squares may have been lost, adds its elements again in fp64.
+#include <algorithm>
 #include <cmath>
+#include <exception>
+#include <vector>
 
 #include "ssa_internal.h"
 #include "ssa_sm100.cuh"
@@ -270,6 +273,40 @@ int64_t total_chunks(const ssa_grad_list_t* l) {
   return n;
 }
 
+struct Range {
+  uintptr_t from, to;
+  int written, index;
+};
+
+// Two blocks may not write the same element, nor one write what another reads: a written tensor
+// meets no other tensor. (An output may be its own gradient.)
+int check_ranges(const ssa_grad_list_t* l) {
+  const size_t es = l->dtype == SSA_DTYPE_F32 ? 4 : 2;
+  const size_t eo = l->outs && l->out_dtype == SSA_DTYPE_F32 ? 4 : es;
+  try {
+    std::vector<Range> r;
+    r.reserve(2 * (size_t)l->count);
+    for (int i = 0; i < l->count; ++i) {
+      if (!l->sizes[i]) continue;
+      const uintptr_t in = (uintptr_t)l->grads[i], out = l->outs ? (uintptr_t)l->outs[i] : in;
+      r.push_back(Range{out, out + eo * (size_t)l->sizes[i], 1, i});
+      if (out != in || eo != es) r.push_back(Range{in, in + es * (size_t)l->sizes[i], 0, i});
+    }
+    std::sort(r.begin(), r.end(), [](const Range& a, const Range& b) { return a.from < b.from; });
+    uintptr_t end_written = 0, end_any = 0;
+    for (const Range& x : r) {
+      if (x.from < end_written || (x.written && x.from < end_any))
+        return abi_error(SSA_ERR_BAD_SHAPE, "grad_clip: tensors that are written must not share "
+                         "memory with another (tensor %d)", x.index);
+      if (x.to > end_any) end_any = x.to;
+      if (x.written && x.to > end_written) end_written = x.to;
+    }
+  } catch (const std::exception& e) {
+    return abi_error(SSA_ERR_CUDA, "grad_clip: %s", e.what());
+  }
+  return SSA_OK;
+}
+
 int list_check(const ssa_grad_list_t* l, bool outs) {
   if (!l) return abi_error(SSA_ERR_NULL, "list is NULL");
   if (l->dtype < SSA_DTYPE_F32 || l->dtype > SSA_DTYPE_BF16)
@@ -288,14 +325,15 @@ int list_check(const ssa_grad_list_t* l, bool outs) {
   }
   if (total_chunks(l) > INT32_MAX)
     return abi_error(SSA_ERR_BAD_SHAPE, "grad_clip: too many elements");
-  if (!outs || !l->outs) return SSA_OK;
+  if (!outs) return SSA_OK;
+  if (!l->outs) return check_ranges(l);
   if (l->out_dtype != l->dtype && l->out_dtype != SSA_DTYPE_F32)
     return abi_error(SSA_ERR_UNSUPPORTED, "grad_clip: outputs are fp32 or of the gradients' dtype");
   const uintptr_t eo = l->out_dtype == SSA_DTYPE_F32 ? 4 : 2;
   for (int i = 0; i < l->count; ++i)
     if (l->sizes[i] && (!l->outs[i] || (uintptr_t)l->outs[i] % eo))
       return abi_error(SSA_ERR_NULL, "grad_clip: output %d is NULL or not aligned to its type", i);
-  return SSA_OK;
+  return check_ranges(l);
 }
 
 int first_tensor(const ssa_grad_list_t* l) {
