@@ -29,34 +29,19 @@ struct FfnFwdArgs {
 template <int BN, bool BF16>
 struct EpiFfnFwd {
   using Args = FfnFwdArgs;
-  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, int r,
-                                              const AccReader& rd) {
-    const int row = w.mt * 128 + r;
-    const int col0 = w.nt * (BN / 2);
-    T* hrow = reinterpret_cast<T*>(a.h) + (int64_t)row * a.ldh;
+  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, const EpiCtx& e) {
+    const int off = e.half * (BN / 4);  // a warp's gate columns; the up projection's are BN / 2 on
+    uint16_t* base = reinterpret_cast<uint16_t*>(a.h) + (int64_t)e.row0 * a.ldh;
 #pragma unroll 1
-    for (int c = 0; c < BN / 2; c += 32) {
-      if (col0 + c >= a.ffn) break;
+    for (int c = 0; c < BN / 4; c += 32) {
+      const int col = w.nt * (BN / 2) + off + c;
+      if (col >= a.ffn) break;
       float g[32], u[32];
-      rd(c, g);
-      rd(BN / 2 + c, u);
-      if (row >= a.rows) continue;
+      e.read(off + c, g);
+      e.read(BN / 2 + off + c, u);
 #pragma unroll
       for (int i = 0; i < 32; ++i) g[i] = g[i] * sigmoid_approx(g[i]) * u[i];
-#pragma unroll
-      for (int i = 0; i < 32; i += 8) {
-        const int col = col0 + c + i;
-        if (a.vec && col + 8 <= a.ffn) {
-          *reinterpret_cast<uint4*>(hrow + col) =
-              make_uint4(pack2<BF16>(g[i], g[i + 1]), pack2<BF16>(g[i + 2], g[i + 3]),
-                         pack2<BF16>(g[i + 4], g[i + 5]), pack2<BF16>(g[i + 6], g[i + 7]));
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (col + j < a.ffn) hrow[col + j] = from_f32<T>(g[i + j]);
-        }
-      }
+      store_block16<BF16>(e, g, base, a.ldh, a.rows - e.row0, col, a.ffn, a.vec);
     }
   }
 };
@@ -73,46 +58,48 @@ template <int BN, bool BF16>
 struct EpiFfnBwd {
   using Args = FfnBwdArgs;
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, int r,
-                                              const AccReader& rd) {
-    const int row = w.mt * 128 + r;
-    const int col0 = w.nt * (BN / 2);
-    const T* dhrow = reinterpret_cast<const T*>(a.dh) + (int64_t)row * a.lddh;
-    T* drow = reinterpret_cast<T*>(a.d) + (int64_t)row * (2 * a.wide);
+  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, const EpiCtx& e) {
+    const int off = e.half * (BN / 4);
+    const int rows = a.rows - e.row0;
+    const uint16_t* dhbase = reinterpret_cast<const uint16_t*>(a.dh) + (int64_t)e.row0 * a.lddh;
+    uint16_t* base = reinterpret_cast<uint16_t*>(a.d) + (int64_t)e.row0 * (2 * a.wide);
+    uint8_t* in = e.exch + 2048;  // dh's block; the first half of the buffer carries d's
 #pragma unroll 1
-    for (int c = 0; c < BN / 2; c += 32) {
-      float g[32], u[32];
-      rd(c, g);
-      rd(BN / 2 + c, u);
-      if (row >= a.rows) continue;
+    for (int c = 0; c < BN / 4; c += 32) {
+      const int col = w.nt * (BN / 2) + off + c;
+      if (a.vec && col + 32 <= a.ffn) {
+        const int p = e.lane & 3;
 #pragma unroll
-      for (int i = 0; i < 32; i += 8) {
-        const int col = col0 + c + i;
-        float dh[8];
-        if (a.vec && col + 8 <= a.ffn) {
-          const uint4 x = __ldg(reinterpret_cast<const uint4*>(dhrow + col));
-          const T* t = reinterpret_cast<const T*>(&x);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) dh[j] = to_f32<T>(t[j]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) dh[j] = col + j < a.ffn ? to_f32<T>(dhrow[col + j]) : 0.f;
+        for (int it = 0; it < 4; ++it) {
+          const int r = it * 8 + (e.lane >> 2);
+          *exch16(in, r, p) = r < rows ? __ldg(reinterpret_cast<const uint4*>(
+                                             dhbase + (int64_t)r * a.lddh + col + 8 * p))
+                                       : make_uint4(0u, 0u, 0u, 0u);
         }
-        float dg[8], du[8];
+      } else {
+        for (int r = 0; r < 32; ++r)
+          reinterpret_cast<uint16_t*>(exch16(in, r, e.lane >> 3))[e.lane & 7] =
+              r < rows && col + e.lane < a.ffn ? dhbase[(int64_t)r * a.lddh + col + e.lane] : 0;
+      }
+      __syncwarp();
+      float g[32], u[32];
+      e.read(off + c, g);
+      e.read(BN / 2 + off + c, u);
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const uint4 x = *exch16(in, e.lane, p);
+        const T* t = reinterpret_cast<const T*>(&x);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float x = g[i + j], s = sigmoid_approx(x);
-          dg[j] = dh[j] * u[i + j] * (s * fmaf(x, 1.f - s, 1.f));
-          du[j] = dh[j] * (x * s);
-          if (col + j >= a.ffn) dg[j] = du[j] = 0.f;
+          const int i = 8 * p + j;
+          const float dh = to_f32<T>(t[j]), z = g[i], s = sigmoid_approx(z);
+          g[i] = dh * u[i] * (s * fmaf(z, 1.f - s, 1.f));
+          u[i] = dh * (z * s);
+          if (col + i >= a.ffn) g[i] = u[i] = 0.f;
         }
-        *reinterpret_cast<uint4*>(drow + col) =
-            make_uint4(pack2<BF16>(dg[0], dg[1]), pack2<BF16>(dg[2], dg[3]),
-                       pack2<BF16>(dg[4], dg[5]), pack2<BF16>(dg[6], dg[7]));
-        *reinterpret_cast<uint4*>(drow + a.wide + col) =
-            make_uint4(pack2<BF16>(du[0], du[1]), pack2<BF16>(du[2], du[3]),
-                       pack2<BF16>(du[4], du[5]), pack2<BF16>(du[6], du[7]));
       }
+      store_block16<BF16>(e, g, base, 2 * a.wide, rows, col, a.wide, true);
+      store_block16<BF16>(e, u, base, 2 * a.wide, rows, a.wide + col, 2 * a.wide, true);
     }
   }
 };
@@ -124,20 +111,23 @@ namespace {
 using namespace sm100;
 
 struct FfnPlan {
-  int bn;         // 128-row tiles of bn / 2 gate and bn / 2 up columns
+  GemmForm pair, bwd;  // tiles of the pre-activations, and of dx and dw
   int wide;
-  int dx_bn, dx_splits;
+  int dx_splits;
   size_t off_sum, bwd_bytes;
 };
 
 FfnPlan ffn_plan(const ssa_gated_ffn_t* p) {
   FfnPlan q{};
-  const int tm = cdiv(p->rows, 128);
-  // Fewer tiles than multiprocessors at the wide tile: the narrow one.
-  q.bn = (int64_t)tm * cdiv(p->ffn, 128) >= kPlanSms ? 256 : 128;
-  q.wide = cdiv(p->ffn, q.bn / 2) * (q.bn / 2);
-  q.dx_bn = (int64_t)tm * cdiv(p->hidden, 256) >= kPlanSms ? 256 : 128;
-  q.dx_splits = split_count(tm * cdiv(p->hidden, q.dx_bn), 2 * q.wide / 64);
+  q.pair = gemm_form((int64_t)cdiv(p->rows, 256) * cdiv(p->ffn, 128));
+  q.wide = cdiv(p->ffn, q.pair.bn / 2) * (q.pair.bn / 2);
+  const int64_t dx256 = (int64_t)cdiv(p->rows, 256) * cdiv(p->hidden, 256);
+  const int64_t dw256 = (int64_t)cdiv(2 * q.wide, 256) * cdiv(p->hidden, 256);
+  q.bwd = gemm_form(dx256 > dw256 ? dx256 : dw256);
+  const int64_t dx_tiles = (int64_t)cdiv(p->rows, q.bwd.bm) * cdiv(p->hidden, q.bwd.bn);
+  const int64_t dw_tiles = (int64_t)cdiv(2 * q.wide, q.bwd.bm) * cdiv(p->hidden, q.bwd.bn);
+  q.dx_splits = split_count(dx_tiles, 2 * q.wide / 64, dw_tiles * (cdiv(p->rows, 64) + kTileCost),
+                            q.bwd.workers);
   q.off_sum = up256(4 * (size_t)p->rows * q.wide);
   q.bwd_bytes = q.off_sum;
   if (q.dx_splits > 1)
@@ -169,11 +159,12 @@ template <template <int, bool> class Epi, bool BF16, class Args>
 int ffn_pair_gemm(const ssa_gated_ffn_t* p, const FfnPlan& q, const Args& a, cudaStream_t st) {
   const GemmOperand A{p->x, p->rows, p->hidden, p->x_stride, "x"};
   const GemmOperand B{p->w, 2 * (int64_t)p->ffn, p->hidden, p->w_stride, "w"};
-  GemmShape g = plain_shape(cdiv(p->rows, 128), cdiv(p->ffn, q.bn / 2), cdiv(p->hidden, 64),
-                            2 * (int64_t)p->rows * p->hidden);
+  GemmShape g = plain_shape(cdiv(p->rows, q.pair.bm), cdiv(p->ffn, q.pair.bn / 2),
+                            cdiv(p->hidden, 64), 2 * (int64_t)p->rows * p->hidden);
   g.b_pair = p->ffn;
-  return q.bn == 256 ? launch_gemm<Epi<256, BF16>, 256, false, false, BF16>(A, B, g, a, st)
-                     : launch_gemm<Epi<128, BF16>, 128, false, false, BF16>(A, B, g, a, st);
+  return q.pair.pair
+             ? launch_gemm<Epi<256, BF16>, 2, 256, 0, false, BF16>({A, B, g, a}, nullptr, st)
+             : launch_gemm<Epi<128, BF16>, 1, 128, 0, false, BF16>({A, B, g, a}, nullptr, st);
 }
 
 template <bool BF16>
@@ -185,43 +176,31 @@ int ffn_bwd(const ssa_gated_ffn_t* p, const FfnPlan& q, const void* dh, int64_t 
   if (rc != SSA_OK) return rc;
   const int64_t k2 = 2 * (int64_t)q.wide;
   float* sum = reinterpret_cast<float*>(ws + q.off_sum);
-  const int tm = cdiv(p->rows, 128);
-  if (dx) {
-    StoreArgs s{};
-    s.out = q.dx_splits == 1 ? dx : nullptr;
-    s.sum = sum;
-    s.rows = p->rows;
-    s.ldo = s.cols = p->hidden;
-    const int kblocks = (int)(k2 / 64);
-    GemmShape g = plain_shape(tm, cdiv(p->hidden, q.dx_bn), kblocks, 2 * (int64_t)p->rows * k2);
-    g.kb_split = cdiv(kblocks, q.dx_splits);
-    g.splits = q.dx_splits;
-    g.b_kjump_at = q.wide / 64;  // du's columns meet the up projection's rows
-    g.b_kjump = p->ffn;
-    const GemmOperand A{ws, p->rows, k2, k2, "d"};
-    const GemmOperand B{p->w, p->hidden, 2 * (int64_t)p->ffn, p->w_stride, "w"};
-    rc = q.dx_bn == 256 ? launch_gemm<EpiStore<256, BF16>, 256, false, true, BF16>(A, B, g, s, st)
-                        : launch_gemm<EpiStore<128, BF16>, 128, false, true, BF16>(A, B, g, s, st);
-    if (rc != SSA_OK) return rc;
-    if (q.dx_splits > 1) {
-      rc = launch_sum_splits<BF16>(sum, dx, nullptr, p->rows, p->hidden, p->hidden, q.dx_splits, st);
-      if (rc != SSA_OK) return rc;
-    }
-  }
-  if (dw) {
-    StoreArgs s{};
-    s.out = dw;
-    s.rows = k2;
-    s.ldo = s.cols = p->hidden;
-    s.jump_at = q.wide;
-    s.jump = s.jump_rows = p->ffn;
-    rc = launch_gemm<EpiStore<256, BF16>, 256, true, true, BF16>(
-        GemmOperand{ws, k2, p->rows, k2, "d"},
-        GemmOperand{p->x, p->hidden, p->rows, p->x_stride, "x"},
-        plain_shape((int)(k2 / 128), cdiv(p->hidden, 256), cdiv(p->rows, 64),
-                    2 * (int64_t)p->rows * k2), s, st);
-    if (rc != SSA_OK) return rc;
-  }
+  StoreArgs sx{}, sw{};
+  sx.out = q.dx_splits == 1 ? dx : nullptr;
+  sx.sum = sum;
+  sx.rows = p->rows;
+  sx.ldo = sx.cols = sw.ldo = sw.cols = p->hidden;
+  const int kblocks = (int)(k2 / 64), tiles_h = cdiv(p->hidden, q.bwd.bn);
+  GemmShape gx = plain_shape(cdiv(p->rows, q.bwd.bm), tiles_h, kblocks, 2 * (int64_t)p->rows * k2);
+  gx.kb_split = cdiv(kblocks, q.dx_splits);
+  gx.splits = q.dx_splits;
+  gx.b_kjump_at = q.wide / 64;  // du's columns meet the up projection's rows
+  gx.b_kjump = p->ffn;
+  sw.out = dw;
+  sw.rows = (int)k2;
+  sw.jump_at = q.wide;
+  sw.jump = sw.jump_rows = p->ffn;
+  const GemmShape gw = plain_shape(cdiv(k2, q.bwd.bm), tiles_h, cdiv(p->rows, 64),
+                                   2 * (int64_t)p->rows * k2);
+  const GemmOperand dk{ws, p->rows, k2, k2, "d"}, dmn{ws, k2, p->rows, k2, "d"};
+  const GemmOperand wb{p->w, p->hidden, 2 * (int64_t)p->ffn, p->w_stride, "w"};
+  const GemmOperand xb{p->x, p->hidden, p->rows, p->x_stride, "x"};
+  const StoreProduct px{dk, wb, gx, sx}, pw{dmn, xb, gw, sw};
+  rc = launch_gradients(BF16, q.bwd.pair, dx ? &px : nullptr, dw ? &pw : nullptr, st);
+  if (rc != SSA_OK) return rc;
+  if (dx && q.dx_splits > 1)
+    return launch_sum_splits(BF16, sum, dx, nullptr, p->rows, p->hidden, p->hidden, q.dx_splits, st);
   return SSA_OK;
 }
 

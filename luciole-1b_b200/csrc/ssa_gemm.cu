@@ -1,0 +1,130 @@
+// ssa_gemm.cu — the plain products of the backward passes (dx and dW) on the core in ssa_gemm.cuh.
+#include "ssa_gemm.cuh"
+
+#include <atomic>
+
+namespace ssa {
+namespace sm100 {
+
+int device_sm_count() {
+  static std::atomic<int> counts[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return kPlanSms;
+  if ((n = counts[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1)
+    return kPlanSms;
+  counts[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+namespace {
+
+template <int BN, bool BF16>
+struct EpiStore {
+  using Args = StoreArgs;
+  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, const EpiCtx& e) {
+    const float sc = a.scale ? __ldg(a.scale) : 1.f;
+    const int col0 = w.nt * BN + e.half * (BN / 2);
+#pragma unroll 1
+    for (int c = 0; c < BN / 2; c += 32) {
+      const int col = col0 + c;
+      if (col >= a.cols) break;
+      float v[32];
+      e.read(e.half * (BN / 2) + c, v);
+#pragma unroll
+      for (int p = 0; p < 8; ++p)
+        *exch32(e.exch, e.lane, p) = make_float4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
+      __syncwarp();
+      // four lanes per row, 8 columns each
+      const int q = e.lane & 3, my = col + 8 * q;
+#pragma unroll
+      for (int it = 0; it < 4; ++it) {
+        const int r = it * 8 + (e.lane >> 2);
+        const int64_t row = (int64_t)e.row0 + r;
+        float4 x = *exch32(e.exch, r, 2 * q), y = *exch32(e.exch, r, 2 * q + 1);
+        bool ok = row < a.rows && my < a.cols;
+        int64_t orow = row;
+        if (a.jump_at) {
+          const int64_t in = row < a.jump_at ? row : row - a.jump_at;
+          ok = ok && in < a.jump_rows;
+          orow = row < a.jump_at ? row : a.jump + in;
+        }
+        if (!ok) continue;
+        float4* sp = reinterpret_cast<float4*>(
+            a.sum + ((int64_t)w.sp * a.rows + row) * a.cols + my);
+        if (a.add_prev) {
+          const float4 b = sp[0], d = sp[1];
+          x.x += b.x, x.y += b.y, x.z += b.z, x.w += b.w;
+          y.x += d.x, y.y += d.y, y.z += d.z, y.w += d.w;
+        }
+        if (a.out)
+          *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + orow * a.ldo + my) =
+              make_uint4(pack2<BF16>(x.x * sc, x.y * sc), pack2<BF16>(x.z * sc, x.w * sc),
+                         pack2<BF16>(y.x * sc, y.y * sc), pack2<BF16>(y.z * sc, y.w * sc));
+        else
+          sp[0] = x, sp[1] = y;
+      }
+      __syncwarp();
+    }
+  }
+};
+
+// out[row, col] = scale * sum over splits, in split order (deterministic).
+template <bool BF16>
+__global__ void __launch_bounds__(256) sum_splits_kernel(const float* sum, void* out,
+                                                         const float* scale, int64_t rows, int cols,
+                                                         int64_t ldo, int splits) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const float sc = scale ? __ldg(scale) : 1.f;
+  const int per_row = cols / 4;
+  const int64_t total = rows * per_row, plane = rows * (int64_t)cols;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / per_row;
+    const int col = (int)(i - row * per_row) * 4;
+    const float* p = sum + row * cols + col;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < splits; ++k) {
+      const float4 x = *reinterpret_cast<const float4*>(p + k * plane);
+      s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+    }
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(out) + row * ldo + col) =
+        make_uint2(pack2<BF16>(s.x * sc, s.y * sc), pack2<BF16>(s.z * sc, s.w * sc));
+  }
+}
+
+template <int CG, int BN, bool BF16>
+int gradients(const StoreProduct* dx, const StoreProduct* dw, cudaStream_t st) {
+  using Epi = EpiStore<BN, BF16>;
+  auto product = [](const StoreProduct* p) { return GemmProduct<Epi>{p->a, p->b, p->g, p->ea}; };
+  if (!dw) return launch_gemm<Epi, CG, BN, 0, true, BF16>(product(dx), nullptr, st);
+  if (!dx) return launch_gemm<Epi, CG, BN, 1, true, BF16>(product(dw), nullptr, st);
+  const GemmProduct<Epi> second = product(dw);
+  return launch_gemm<Epi, CG, BN, 2, true, BF16>(product(dx), &second, st);
+}
+
+}  // namespace
+
+int launch_gradients(bool bf16, bool pair, const StoreProduct* dx, const StoreProduct* dw,
+                     cudaStream_t st) {
+  if (pair) return bf16 ? gradients<2, 256, true>(dx, dw, st) : gradients<2, 256, false>(dx, dw, st);
+  return bf16 ? gradients<1, 128, true>(dx, dw, st) : gradients<1, 128, false>(dx, dw, st);
+}
+
+int launch_sum_splits(bool bf16, const float* sum, void* out, const float* scale, int64_t rows,
+                      int cols, int64_t ldo, int splits, cudaStream_t st) {
+  const int64_t blocks = (rows * (cols / 4) + 255) / 256;
+  const int64_t most = (int64_t)device_sm_count() * 8;
+  const dim3 grid((unsigned)(blocks < most ? blocks : most));
+  const cudaError_t e =
+      bf16 ? launch_pdl(sum_splits_kernel<true>, grid, dim3(256), 0, st, sum, out, scale, rows, cols,
+                        ldo, splits)
+           : launch_pdl(sum_splits_kernel<false>, grid, dim3(256), 0, st, sum, out, scale, rows, cols,
+                        ldo, splits);
+  if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "sum_splits: %s", cudaGetErrorString(e));
+  note_launches(1);
+  return SSA_OK;
+}
+
+}  // namespace sm100
+}  // namespace ssa

@@ -2,15 +2,26 @@
 // is a template argument: the shared core of the linear cross entropy (ssa_linear_ce.cu) and the
 // gated feed-forward (ssa_gated_ffn.cu).
 //
-// Roles (192 threads): warp 0 issues TMA loads, warp 1 issues the MMAs, warps 2..5 run the
-// epilogue, one thread per accumulator row. A tile's fp32 accumulator is BN TMEM columns and there
-// are two of them, so the epilogue of one tile runs under the MMAs of the next.
+// A tile is 128 CG rows by BN columns, made by a cluster of CG CTAs. Each CTA holds 128 rows of A and
+// BN / CG = 128 rows of B per 64-wide K block in shared memory (32 KB a stage, 6 stages) and the
+// fp32 accumulator of its 128 rows in BN TMEM columns, twice, so that the epilogue of one tile runs
+// under the MMAs of the next. CG = 2, BN = 256 is the form for large products: the pair's MMA reads
+// both halves of B, so a CTA fetches 32 KB per 4.2 MFLOP where a lone 128 x 256 tile fetches 48 KB.
+// CG = 1, BN = 128 is for products with too few such tiles.
+//
+// Roles (320 threads): warp 0 issues TMA loads, warp 1 of the leading CTA issues the MMAs, warps
+// 2..9 run the epilogue: two warps per 32 accumulator rows, each with half of the columns. Results
+// are exchanged through shared memory so that global accesses are whole 64- or 128-byte row pieces.
 //
 // Operands are 16-bit matrices in global memory, each either K-major (the contraction index is
 // contiguous) or MN-major (the row index m or n is contiguous): a gradient product reads its
 // operands in place, with no transposed copy. Both arrive as 64-element (128-byte) wide boxes in
 // the 128-byte swizzle; a box past an edge of the matrix reads zeros, so M, N and K are arbitrary.
 // Only alignment is asked for: 16-byte base and row stride.
+//
+// A launch may hold two products (dx and dW of one backward): their tiles are dealt out together,
+// the longer ones first, which fills the multiprocessors where each alone leaves a part-filled last
+// round.
 //
 // Every wait is bounded. When one expires, or an earlier launch left the device status set, the
 // epilogue runs on NaN accumulators for every tile this CTA still owes, so the failure shows.
@@ -25,9 +36,9 @@
 namespace ssa {
 namespace sm100 {
 
-// How the tiles of one launch are laid out (plain data, passed by value).
+// One product of a launch (plain data, passed by value).
 struct GemmShape {
-  int tiles_m, tiles_n;  // 128-row and BN-column tiles
+  int tiles_m, tiles_n;  // tiles of 128 CG rows and BN columns
   int splits;            // contiguous K ranges per tile, each a unit of work
   int kblocks;           // 64-wide K blocks of a tile
   int kb_split;          // K blocks per split
@@ -35,7 +46,6 @@ struct GemmShape {
   int b_kjump_at;        // MN-major B: K blocks from here on read rows b_kjump + 64 (kb - at)
   int b_kjump;
   int b_pair;            // 0, or B is a pair of row blocks this far apart, BN / 2 rows of each
-  unsigned int* status;
 };
 
 struct GemmUnit {
@@ -56,33 +66,152 @@ __device__ __forceinline__ GemmUnit gemm_unit(const GemmShape& g, int u) {
   return w;
 }
 
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
-                                            int c0, int c1) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
-      : "memory");
-}
-
-template <int BN_>
-struct GemmCfg {
-  static constexpr int BM = 128, BN = BN_, BK = 64;
-  static constexpr uint32_t A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;
-  static constexpr uint32_t STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGES = 196608 / STAGE > 8 ? 8 : 196608 / STAGE;
-  static constexpr uint32_t OFF_BAR = STAGES * STAGE;
-  static constexpr uint32_t SMEM_BYTES = OFF_BAR + 256 + 1024;  // + slack for 1 KB alignment
-  static constexpr uint32_t TMEM_COLS = 2 * BN;
-  static constexpr int THREADS = 192;
+// The products of a launch and how their units are dealt to `workers` clusters: the product with the
+// longer units (`lead`) round robin; where its last round is part-filled, each cluster left out
+// takes `extra` units of the other first; the rest of the other round robin.
+struct GemmWork {
+  GemmShape g[2];
+  int units0, units1;  // of the leading product, of the other
+  int lead;
+  int extra;
+  unsigned int* status;
 };
 
-// Reads accumulator columns [32 c, 32 c + 32) of the calling thread's row (every lane of the warp
-// calls it): the values in TMEM, or NaN when the launch failed.
-struct AccReader {
-  uint32_t taddr;
+// The i-th unit of cluster c: its product in `which`, its index returned, -1 past the end.
+__device__ __forceinline__ int gemm_deal(const GemmWork& w, int c, int workers, int i, int& which) {
+  const int rem = w.units0 % workers;
+  const int mine = w.units0 / workers + (c < rem ? 1 : 0);
+  which = w.lead;
+  if (i < mine) return c + i * workers;
+  which = w.lead ^ 1;
+  int j = i - mine, u;
+  const int first = rem ? (workers - rem) * w.extra : 0;
+  if (rem && c >= rem) {
+    if (j < w.extra) u = (c - rem) * w.extra + j;
+    else u = first + c + (j - w.extra) * workers;
+  } else {
+    u = first + c + j * workers;
+  }
+  return u < w.units1 ? u : -1;
+}
+
+template <int CG>
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                            int c0, int c1) {
+  if constexpr (CG == 1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+  } else {  // into this CTA's memory, counted by the leading CTA's barrier
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+  }
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// The address in the cluster's shared window of `addr` (this CTA's window) as seen in CTA `rank`.
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// The pair forms of the TMEM and MMA instructions (both CTAs of the cluster take part).
+template <int CG>
+__device__ __forceinline__ void tmem_alloc_cg(uint32_t smem_dst, uint32_t ncols) {
+  if constexpr (CG == 1) {
+    tmem_alloc(smem_dst, ncols);
+    tmem_relinquish();
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst),
+                 "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_dealloc_cg(uint32_t taddr, uint32_t ncols) {
+  if constexpr (CG == 1)
+    tmem_dealloc(taddr, ncols);
+  else
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols)
+                 : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void mma_cg(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,
+                                       uint32_t accumulate) {
+  if constexpr (CG == 1) {
+    mma_ss_lo(d_tmem, a_lo, b_lo, idesc, accumulate);
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %5};\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHiSW128)
+        : "memory");
+  }
+}
+// Arrives on the barrier (in both CTAs of a pair) once the MMAs issued so far have completed.
+template <int CG>
+__device__ __forceinline__ void mma_commit_cg(uint32_t bar) {
+  if constexpr (CG == 1) {
+    mma_commit(bar);
+  } else {
+    const uint16_t both = 3;
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;" ::"r"(bar),
+        "h"(both)
+        : "memory");
+  }
+}
+
+template <int CG_, int BN_>
+struct GemmCfg {
+  static constexpr int CG = CG_, BM = 128, BN = BN_, BK = 64;
+  static constexpr int RB = BN / CG;  // rows of B in one CTA
+  static constexpr uint32_t A_BYTES = BM * BK * 2, B_BYTES = RB * BK * 2;
+  static constexpr uint32_t STAGE = A_BYTES + B_BYTES;
+  static constexpr int STAGES = 196608 / STAGE;
+  static constexpr int EPI_WARPS = 8;
+  static constexpr uint32_t OFF_EXCH = STAGES * STAGE;  // 4 KB per epilogue warp
+  static constexpr uint32_t OFF_BAR = OFF_EXCH + EPI_WARPS * 4096;
+  static constexpr uint32_t SMEM_BYTES = OFF_BAR + 256 + 1024;  // + slack for 1 KB alignment
+  static constexpr uint32_t TMEM_COLS = 2 * BN;
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+  static_assert(SMEM_BYTES <= 232448, "shared memory of one CTA");
+};
+
+// What an epilogue warp works on: accumulator rows row0 .. row0 + 31 of the unit's tile (one per
+// lane), half `half` of its columns.
+struct EpiCtx {
+  uint32_t taddr;   // TMEM address of the accumulator's column 0 in this warp's lanes
   bool failed;
-  __device__ __forceinline__ void operator()(int col, float (&v)[32]) const {
+  uint8_t* exch;    // this warp's 4 KB of shared memory
+  uint8_t* exch0;   // the 4 KB of epilogue warp 0
+  int lane, quad, half, turn;
+  int row0;         // global row of lane 0
+
+  // Accumulator columns [col, col + 32) of this lane's row (every lane of the warp calls it).
+  __device__ __forceinline__ void read(int col, float (&v)[32]) const {
     if (failed) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = nan_f32();
@@ -96,14 +225,64 @@ struct AccReader {
   }
 };
 
-// Epi: struct with `Args` and `static void tile(const Args&, const GemmUnit&, int row, const
-// AccReader&)`, run by every epilogue thread for its accumulator row (0..127) of each unit.
-template <class Epi, int BN, bool A_MN, bool B_MN, bool BF16>
-__global__ void __launch_bounds__(192, 1)
-    gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmA,
-                      const __grid_constant__ CUtensorMap tmB, const GemmShape g,
-                      const typename Epi::Args ea) {
-  using C = GemmCfg<BN>;
+// Exchange of a [32 rows x 32 columns] block of 16-bit values within a warp: a lane's row of 64
+// bytes on one side, four lanes per row (8 columns each, rows 8 it + lane / 4) on the other. Row r
+// keeps its 16-byte pieces in order c ^ (r / 2 % 4), which spreads both sides over all banks.
+__device__ __forceinline__ uint4* exch16(uint8_t* buf, int row, int piece) {
+  return reinterpret_cast<uint4*>(buf + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4));
+}
+// The same for fp32 (128 bytes a row, eight lanes per row, rows 4 it + lane / 8).
+__device__ __forceinline__ float4* exch32(uint8_t* buf, int row, int piece) {
+  return reinterpret_cast<float4*>(buf + row * 128 + ((piece ^ (row & 7)) << 4));
+}
+
+template <bool BF16>
+__device__ __forceinline__ void put_row16(const EpiCtx& e, const float (&v)[32]) {
+#pragma unroll
+  for (int p = 0; p < 4; ++p)
+    *exch16(e.exch, e.lane, p) =
+        make_uint4(pack2<BF16>(v[8 * p], v[8 * p + 1]), pack2<BF16>(v[8 * p + 2], v[8 * p + 3]),
+                   pack2<BF16>(v[8 * p + 4], v[8 * p + 5]), pack2<BF16>(v[8 * p + 6], v[8 * p + 7]));
+}
+
+// Stores the warp's block of 16-bit values (one row of 32 per lane) to rows base + r * ld of
+// columns [col, col + 32), rows and columns below the limits only. base: row 0, column 0.
+// vec: base and ld are multiples of 16 bytes.
+template <bool BF16>
+__device__ __forceinline__ void store_block16(const EpiCtx& e, const float (&v)[32], uint16_t* base,
+                                              int64_t ld, int rows, int col, int cols, bool vec) {
+  put_row16<BF16>(e, v);
+  __syncwarp();
+  if (vec && col + 32 <= cols) {
+    const int p = e.lane & 3;
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+      const int r = it * 8 + (e.lane >> 2);
+      if (r < rows)
+        *reinterpret_cast<uint4*>(base + (int64_t)r * ld + col + 8 * p) = *exch16(e.exch, r, p);
+    }
+  } else if (col + e.lane < cols) {
+    const int n = min(rows, 32);
+    for (int r = 0; r < n; ++r)
+      base[(int64_t)r * ld + col + e.lane] =
+          reinterpret_cast<const uint16_t*>(exch16(e.exch, r, e.lane >> 3))[e.lane & 7];
+  }
+  __syncwarp();
+}
+
+// Epi: struct with `Args` and `static void tile(const Args&, const GemmUnit&, const EpiCtx&)`, run
+// by every epilogue warp for each unit. A_MODE: 0 A is K-major, 1 MN-major, 2 K-major in product 0
+// and MN-major in product 1.
+template <class Epi, int CG, int BN, int A_MODE, bool B_MN, bool BF16>
+__global__ void __launch_bounds__(320, 1)
+    gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmA0,
+                      const __grid_constant__ CUtensorMap tmB0,
+                      const __grid_constant__ CUtensorMap tmA1,
+                      const __grid_constant__ CUtensorMap tmB1,
+                      const __grid_constant__ GemmWork work,
+                      const __grid_constant__ typename Epi::Args ea0,
+                      const __grid_constant__ typename Epi::Args ea1) {
+  using C = GemmCfg<CG, BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -116,21 +295,14 @@ __global__ void __launch_bounds__(192, 1)
   const uint32_t bar_end = bar0 + 8u * (2 * C::STAGES + 4);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_BAR + 8 * (2 * C::STAGES + 5));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile uint32_t* status_slot = tmem_slot + 2;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
+  const int worker = (int)blockIdx.x / CG, workers = (int)gridDim.x / CG;
   // Launched programmatically: nothing global is touched before the previous kernel is done.
   griddep_wait();
   griddep_launch_dependents();
-  const int units = g.tiles_m * g.tiles_n * g.splits;
-
-  if (block_status_failed(g.status)) {  // block-uniform
-    if (warp >= 2) {
-      const AccReader nan_acc{0, true};
-      for (int u = blockIdx.x; u < units; u += gridDim.x)
-        Epi::tile(ea, gemm_unit(g, u), (warp & 3) * 32 + lane, nan_acc);
-    }
-    return;
-  }
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -139,81 +311,111 @@ __global__ void __launch_bounds__(192, 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(tfull(s), 1);
-      mbar_init(tempty(s), 128);
+      mbar_init(tempty(s), CG * C::EPI_WARPS);
     }
     mbar_init(bar_end, 1);
     *abort_flag = 0;
+    *status_slot = *reinterpret_cast<const volatile unsigned int*>(work.status);
     fence_mbar_init();
   }
   if (warp == 1) {
     __syncwarp();
-    tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
-    tmem_relinquish();
+    tmem_alloc_cg<CG>(smem_u32(tmem_slot), C::TMEM_COLS);
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) cluster_sync();  // both CTAs' barriers are initialised
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  // The CTAs of a pair decide alike: either's view of the status word counts.
+  uint32_t status = *status_slot;
+  if constexpr (CG == 2) {
+    uint32_t other;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];"
+                 : "=r"(other)
+                 : "r"(map_rank(smem_u32(tmem_slot + 2), rank ^ 1u))
+                 : "memory");
+    status |= other;
+  }
+  const bool dead = status != 0;
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      prefetch_tmap(&tmA);
-      prefetch_tmap(&tmB);
+    if (lane == 0 && !dead) {
+      prefetch_tmap(&tmA0);
+      prefetch_tmap(&tmB0);
       int it = 0;
       bool ok = true;
-      for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+      for (int i = 0; ok; ++i) {
+        int which;
+        const int u = gemm_deal(work, worker, workers, i, which);
+        if (u < 0) break;
+        const bool second = A_MODE == 2 && which == 1;
+        const GemmShape& g = work.g[second ? 1 : 0];
+        const CUtensorMap* ta = second ? &tmA1 : &tmA0;
+        const CUtensorMap* tb = second ? &tmB1 : &tmB0;
+        const bool a_mn = A_MODE == 1 || second;
         const GemmUnit w = gemm_unit(g, u);
-        const int m0 = w.mt * C::BM;
-        const int n0 = g.b_pair ? w.nt * (BN / 2) : w.nt * BN;
+        const int m0 = (w.mt * CG + (int)rank) * C::BM;
+        const int n0 = g.b_pair ? w.nt * (BN / 2) + (CG == 2 && rank ? g.b_pair : 0)
+                                : w.nt * BN + (int)rank * C::RB;
         for (int kb = w.k0; kb < w.k1; ++kb, ++it) {
           const int st = it % C::STAGES, use = it / C::STAGES;
-          if (use > 0) ok = mbar_wait(empty(st), (use - 1) & 1, g.status);
+          if (use > 0) ok = mbar_wait(empty(st), (use - 1) & 1, work.status);
           if (!ok || *abort_flag) {
             ok = false;
             break;
           }
           const uint32_t sa = sbase + st * C::STAGE, sb = sa + C::A_BYTES;
-          mbar_expect_tx(full(st), C::STAGE);
+          uint32_t fb = full(st);
+          if constexpr (CG == 2) fb = map_rank(fb, 0);
+          if (rank == 0) mbar_expect_tx(full(st), CG * C::STAGE);
           const int k = kb * C::BK;
-          if constexpr (A_MN) {
+          if (a_mn) {
 #pragma unroll
-            for (int i = 0; i < C::BM / 64; ++i)
-              tma_load_2d(sa + i * 8192, &tmA, full(st), m0 + i * 64, k);
+            for (int j = 0; j < C::BM / 64; ++j)
+              tma_load_2d<CG>(sa + j * 8192, ta, fb, m0 + j * 64, k);
           } else {
-            tma_load_2d(sa, &tmA, full(st), k, m0);
+            tma_load_2d<CG>(sa, ta, fb, k, m0);
           }
           if constexpr (B_MN) {
             const int kr = kb < g.b_kjump_at ? k : g.b_kjump + (kb - g.b_kjump_at) * C::BK;
 #pragma unroll
-            for (int i = 0; i < BN / 64; ++i)
-              tma_load_2d(sb + i * 8192, &tmB, full(st), n0 + i * 64, kr);
-          } else {  // two boxes of BN / 2 rows: one after the other, or the two of a pair
-            tma_load_2d(sb, &tmB, full(st), k, n0);
-            tma_load_2d(sb + C::B_BYTES / 2, &tmB, full(st), k,
-                        g.b_pair ? g.b_pair + n0 : n0 + BN / 2);
+            for (int j = 0; j < C::RB / 64; ++j)
+              tma_load_2d<CG>(sb + j * 8192, tb, fb, n0 + j * 64, kr);
+          } else {
+            tma_load_2d<CG>(sb, tb, fb, k, n0);
+            if constexpr (CG == 1)  // the second half of B, or the pair's other block
+              tma_load_2d<CG>(sb + C::B_BYTES / 2, tb, fb, k, g.b_pair ? n0 + g.b_pair : n0 + BN / 2);
           }
         }
       }
       if (!ok) {
         *abort_flag = 1;
-        // this CTA's own loads land before its shared memory is released
-        for (int j = max(0, it - C::STAGES); j < it; ++j)
-          mbar_wait(full(j % C::STAGES), (j / C::STAGES) & 1, g.status);
+        // loads in flight land before the shared memory is released
+        if (rank == 0)
+          for (int j = max(0, it - C::STAGES); j < it; ++j)
+            mbar_wait(full(j % C::STAGES), (j / C::STAGES) & 1, work.status);
       }
     }
+    __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t idesc = idesc_f16(BF16, A_MN, B_MN, C::BM, BN);
-      constexpr uint32_t LBO = 8192;                  // MN-major: next 64 rows of m or n
-      constexpr uint32_t KA = A_MN ? 2048 >> 4 : 2, KB = B_MN ? 2048 >> 4 : 2;  // 16 k's on
+    if (lane == 0 && rank == 0 && !dead) {
+      constexpr uint32_t LBO = 8192;  // MN-major: next 64 rows of m or n
       int it = 0, i = 0;
       bool ok = true;
-      for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++i) {
-        const GemmUnit w = gemm_unit(g, u);
+      for (; ok; ++i) {
+        int which;
+        const int u = gemm_deal(work, worker, workers, i, which);
+        if (u < 0) break;
+        const bool second = A_MODE == 2 && which == 1;
+        const bool a_mn = A_MODE == 1 || second;
+        const GemmUnit w = gemm_unit(work.g[second ? 1 : 0], u);
+        const uint32_t idesc = idesc_f16(BF16, false, B_MN, 128 * CG, BN) | (a_mn ? 1u << 15 : 0u);
+        const uint32_t ka = a_mn ? 2048 >> 4 : 2, kb_step = B_MN ? 2048 >> 4 : 2;  // 16 k's on
         const uint32_t acc = tmem + (uint32_t)((i & 1) * BN);
-        if (i >= 2) ok = mbar_wait(tempty(i & 1), ((i >> 1) - 1) & 1, g.status);
+        if (i >= 2) ok = mbar_wait(tempty(i & 1), ((i >> 1) - 1) & 1, work.status);
         if (!ok || *abort_flag) {
           ok = false;
           break;
@@ -221,55 +423,76 @@ __global__ void __launch_bounds__(192, 1)
         tc_fence_after();
         for (int kb = w.k0; kb < w.k1; ++kb, ++it) {
           const int st = it % C::STAGES;
-          ok = mbar_wait(full(st), (it / C::STAGES) & 1, g.status);
+          ok = mbar_wait(full(st), (it / C::STAGES) & 1, work.status);
           if (!ok || *abort_flag) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a_lo = sdesc_lo(sbase + st * C::STAGE, A_MN ? LBO : 16);
+          const uint32_t a_lo = sdesc_lo(sbase + st * C::STAGE, a_mn ? LBO : 16);
           const uint32_t b_lo = sdesc_lo(sbase + st * C::STAGE + C::A_BYTES, B_MN ? LBO : 16);
 #pragma unroll
           for (int kk = 0; kk < C::BK / 16; ++kk)
-            mma_ss_lo(acc, a_lo + kk * KA, b_lo + kk * KB, idesc, (kb > w.k0 || kk > 0) ? 1u : 0u);
-          mma_commit(empty(st));
+            mma_cg<CG>(acc, a_lo + kk * ka, b_lo + kk * kb_step, idesc,
+                       (kb > w.k0 || kk > 0) ? 1u : 0u);
+          mma_commit_cg<CG>(empty(st));
         }
-        if (ok) mma_commit(tfull(i & 1));
+        if (ok) mma_commit_cg<CG>(tfull(i & 1));
       }
       if (!ok) *abort_flag = 1;
-      mma_commit(bar_end);  // every MMA of this CTA retires before TMEM is freed
-      mbar_wait(bar_end, 0, g.status);
+      mma_commit_cg<CG>(bar_end);  // every MMA retires before TMEM and shared memory are released
+      mbar_wait(bar_end, 0, work.status);
     }
     __syncwarp();
   } else {
-    // ------------------------------------------------------------------ epilogue rows
-    const int quad = warp & 3;
-    const int row = quad * 32 + lane;
-    AccReader rd{tmem + ((uint32_t)(quad * 32) << 16), false};
-    int i = 0;
-    for (int u = blockIdx.x; u < units; u += gridDim.x, ++i) {
-      const GemmUnit w = gemm_unit(g, u);
-      if (!rd.failed) {
-        const bool ok = mbar_wait(tfull(i & 1), (i >> 1) & 1, g.status);
+    // ------------------------------------------------------------------ epilogue
+    EpiCtx e;
+    e.failed = dead;
+    e.lane = lane;
+    e.quad = warp & 3;  // the 32 TMEM lanes this warp can read
+    e.half = (warp - 2) >> 2;
+    e.exch0 = smem + C::OFF_EXCH;
+    e.exch = e.exch0 + (warp - 2) * 4096;
+    for (int i = 0;; ++i) {
+      int which;
+      const int u = gemm_deal(work, worker, workers, i, which);
+      if (u < 0) break;
+      const bool second = A_MODE == 2 && which == 1;
+      const GemmUnit w = gemm_unit(work.g[second ? 1 : 0], u);
+      if (!e.failed) {
+        const bool ok = mbar_wait(tfull(i & 1), (i >> 1) & 1, work.status);
         if (!__all_sync(0xffffffffu, ok && !*abort_flag)) {
-          rd.failed = true;
+          e.failed = true;
           *abort_flag = 1;
         }
         tc_fence_after();
-        rd.taddr = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)((i & 1) * BN);
       }
-      Epi::tile(ea, w, row, rd);
+      e.taddr = tmem + ((uint32_t)(e.quad * 32) << 16) + (uint32_t)((i & 1) * BN);
+      e.turn = i;
+      e.row0 = (w.mt * CG + (int)rank) * C::BM + e.quad * 32;
+      Epi::tile(second ? ea1 : ea0, w, e);
       tc_fence_before();
-      if (!rd.failed) mbar_arrive(tempty(i & 1));
+      __syncwarp();
+      if (!e.failed && lane == 0) {
+        if constexpr (CG == 2) mbar_arrive_cluster(map_rank(tempty(i & 1), 0));
+        else mbar_arrive(tempty(i & 1));
+      }
     }
   }
 
   tc_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) {
+    // every arrival the leading CTA's MMAs send here has come, and the other CTA is done with this
+    // one's memory
+    if (threadIdx.x == 0 && rank == 1 && !dead) mbar_wait(bar_end, 0, work.status);
+    __syncthreads();
+    cluster_sync();
+  }
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem, C::TMEM_COLS);
+    tmem_dealloc_cg<CG>(tmem, C::TMEM_COLS);
   }
 }
 
@@ -308,29 +531,69 @@ int device_sm_count();  // multiprocessors of the current device (cached)
 
 // Multiprocessors that plans are made for, so that a workspace size needs no device.
 constexpr int kPlanSms = 148;
+// A tile's cost outside its K blocks (epilogue, pipeline fill), in K blocks.
+constexpr int kTileCost = 8;
 
-template <class Epi, int BN, bool A_MN, bool B_MN, bool BF16>
-int launch_gemm(const GemmOperand& a, const GemmOperand& b, GemmShape g,
-                const typename Epi::Args& ea, cudaStream_t st) {
-  using C = GemmCfg<BN>;
+// One product, or two that are dealt out together.
+template <class Epi>
+struct GemmProduct {
+  GemmOperand a, b;
+  GemmShape g;
+  typename Epi::Args ea;
+};
+
+template <class Epi, int CG, int BN, int A_MODE, bool B_MN, bool BF16>
+int launch_gemm(const GemmProduct<Epi>& p0, const GemmProduct<Epi>* p1, cudaStream_t st) {
+  using C = GemmCfg<CG, BN>;
+  static_assert(A_MODE == 2 || A_MODE == 0 || A_MODE == 1, "layout of A");
   constexpr int dtype = BF16 ? SSA_DTYPE_BF16 : SSA_DTYPE_F16;
-  CUtensorMap ta, tb;
-  int rc;
-  rc = A_MN ? make_tmap_2d(&ta, a.ptr, dtype, a.mn, a.k, a.ld, 64, a.name)
-            : make_tmap_2d(&ta, a.ptr, dtype, a.k, a.mn, a.ld, C::BM, a.name);
-  if (rc != SSA_OK) return rc;
-  rc = B_MN ? make_tmap_2d(&tb, b.ptr, dtype, b.mn, b.k, b.ld, 64, b.name)
-            : make_tmap_2d(&tb, b.ptr, dtype, b.k, b.mn, b.ld, BN / 2, b.name);
-  if (rc != SSA_OK) return rc;
-  g.status = device_status_ptr();
-  if (!g.status) return abi_error(SSA_ERR_CUDA, "cannot resolve the device status word");
-  auto kern = gemm_sm100_kernel<Epi, BN, A_MN, B_MN, BF16>;
+  CUtensorMap t[4];
+  const GemmProduct<Epi>& q1 = p1 ? *p1 : p0;
+  for (int i = 0; i < (p1 ? 2 : 1); ++i) {
+    const GemmProduct<Epi>& p = i ? q1 : p0;
+    const bool a_mn = A_MODE == 1 || (A_MODE == 2 && i == 1);
+    int rc = a_mn ? make_tmap_2d(&t[2 * i], p.a.ptr, dtype, p.a.mn, p.a.k, p.a.ld, 64, p.a.name)
+                  : make_tmap_2d(&t[2 * i], p.a.ptr, dtype, p.a.k, p.a.mn, p.a.ld, C::BM, p.a.name);
+    if (rc != SSA_OK) return rc;
+    rc = B_MN ? make_tmap_2d(&t[2 * i + 1], p.b.ptr, dtype, p.b.mn, p.b.k, p.b.ld, 64, p.b.name)
+              : make_tmap_2d(&t[2 * i + 1], p.b.ptr, dtype, p.b.k, p.b.mn, p.b.ld, BN / 2, p.b.name);
+    if (rc != SSA_OK) return rc;
+  }
+  if (!p1) t[2] = t[0], t[3] = t[1];
+  GemmWork w{};
+  w.g[0] = p0.g;
+  w.g[1] = q1.g;
+  const int64_t u0 = (int64_t)p0.g.tiles_m * p0.g.tiles_n * p0.g.splits;
+  const int64_t u1 = p1 ? (int64_t)q1.g.tiles_m * q1.g.tiles_n * q1.g.splits : 0;
+  if (u0 + u1 > INT32_MAX / 2) return abi_error(SSA_ERR_BAD_SHAPE, "too many tiles");
+  w.lead = p1 && q1.g.kb_split > p0.g.kb_split ? 1 : 0;
+  w.units0 = (int)(w.lead ? u1 : u0);
+  w.units1 = (int)(w.lead ? u0 : u1);
+  if (p1) {
+    const int a = w.g[w.lead].kb_split + kTileCost, b = w.g[w.lead ^ 1].kb_split + kTileCost;
+    w.extra = (a + b / 2) / b;
+  }
+  w.status = device_status_ptr();
+  if (!w.status) return abi_error(SSA_ERR_CUDA, "cannot resolve the device status word");
+  auto kern = gemm_sm100_kernel<Epi, CG, BN, A_MODE, B_MN, BF16>;
   if (set_smem_limit_once(reinterpret_cast<const void*>(kern), (int)C::SMEM_BYTES) != SSA_OK)
     return abi_error(SSA_ERR_CUDA, "cannot raise the shared memory limit");
-  const int64_t units = (int64_t)g.tiles_m * g.tiles_n * g.splits;
-  const int grid = (int)(units < device_sm_count() ? units : device_sm_count());
-  const cudaError_t e = launch_pdl(kern, dim3((unsigned)grid), dim3(C::THREADS), C::SMEM_BYTES, st,
-                                   ta, tb, g, ea);
+  const int most = device_sm_count() / CG;
+  const int workers = (int)(u0 + u1 < most ? u0 + u1 : most);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(workers * CG));
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM_BYTES;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CG;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CG == 2 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, t[0], t[1], t[2], t[3], w, p0.ea, q1.ea);
   if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "%s", cudaGetErrorString(e));
   note_launches(1);
   return SSA_OK;
@@ -339,27 +602,39 @@ int launch_gemm(const GemmOperand& a, const GemmOperand& b, GemmShape g,
 inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 inline size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// Row tiles walked before the column advances: all of them while that operand's panel stays in L2
-// beside the other's stream, else 16, a square-ish set of tiles in flight.
-inline int gemm_band(int tiles_m, int64_t a_bytes) {
-  return a_bytes <= (int64_t)40 << 20 ? tiles_m : (tiles_m < 16 ? tiles_m : 16);
+// Tile form: the pair's 256 x 256 tiles once they fill the clusters, else 128 x 128 tiles. Measured
+// on B200: see the callers.
+struct GemmForm {
+  bool pair;
+  int bm, bn, workers;
+};
+inline GemmForm gemm_form(int64_t tiles_256) {
+  const bool pair = tiles_256 >= kPlanSms / 2;
+  return pair ? GemmForm{true, 256, 256, kPlanSms / 2} : GemmForm{false, 128, 128, kPlanSms};
 }
 
+// Row tiles walked before the column advances: all of them while that operand's panel stays in L2
+// beside the other's stream; else, when the column tiles are few, as many as keep one whole set of
+// columns in flight (A is then read once, B from L2); else 16, a square-ish set of tiles.
 inline GemmShape plain_shape(int tiles_m, int tiles_n, int kblocks, int64_t a_bytes) {
   GemmShape g{};
   g.tiles_m = tiles_m;
   g.tiles_n = tiles_n;
   g.splits = 1;
   g.kblocks = g.kb_split = kblocks;
-  g.band = gemm_band(tiles_m, a_bytes);
+  int band = tiles_n <= 18 ? kPlanSms / 2 / tiles_n : 16;
+  if (band < 1) band = 1;
+  g.band = a_bytes <= (int64_t)40 << 20 || tiles_m < band ? tiles_m : band;
   g.b_kjump_at = INT32_MAX;
   return g;
 }
 
-// Splits of each tile's contraction when there are fewer tiles than multiprocessors, of at least
-// four K blocks each.
-inline int split_count(int tiles, int kblocks) {
-  int s = tiles < kPlanSms ? kPlanSms / tiles : 1;
+// Splits of the contraction of `tiles` tiles of `kblocks` K blocks beside `other` K blocks of the
+// launch's other product, so that no unit is longer than a worker's share of everything; of at least
+// four blocks each. The same whether the other product is asked for or not: so are the bits.
+inline int split_count(int64_t tiles, int kblocks, int64_t other, int workers) {
+  const int64_t share = (tiles * kblocks + other) / workers;
+  int64_t s = share > 0 ? (kblocks + share - 1) / share : kblocks;
   if (s > kblocks / 4) s = kblocks / 4;
   return s > 1 ? cdiv(kblocks, cdiv(kblocks, s)) : 1;
 }
@@ -371,96 +646,27 @@ struct StoreArgs {
   void* out;             // 16-bit [.., ldo], or nullptr: keep the sum in fp32
   float* sum;            // fp32 [splits][rows][cols], or nullptr
   const float* scale;    // device scalar, or nullptr (1)
-  int64_t rows, ldo;
-  int cols;              // a multiple of 8
+  int64_t ldo;
+  int rows, cols;        // cols: a multiple of 8
   int add_prev;          // add the matching element of sum
   int jump_at, jump;     // rows >= jump_at are stored at jump + row - jump_at; rows in
   int jump_rows;         //   [jump_rows, jump_at) and past jump_at + jump_rows are dropped
 };
 
-template <int BN, bool BF16>
-struct EpiStore {
-  using Args = StoreArgs;
-  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, int r,
-                                              const AccReader& rd) {
-    const int64_t row = (int64_t)w.mt * 128 + r;
-    const int col0 = w.nt * BN;
-    int64_t orow = row;
-    bool ok = row < a.rows;
-    if (a.jump_at) {
-      const int64_t in = row < a.jump_at ? row : row - a.jump_at;
-      ok = ok && in < a.jump_rows;
-      orow = row < a.jump_at ? row : a.jump + in;
-    }
-    const float sc = a.scale ? __ldg(a.scale) : 1.f;
-    float* srow = a.sum ? a.sum + ((int64_t)w.sp * a.rows + row) * a.cols : nullptr;
-    uint16_t* drow = a.out ? reinterpret_cast<uint16_t*>(a.out) + orow * a.ldo : nullptr;
-#pragma unroll 1
-    for (int c = 0; c < BN; c += 32) {
-      if (col0 + c >= a.cols) break;
-      float v[32];
-      rd(c, v);
-      if (!ok) continue;
-#pragma unroll
-      for (int i = 0; i < 32; i += 8) {
-        const int col = col0 + c + i;
-        if (col >= a.cols) break;
-        if (a.add_prev) {
-          const float4* p = reinterpret_cast<const float4*>(srow + col);
-          const float4 x = p[0], y = p[1];
-          v[i] += x.x, v[i + 1] += x.y, v[i + 2] += x.z, v[i + 3] += x.w;
-          v[i + 4] += y.x, v[i + 5] += y.y, v[i + 6] += y.z, v[i + 7] += y.w;
-        }
-        if (drow) {
-          *reinterpret_cast<uint4*>(drow + col) =
-              make_uint4(pack2<BF16>(v[i] * sc, v[i + 1] * sc), pack2<BF16>(v[i + 2] * sc, v[i + 3] * sc),
-                         pack2<BF16>(v[i + 4] * sc, v[i + 5] * sc), pack2<BF16>(v[i + 6] * sc, v[i + 7] * sc));
-        } else {
-          float4* p = reinterpret_cast<float4*>(srow + col);
-          p[0] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-          p[1] = make_float4(v[i + 4], v[i + 5], v[i + 6], v[i + 7]);
-        }
-      }
-    }
-  }
+struct StoreProduct {
+  GemmOperand a, b;
+  GemmShape g;
+  StoreArgs ea;
 };
 
-// out[row, col] = scale * sum over splits, in split order (deterministic).
-template <bool BF16>
-__global__ void __launch_bounds__(256) sum_splits_kernel(const float* sum, void* out,
-                                                         const float* scale, int64_t rows, int cols,
-                                                         int64_t ldo, int splits) {
-  griddep_wait();
-  griddep_launch_dependents();
-  const float sc = scale ? __ldg(scale) : 1.f;
-  const int per_row = cols / 4;
-  const int64_t total = rows * per_row, plane = rows * (int64_t)cols;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / per_row;
-    const int col = (int)(i - row * per_row) * 4;
-    const float* p = sum + row * cols + col;
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < splits; ++k) {
-      const float4 x = *reinterpret_cast<const float4*>(p + k * plane);
-      s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
-    }
-    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(out) + row * ldo + col) =
-        make_uint2(pack2<BF16>(s.x * sc, s.y * sc), pack2<BF16>(s.z * sc, s.w * sc));
-  }
-}
+// dx = d W (d K-major) and dW = d^T x (d MN-major), B MN-major in both: one launch for both, or either
+// alone where the other is nullptr. `pair`: the tile form (GemmForm::pair).
+int launch_gradients(bool bf16, bool pair, const StoreProduct* dx, const StoreProduct* dw,
+                     cudaStream_t st);
 
-template <bool BF16>
-int launch_sum_splits(const float* sum, void* out, const float* scale, int64_t rows, int cols,
-                      int64_t ldo, int splits, cudaStream_t st) {
-  const int64_t blocks = (rows * (cols / 4) + 255) / 256;
-  const int64_t most = (int64_t)device_sm_count() * 8;
-  const cudaError_t e =
-      launch_pdl(sum_splits_kernel<BF16>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256),
-                 0, st, sum, out, scale, rows, cols, ldo, splits);
-  if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "%s", cudaGetErrorString(e));
-  note_launches(1);
-  return SSA_OK;
-}
+// out[row, col] = scale * (the splits' sums [splits][rows][cols], added in split order).
+int launch_sum_splits(bool bf16, const float* sum, void* out, const float* scale, int64_t rows,
+                      int cols, int64_t ldo, int splits, cudaStream_t st);
 
 }  // namespace sm100
 }  // namespace ssa

@@ -9,24 +9,12 @@
 // formed again and leave as d in 16 bits, then two products read that piece: dx is summed over the
 // pieces in fp32, dW's rows of the piece are final. Bound: the tensor cores, 8 rows hidden vocab
 // operations for forward and backward against the 6 that a kept logit matrix would need.
-#include <atomic>
 #include <cmath>
 
 #include "ssa_gemm.cuh"
 
 namespace ssa {
 namespace sm100 {
-
-int device_sm_count() {
-  static std::atomic<int> counts[64];
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return kPlanSms;
-  if ((n = counts[dev].load(std::memory_order_relaxed)) > 0) return n;
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1)
-    return kPlanSms;
-  counts[dev].store(n, std::memory_order_relaxed);
-  return n;
-}
 
 constexpr float kLowest = -3.0e38f;  // start of a running maximum: finite, so that max - max is 0
 
@@ -40,18 +28,17 @@ struct CeFwdArgs {
 template <int BN>
 struct EpiCeFwd {
   using Args = CeFwdArgs;
-  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, int r,
-                                              const AccReader& rd) {
-    const int row = w.mt * 128 + r;
-    const int col0 = w.nt * BN;
+  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, const EpiCtx& e) {
+    const int row = e.row0 + e.lane;
+    const int off = e.half * (BN / 2), col0 = w.nt * BN + off;
     const bool ok = row < a.rows;
     const int64_t t = ok ? __ldg(a.targets + row) : -1;
     float m = kLowest, s = 0.f;
 #pragma unroll 1
-    for (int c = 0; c < BN; c += 32) {
+    for (int c = 0; c < BN / 2; c += 32) {
       if (col0 + c >= a.vocab) break;
       float v[32];
-      rd(c, v);
+      e.read(off + c, v);
       if (col0 + c + 32 > a.vocab) {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
@@ -75,7 +62,17 @@ struct EpiCeFwd {
         a.target_logit[row] = x;
       }
     }
-    if (ok) a.part[(int64_t)w.nt * a.rows + row] = make_float2(m, s);
+    // The row's other half is in the warp with the same lanes: its pair comes through shared
+    // memory, in two places in turn, so that one barrier per tile is enough.
+    float2* mine = reinterpret_cast<float2*>(e.exch + (e.turn & 1) * 256) + e.lane;
+    if (e.half == 1) *mine = make_float2(m, s);
+    named_bar_sync(1 + e.quad, 64);
+    if (e.half == 0 && ok) {
+      const float2 p = *reinterpret_cast<const float2*>(reinterpret_cast<uint8_t*>(mine) + 4 * 4096);
+      const float mn = fmaxf(m, p.x);
+      s = s * ex2_approx((m - mn) * kLog2e) + p.y * ex2_approx((p.x - mn) * kLog2e);
+      a.part[(int64_t)w.nt * a.rows + row] = make_float2(mn, s);
+    }
   }
 };
 
@@ -194,19 +191,19 @@ struct CeBwdArgs {
 template <int BN, bool BF16>
 struct EpiCeBwd {
   using Args = CeBwdArgs;
-  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, int r,
-                                              const AccReader& rd) {
-    const int row = w.mt * 128 + r;
+  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, const EpiCtx& e) {
+    const int row = e.row0 + e.lane;
     const bool ok = row < a.rows;
     const float g = ok ? __ldg(a.weight + row) : 0.f;
     const float b = ok ? -__ldg(a.lse + row) * kLog2e : 0.f;
     const int64_t t = ok ? __ldg(a.targets + row) : -1;
-    uint16_t* drow = reinterpret_cast<uint16_t*>(a.d) + (int64_t)row * a.ldd + w.nt * BN;
+    const int off = e.half * (BN / 2);
+    uint16_t* base = reinterpret_cast<uint16_t*>(a.d) + (int64_t)e.row0 * a.ldd + w.nt * BN + off;
 #pragma unroll 1
-    for (int c = 0; c < BN; c += 32) {
-      const int col = a.piece0 + w.nt * BN + c;
+    for (int c = 0; c < BN / 2; c += 32) {
+      const int col = a.piece0 + w.nt * BN + off + c;
       float v[32];
-      rd(c, v);
+      e.read(off + c, v);
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = ex2_approx(fmaf(v[i], kLog2e, b)) * g;
       const int64_t at = t - col;
@@ -219,14 +216,7 @@ struct EpiCeBwd {
         for (int i = 0; i < 32; ++i)
           if (g == 0.f || col + i >= a.vocab) v[i] = 0.f;
       }
-      if (ok) {
-        uint4* o = reinterpret_cast<uint4*>(drow + c);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          o[i] = make_uint4(pack2<BF16>(v[8 * i], v[8 * i + 1]), pack2<BF16>(v[8 * i + 2], v[8 * i + 3]),
-                            pack2<BF16>(v[8 * i + 4], v[8 * i + 5]),
-                            pack2<BF16>(v[8 * i + 6], v[8 * i + 7]));
-      }
+      store_block16<BF16>(e, v, base, a.ldd, a.rows - e.row0, c, BN / 2, true);
     }
   }
 };
@@ -241,10 +231,11 @@ using namespace sm100;
 constexpr int64_t kPieceBytes = (int64_t)256 << 20;
 
 struct CePlan {
-  int tiles_n;                 // forward column tiles
+  GemmForm fwd, bwd;           // tiles of the logits, and of dx and dw
+  int fwd_tiles;               // column tiles of the forward
   int64_t ldd;                 // columns of a piece (a multiple of 256)
   int pieces;
-  int dx_bn, dx_splits;
+  int dx_splits;
   size_t off_target, off_rows, fwd_bytes;
   size_t off_inv, off_d, off_sum, bwd_bytes;
 };
@@ -252,8 +243,9 @@ struct CePlan {
 CePlan ce_plan(const ssa_linear_ce_t* p) {
   CePlan q{};
   const int64_t rows = p->rows;
-  q.tiles_n = cdiv(p->vocab, 256);
-  q.off_target = up256(sizeof(float2) * (size_t)q.tiles_n * rows);
+  q.fwd = gemm_form((int64_t)cdiv(rows, 256) * cdiv(p->vocab, 256));
+  q.fwd_tiles = cdiv(p->vocab, q.fwd.bn);
+  q.off_target = up256(sizeof(float2) * (size_t)q.fwd_tiles * rows);
   q.off_rows = q.off_target + up256(sizeof(float) * rows);
   q.fwd_bytes = q.off_rows + up256(sizeof(float) * rows);
 
@@ -264,13 +256,13 @@ CePlan ce_plan(const ssa_linear_ce_t* p) {
   q.pieces = cdiv(all, cols);
   q.ldd = (int64_t)cdiv(all / 256, q.pieces) * 256;  // pieces of about equal width
   q.pieces = cdiv(all, q.ldd);
-  const int tm = cdiv(rows, 128);
-  // dx: [rows, hidden] tiles that contract over the vocabulary. Too few of them for the
-  // multiprocessors: narrower tiles, then each tile's contraction in splits.
-  q.dx_bn = (int64_t)tm * cdiv(p->hidden, 256) >= kPlanSms ? 256 : 128;
-  const int tiles = tm * cdiv(p->hidden, q.dx_bn);
-  const int kblocks = (int)(q.ldd / 64);
-  q.dx_splits = split_count(tiles, kblocks);
+  const int64_t dx256 = (int64_t)cdiv(rows, 256) * cdiv(p->hidden, 256);
+  const int64_t dw256 = (q.ldd / 256) * cdiv(p->hidden, 256);
+  q.bwd = gemm_form(dx256 > dw256 ? dx256 : dw256);
+  const int64_t dx_tiles = (int64_t)cdiv(rows, q.bwd.bm) * cdiv(p->hidden, q.bwd.bn);
+  const int64_t dw_tiles = (int64_t)cdiv(q.ldd, q.bwd.bm) * cdiv(p->hidden, q.bwd.bn);
+  q.dx_splits = split_count(dx_tiles, (int)(q.ldd / 64), dw_tiles * (cdiv(rows, 64) + kTileCost),
+                            q.bwd.workers);
   q.off_inv = up256(sizeof(float) * rows);
   q.off_d = q.off_inv + 256;
   q.off_sum = q.off_d + up256(2 * (size_t)rows * q.ldd);
@@ -303,21 +295,30 @@ int ce_check(const ssa_linear_ce_t* p) {
   return SSA_OK;
 }
 
+// The product of x with (a piece of) W, with a forward or backward epilogue.
+template <class Epi256, class Epi128, bool BF16, class Args>
+int ce_logits(const ssa_linear_ce_t* p, const GemmForm& f, const void* w, int64_t cols, int tiles_n,
+              const Args& a, cudaStream_t st) {
+  const GemmOperand A{p->x, p->rows, p->hidden, p->x_stride, "x"};
+  const GemmOperand B{w, cols, p->hidden, p->w_stride, "w"};
+  const GemmShape g = plain_shape(cdiv(p->rows, f.bm), tiles_n, cdiv(p->hidden, 64),
+                                  2 * (int64_t)p->rows * p->hidden);
+  return f.pair ? launch_gemm<Epi256, 2, 256, 0, false, BF16>({A, B, g, a}, nullptr, st)
+                : launch_gemm<Epi128, 1, 128, 0, false, BF16>({A, B, g, a}, nullptr, st);
+}
+
 template <bool BF16>
 int ce_fwd(const ssa_linear_ce_t* p, const CePlan& q, float* loss, float* lse, float* count,
            uint8_t* ws, cudaStream_t st) {
   CeFwdArgs a{p->targets, reinterpret_cast<float2*>(ws),
               reinterpret_cast<float*>(ws + q.off_target), p->rows, p->vocab};
-  const GemmShape g = plain_shape(cdiv(p->rows, 128), q.tiles_n, cdiv(p->hidden, 64),
-                                  2 * (int64_t)p->rows * p->hidden);
-  int rc = launch_gemm<EpiCeFwd<256>, 256, false, false, BF16>(
-      GemmOperand{p->x, p->rows, p->hidden, p->x_stride, "x"},
-      GemmOperand{p->w, p->vocab, p->hidden, p->w_stride, "w"}, g, a, st);
+  const int rc = ce_logits<EpiCeFwd<256>, EpiCeFwd<128>, BF16>(p, q.fwd, p->w, p->vocab, q.fwd_tiles,
+                                                               a, st);
   if (rc != SSA_OK) return rc;
   float* rows_loss = p->reduction ? reinterpret_cast<float*>(ws + q.off_rows) : loss;
   cudaError_t e = launch_pdl(ce_join_kernel, dim3((unsigned)cdiv(p->rows, 32)), dim3(1024), 0, st,
                              (const float2*)a.part, (const float*)a.target_logit, p->targets,
-                             p->ignore_index, p->rows, p->vocab, q.tiles_n, lse, rows_loss);
+                             p->ignore_index, p->rows, p->vocab, q.fwd_tiles, lse, rows_loss);
   if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "ce_join: %s", cudaGetErrorString(e));
   note_launches(1);
   if (p->reduction) {
@@ -341,58 +342,42 @@ int ce_bwd(const ssa_linear_ce_t* p, const CePlan& q, const float* lse, const fl
                                    p->vocab, count, (int)(p->reduction == 1), weight, inv);
   if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "ce_row_weights: %s", cudaGetErrorString(e));
   note_launches(1);
-  const int tm = cdiv(p->rows, 128);
   for (int i = 0; i < q.pieces; ++i) {
     const int64_t v0 = (int64_t)i * q.ldd;
     const int64_t cols = p->vocab - v0 < q.ldd ? p->vocab - v0 : q.ldd;  // of the vocabulary
     const int64_t wide = (int64_t)cdiv(cols, 256) * 256;                 // written to d
     const uint8_t* w0 = static_cast<const uint8_t*>(p->w) + 2 * v0 * p->w_stride;
-    CeBwdArgs a{p->targets, lse, weight, d, q.ldd, p->rows, (int)v0, p->vocab};
-    int rc = launch_gemm<EpiCeBwd<256, BF16>, 256, false, false, BF16>(
-        GemmOperand{p->x, p->rows, p->hidden, p->x_stride, "x"},
-        GemmOperand{w0, cols, p->hidden, p->w_stride, "w"},
-        plain_shape(tm, (int)(wide / 256), cdiv(p->hidden, 64), 2 * (int64_t)p->rows * p->hidden), a,
-        st);
+    const CeBwdArgs a{p->targets, lse, weight, d, q.ldd, p->rows, (int)v0, p->vocab};
+    const GemmForm form = gemm_form((int64_t)cdiv(p->rows, 256) * (wide / 256));
+    int rc = ce_logits<EpiCeBwd<256, BF16>, EpiCeBwd<128, BF16>, BF16>(
+        p, form, w0, cols, (int)(wide / form.bn), a, st);
     if (rc != SSA_OK) return rc;
-    if (dx) {
-      const bool direct = q.dx_splits == 1 && i == q.pieces - 1;
-      StoreArgs s{};
-      s.out = direct ? dx : nullptr;
-      s.sum = sum;
-      s.scale = inv;
-      s.rows = p->rows;
-      s.ldo = p->hidden;
-      s.cols = p->hidden;
-      s.add_prev = i > 0;
-      const int kblocks = (int)(wide / 64);
-      GemmShape g = plain_shape(tm, cdiv(p->hidden, q.dx_bn), kblocks,
-                                2 * (int64_t)p->rows * q.ldd);
-      // every piece fills the same split planes: a narrower last piece takes thinner splits
-      g.kb_split = cdiv(kblocks, q.dx_splits);
-      g.splits = cdiv(kblocks, g.kb_split);
-      const GemmOperand A{d, p->rows, wide, q.ldd, "d"};
-      const GemmOperand B{w0, p->hidden, cols, p->w_stride, "w"};
-      rc = q.dx_bn == 256 ? launch_gemm<EpiStore<256, BF16>, 256, false, true, BF16>(A, B, g, s, st)
-                          : launch_gemm<EpiStore<128, BF16>, 128, false, true, BF16>(A, B, g, s, st);
-      if (rc != SSA_OK) return rc;
-    }
-    if (dw) {
-      StoreArgs s{};
-      s.out = static_cast<uint8_t*>(dw) + 2 * v0 * p->hidden;
-      s.scale = inv;
-      s.rows = cols;
-      s.ldo = p->hidden;
-      s.cols = p->hidden;
-      rc = launch_gemm<EpiStore<256, BF16>, 256, true, true, BF16>(
-          GemmOperand{d, wide, p->rows, q.ldd, "d"},
-          GemmOperand{p->x, p->hidden, p->rows, p->x_stride, "x"},
-          plain_shape((int)cdiv(cols, 128), cdiv(p->hidden, 256), cdiv(p->rows, 64),
-                      2 * (int64_t)p->rows * q.ldd), s, st);
-      if (rc != SSA_OK) return rc;
-    }
+
+    StoreArgs sx{}, sw{};
+    sx.out = q.dx_splits == 1 && i == q.pieces - 1 ? dx : nullptr;
+    sx.sum = sum;
+    sx.scale = sw.scale = inv;
+    sx.rows = p->rows;
+    sx.ldo = sx.cols = sw.ldo = sw.cols = p->hidden;
+    sx.add_prev = i > 0;
+    const int kblocks = (int)(wide / 64), tiles_h = cdiv(p->hidden, q.bwd.bn);
+    GemmShape gx = plain_shape(cdiv(p->rows, q.bwd.bm), tiles_h, kblocks, 2 * (int64_t)p->rows * q.ldd);
+    // every piece fills the same split planes: a narrower last piece takes thinner splits
+    gx.kb_split = cdiv(kblocks, q.dx_splits);
+    gx.splits = cdiv(kblocks, gx.kb_split);
+    sw.out = static_cast<uint8_t*>(dw) + 2 * v0 * p->hidden;
+    sw.rows = (int)cols;
+    const GemmShape gw = plain_shape(cdiv(cols, q.bwd.bm), tiles_h, cdiv(p->rows, 64),
+                                     2 * (int64_t)p->rows * q.ldd);
+    const GemmOperand dk{d, p->rows, wide, q.ldd, "d"}, dmn{d, wide, p->rows, q.ldd, "d"};
+    const GemmOperand wb{w0, p->hidden, cols, p->w_stride, "w"};
+    const GemmOperand xb{p->x, p->hidden, p->rows, p->x_stride, "x"};
+    const StoreProduct px{dk, wb, gx, sx}, pw{dmn, xb, gw, sw};
+    rc = launch_gradients(BF16, q.bwd.pair, dx ? &px : nullptr, dw ? &pw : nullptr, st);
+    if (rc != SSA_OK) return rc;
   }
   if (dx && q.dx_splits > 1)
-    return launch_sum_splits<BF16>(sum, dx, inv, p->rows, p->hidden, p->hidden, q.dx_splits, st);
+    return launch_sum_splits(BF16, sum, dx, inv, p->rows, p->hidden, p->hidden, q.dx_splits, st);
   return SSA_OK;
 }
 
