@@ -77,7 +77,7 @@ struct GemmWork {
   unsigned int* status;
 };
 
-// The i-th unit of cluster c: its product in `which`, its index returned, -1 past the end.
+// The i-th unit of cluster c (below gemm_count): its product in `which`, its index returned.
 __device__ __forceinline__ int gemm_deal(const GemmWork& w, int c, int workers, int i, int& which) {
   const int rem = w.units0 % workers;
   const int mine = w.units0 / workers + (c < rem ? 1 : 0);
@@ -92,7 +92,19 @@ __device__ __forceinline__ int gemm_deal(const GemmWork& w, int c, int workers, 
   } else {
     u = first + c + j * workers;
   }
-  return u < w.units1 ? u : -1;
+  return u;
+}
+
+// How many units cluster c has.
+__device__ __forceinline__ int gemm_count(const GemmWork& w, int c, int workers) {
+  const int rem = w.units0 % workers;
+  int n = w.units0 / workers + (c < rem ? 1 : 0);
+  int at = c;  // of the other product's round robin
+  if (rem) {
+    at += (workers - rem) * w.extra;
+    if (c >= rem) n += max(0, min(w.extra, w.units1 - (c - rem) * w.extra));
+  }
+  return n + (at < w.units1 ? (w.units1 - at - 1) / workers + 1 : 0);
 }
 
 template <int CG>
@@ -296,6 +308,10 @@ __global__ void __launch_bounds__(320, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_BAR + 8 * (2 * C::STAGES + 5));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile uint32_t* status_slot = tmem_slot + 2;
+  // K blocks of a unit (negative: A is MN-major), from the producer to the MMA issuer. The producer
+  // is at most STAGES units ahead.
+  volatile int* unit_slot = reinterpret_cast<volatile int*>(tmem_slot + 4);
+  static_assert(8 * (2 * C::STAGES + 5) + 16 + 4 * 8 <= 256 && C::STAGES < 8, "barrier page");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
@@ -339,17 +355,21 @@ __global__ void __launch_bounds__(320, 1)
   }
   const bool dead = status != 0;
 
+  // Warps 0 and 1 share their schedulers with epilogue warps and get few issue slots beside them, so
+  // their loops are kept to what each K block needs: running stage and phase, no division, the
+  // abort flag looked at once per unit, the unit's decoding left to the producer (which runs
+  // ahead). Measured on B200, see below.
+  const int count = gemm_count(work, worker, workers);
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0 && !dead) {
       prefetch_tmap(&tmA0);
       prefetch_tmap(&tmB0);
-      int it = 0;
+      int st = 0, round = 0;
       bool ok = true;
-      for (int i = 0; ok; ++i) {
+      for (int i = 0; ok && i < count; ++i) {
         int which;
         const int u = gemm_deal(work, worker, workers, i, which);
-        if (u < 0) break;
         const bool second = A_MODE == 2 && which == 1;
         const GemmShape& g = work.g[second ? 1 : 0];
         const CUtensorMap* ta = second ? &tmA1 : &tmA0;
@@ -359,83 +379,91 @@ __global__ void __launch_bounds__(320, 1)
         const int m0 = (w.mt * CG + (int)rank) * C::BM;
         const int n0 = g.b_pair ? w.nt * (BN / 2) + (CG == 2 && rank ? g.b_pair : 0)
                                 : w.nt * BN + (int)rank * C::RB;
-        for (int kb = w.k0; kb < w.k1; ++kb, ++it) {
-          const int st = it % C::STAGES, use = it / C::STAGES;
-          if (use > 0) ok = mbar_wait(empty(st), (use - 1) & 1, work.status);
-          if (!ok || *abort_flag) {
+        const int n1 = g.b_pair ? n0 + g.b_pair : n0 + BN / 2;  // CG = 1: second half of B
+        int k = w.k0 * C::BK, kr = k;
+        int to_jump = B_MN ? g.b_kjump_at - w.k0 : 0;
+        if (B_MN && to_jump <= 0) kr = g.b_kjump - to_jump * C::BK;
+        unit_slot[i & 7] = a_mn ? w.k0 - w.k1 : w.k1 - w.k0;
+        if (*abort_flag) ok = false;
+        for (int n = w.k1 - w.k0; ok && n > 0; --n) {
+          if (round > 0 && !mbar_wait(empty(st), (round - 1) & 1, work.status)) {
             ok = false;
             break;
           }
           const uint32_t sa = sbase + st * C::STAGE, sb = sa + C::A_BYTES;
           uint32_t fb = full(st);
-          if constexpr (CG == 2) fb = map_rank(fb, 0);
-          if (rank == 0) mbar_expect_tx(full(st), CG * C::STAGE);
-          const int k = kb * C::BK;
+          if constexpr (CG == 2) {
+            if (rank == 0) mbar_expect_tx(fb, CG * C::STAGE);
+            fb = map_rank(fb, 0);
+          } else {
+            mbar_expect_tx(fb, C::STAGE);
+          }
           if (a_mn) {
-#pragma unroll
-            for (int j = 0; j < C::BM / 64; ++j)
-              tma_load_2d<CG>(sa + j * 8192, ta, fb, m0 + j * 64, k);
+            tma_load_2d<CG>(sa, ta, fb, m0, k);
+            tma_load_2d<CG>(sa + 8192, ta, fb, m0 + 64, k);
           } else {
             tma_load_2d<CG>(sa, ta, fb, k, m0);
           }
           if constexpr (B_MN) {
-            const int kr = kb < g.b_kjump_at ? k : g.b_kjump + (kb - g.b_kjump_at) * C::BK;
 #pragma unroll
-            for (int j = 0; j < C::RB / 64; ++j)
-              tma_load_2d<CG>(sb + j * 8192, tb, fb, n0 + j * 64, kr);
+            for (int j = 0; j < C::RB / 64; ++j) tma_load_2d<CG>(sb + j * 8192, tb, fb, n0 + j * 64, kr);
+            kr = --to_jump == 0 ? g.b_kjump : kr + C::BK;
           } else {
             tma_load_2d<CG>(sb, tb, fb, k, n0);
-            if constexpr (CG == 1)  // the second half of B, or the pair's other block
-              tma_load_2d<CG>(sb + C::B_BYTES / 2, tb, fb, k, g.b_pair ? n0 + g.b_pair : n0 + BN / 2);
+            if constexpr (CG == 1) tma_load_2d<CG>(sb + C::B_BYTES / 2, tb, fb, k, n1);
           }
+          k += C::BK;
+          if (++st == C::STAGES) st = 0, ++round;
         }
       }
       if (!ok) {
         *abort_flag = 1;
-        // loads in flight land before the shared memory is released
+        // loads in flight land before the shared memory is released: each stage's last use
         if (rank == 0)
-          for (int j = max(0, it - C::STAGES); j < it; ++j)
-            mbar_wait(full(j % C::STAGES), (j / C::STAGES) & 1, work.status);
+          for (int j = 0; j < C::STAGES; ++j) {
+            const int uses = round + (j < st ? 1 : 0);
+            if (uses > 0) mbar_wait(full(j), (uses - 1) & 1, work.status);
+          }
       }
     }
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
     if (lane == 0 && rank == 0 && !dead) {
-      constexpr uint32_t LBO = 8192;  // MN-major: next 64 rows of m or n
-      int it = 0, i = 0;
+      constexpr uint32_t IDESC = idesc_f16(BF16, A_MODE == 1, B_MN, 128 * CG, BN);
+      constexpr uint32_t KB = B_MN ? 2048 >> 4 : 2;  // 16 k's on (descriptor units)
+      constexpr uint32_t LBO = 8192;                 // MN-major: next 64 rows of m or n
+      const uint32_t a_first = sdesc_lo(sbase, 16), b_first = sdesc_lo(sbase + C::A_BYTES, B_MN ? LBO : 16);
+      uint32_t st = 0, ph = 0;
       bool ok = true;
-      for (; ok; ++i) {
-        int which;
-        const int u = gemm_deal(work, worker, workers, i, which);
-        if (u < 0) break;
-        const bool second = A_MODE == 2 && which == 1;
-        const bool a_mn = A_MODE == 1 || second;
-        const GemmUnit w = gemm_unit(work.g[second ? 1 : 0], u);
-        const uint32_t idesc = idesc_f16(BF16, false, B_MN, 128 * CG, BN) | (a_mn ? 1u << 15 : 0u);
-        const uint32_t ka = a_mn ? 2048 >> 4 : 2, kb_step = B_MN ? 2048 >> 4 : 2;  // 16 k's on
+      // The MMAs of one K block in stage st, then its release.
+      auto block = [&](uint32_t acc, bool a_mn, uint32_t keep) {
+        const uint32_t a_lo = a_first + st * (C::STAGE >> 4) + (a_mn ? ((LBO - 16) >> 4) << 16 : 0u);
+        const uint32_t b_lo = b_first + st * (C::STAGE >> 4);
+        const uint32_t idesc = A_MODE == 2 && a_mn ? IDESC | (1u << 15) : IDESC;
+        const uint32_t ka = a_mn ? 2048 >> 4 : 2;
+#pragma unroll
+        for (int kk = 0; kk < C::BK / 16; ++kk)
+          mma_cg<CG>(acc, a_lo + kk * ka, b_lo + kk * KB, idesc, kk ? 1u : keep);
+        mma_commit_cg<CG>(empty((int)st));
+        if (++st == C::STAGES) st = 0, ph ^= 1;
+      };
+      for (int i = 0; ok && i < count; ++i) {
         const uint32_t acc = tmem + (uint32_t)((i & 1) * BN);
         if (i >= 2) ok = mbar_wait(tempty(i & 1), ((i >> 1) - 1) & 1, work.status);
-        if (!ok || *abort_flag) {
-          ok = false;
-          break;
-        }
+        if (ok) ok = mbar_wait(full((int)st), ph, work.status) && !*abort_flag;
+        if (!ok) break;
         tc_fence_after();
-        for (int kb = w.k0; kb < w.k1; ++kb, ++it) {
-          const int st = it % C::STAGES;
-          ok = mbar_wait(full(st), (it / C::STAGES) & 1, work.status);
-          if (!ok || *abort_flag) {
+        const int n = unit_slot[i & 7];
+        const bool a_mn = A_MODE == 1 || (A_MODE == 2 && n < 0);
+        block(acc, a_mn, 0u);
+        for (int kb = abs(n) - 1; kb > 0; --kb) {
+          if (!mbar_wait(full((int)st), ph, work.status)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a_lo = sdesc_lo(sbase + st * C::STAGE, a_mn ? LBO : 16);
-          const uint32_t b_lo = sdesc_lo(sbase + st * C::STAGE + C::A_BYTES, B_MN ? LBO : 16);
-#pragma unroll
-          for (int kk = 0; kk < C::BK / 16; ++kk)
-            mma_cg<CG>(acc, a_lo + kk * ka, b_lo + kk * kb_step, idesc,
-                       (kb > w.k0 || kk > 0) ? 1u : 0u);
-          mma_commit_cg<CG>(empty(st));
+          block(acc, a_mn, 1u);
         }
         if (ok) mma_commit_cg<CG>(tfull(i & 1));
       }
@@ -453,10 +481,9 @@ __global__ void __launch_bounds__(320, 1)
     e.half = (warp - 2) >> 2;
     e.exch0 = smem + C::OFF_EXCH;
     e.exch = e.exch0 + (warp - 2) * 4096;
-    for (int i = 0;; ++i) {
+    for (int i = 0; i < count; ++i) {
       int which;
       const int u = gemm_deal(work, worker, workers, i, which);
-      if (u < 0) break;
       const bool second = A_MODE == 2 && which == 1;
       const GemmUnit w = gemm_unit(work.g[second ? 1 : 0], u);
       if (!e.failed) {
