@@ -121,9 +121,8 @@ FfnPlan ffn_plan(const ssa_gated_ffn_t* p) {
   FfnPlan q{};
   q.pair = gemm_form((int64_t)cdiv(p->rows, 256) * cdiv(p->ffn, 128));
   q.wide = cdiv(p->ffn, q.pair.bn / 2) * (q.pair.bn / 2);
-  const int64_t dx256 = (int64_t)cdiv(p->rows, 256) * cdiv(p->hidden, 256);
-  const int64_t dw256 = (int64_t)cdiv(2 * q.wide, 256) * cdiv(p->hidden, 256);
-  q.bwd = gemm_form(dx256 > dw256 ? dx256 : dw256);
+  q.bwd = gradient_form(p->rows, 2 * (int64_t)q.wide, p->hidden, 2 * q.wide / 64,
+                        cdiv(p->rows, 64));
   const int64_t dx_tiles = (int64_t)cdiv(p->rows, q.bwd.bm) * cdiv(p->hidden, q.bwd.bn);
   const int64_t dw_tiles = (int64_t)cdiv(2 * q.wide, q.bwd.bm) * cdiv(p->hidden, q.bwd.bn);
   q.dx_splits = split_count(dx_tiles, 2 * q.wide / 64, dw_tiles * (cdiv(p->rows, 64) + kTileCost),
@@ -163,8 +162,8 @@ int ffn_pair_gemm(const ssa_gated_ffn_t* p, const FfnPlan& q, const Args& a, cud
                             cdiv(p->hidden, 64), 2 * (int64_t)p->rows * p->hidden);
   g.b_pair = p->ffn;
   return q.pair.pair
-             ? launch_gemm<Epi<256, BF16>, 2, 256, 0, false, BF16>({A, B, g, a}, nullptr, st)
-             : launch_gemm<Epi<128, BF16>, 1, 128, 0, false, BF16>({A, B, g, a}, nullptr, st);
+             ? launch_gemm<Epi<256, BF16>, 2, 256, 1, 0, false, BF16>({A, B, g, a}, nullptr, st)
+             : launch_gemm<Epi<128, BF16>, 1, 128, 1, 0, false, BF16>({A, B, g, a}, nullptr, st);
 }
 
 template <bool BF16>
@@ -197,7 +196,7 @@ int ffn_bwd(const ssa_gated_ffn_t* p, const FfnPlan& q, const void* dh, int64_t 
   const GemmOperand wb{p->w, p->hidden, 2 * (int64_t)p->ffn, p->w_stride, "w"};
   const GemmOperand xb{p->x, p->hidden, p->rows, p->x_stride, "x"};
   const StoreProduct px{dk, wb, gx, sx}, pw{dmn, xb, gw, sw};
-  rc = launch_gradients(BF16, q.bwd.pair, dx ? &px : nullptr, dw ? &pw : nullptr, st);
+  rc = launch_gradients(BF16, q.bwd, dx ? &px : nullptr, dw ? &pw : nullptr, st);
   if (rc != SSA_OK) return rc;
   if (dx && q.dx_splits > 1)
     return launch_sum_splits(BF16, sum, dx, nullptr, p->rows, p->hidden, p->hidden, q.dx_splits, st);

@@ -93,22 +93,28 @@ __global__ void __launch_bounds__(256) sum_splits_kernel(const float* sum, void*
   }
 }
 
-template <int CG, int BN, bool BF16>
+template <int CG, int BN, int NH, bool BF16>
 int gradients(const StoreProduct* dx, const StoreProduct* dw, cudaStream_t st) {
   using Epi = EpiStore<BN, BF16>;
   auto product = [](const StoreProduct* p) { return GemmProduct<Epi>{p->a, p->b, p->g, p->ea}; };
-  if (!dw) return launch_gemm<Epi, CG, BN, 0, true, BF16>(product(dx), nullptr, st);
-  if (!dx) return launch_gemm<Epi, CG, BN, 1, true, BF16>(product(dw), nullptr, st);
+  if (!dw) return launch_gemm<Epi, CG, BN, NH, 0, true, BF16>(product(dx), nullptr, st);
+  if (!dx) return launch_gemm<Epi, CG, BN, NH, 1, true, BF16>(product(dw), nullptr, st);
   const GemmProduct<Epi> second = product(dw);
-  return launch_gemm<Epi, CG, BN, 2, true, BF16>(product(dx), &second, st);
+  return launch_gemm<Epi, CG, BN, NH, 2, true, BF16>(product(dx), &second, st);
+}
+
+template <bool BF16>
+int gradients_form(const GemmForm& f, const StoreProduct* dx, const StoreProduct* dw,
+                   cudaStream_t st) {
+  if (f.wide) return gradients<2, 256, 2, BF16>(dx, dw, st);
+  return f.pair ? gradients<2, 256, 1, BF16>(dx, dw, st) : gradients<1, 128, 1, BF16>(dx, dw, st);
 }
 
 }  // namespace
 
-int launch_gradients(bool bf16, bool pair, const StoreProduct* dx, const StoreProduct* dw,
+int launch_gradients(bool bf16, const GemmForm& form, const StoreProduct* dx, const StoreProduct* dw,
                      cudaStream_t st) {
-  if (pair) return bf16 ? gradients<2, 256, true>(dx, dw, st) : gradients<2, 256, false>(dx, dw, st);
-  return bf16 ? gradients<1, 128, true>(dx, dw, st) : gradients<1, 128, false>(dx, dw, st);
+  return bf16 ? gradients_form<true>(form, dx, dw, st) : gradients_form<false>(form, dx, dw, st);
 }
 
 int launch_sum_splits(bool bf16, const float* sum, void* out, const float* scale, int64_t rows,

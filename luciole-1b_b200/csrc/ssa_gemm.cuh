@@ -7,7 +7,9 @@
 // fp32 accumulator of its 128 rows in BN TMEM columns, twice, so that the epilogue of one tile runs
 // under the MMAs of the next. CG = 2, BN = 256 is the form for large products: the pair's MMA reads
 // both halves of B, so a CTA fetches 32 KB per 4.2 MFLOP where a lone 128 x 256 tile fetches 48 KB.
-// CG = 1, BN = 128 is for products with too few such tiles.
+// CG = 1, BN = 128 is for products with too few such tiles. NH = 2 gives the pair both accumulators
+// for one 256 x 512 tile: 48 KB per 8.4 MFLOP, at the price of an epilogue that the next tile's MMAs
+// mostly wait for; it is for the long contractions of the gradients.
 //
 // Roles (320 threads): warp 0 issues TMA loads, warp 1 of the leading CTA issues the MMAs, warps
 // 2..9 run the epilogue: two warps per 32 accumulator rows, each with half of the columns. Results
@@ -196,10 +198,11 @@ __device__ __forceinline__ void mma_commit_cg(uint32_t bar) {
   }
 }
 
-template <int CG_, int BN_>
+template <int CG_, int BN_, int NH_>
 struct GemmCfg {
-  static constexpr int CG = CG_, BM = 128, BN = BN_, BK = 64;
-  static constexpr int RB = BN / CG;  // rows of B in one CTA
+  static constexpr int CG = CG_, BM = 128, BN = BN_, NH = NH_, BK = 64;
+  static constexpr int HB = BN / CG;   // rows of B in one CTA for one accumulator of BN columns
+  static constexpr int RB = NH * HB;
   static constexpr uint32_t A_BYTES = BM * BK * 2, B_BYTES = RB * BK * 2;
   static constexpr uint32_t STAGE = A_BYTES + B_BYTES;
   static constexpr int STAGES = 196608 / STAGE;
@@ -207,7 +210,7 @@ struct GemmCfg {
   static constexpr uint32_t OFF_EXCH = STAGES * STAGE;  // 4 KB per epilogue warp
   static constexpr uint32_t OFF_BAR = OFF_EXCH + EPI_WARPS * 4096;
   static constexpr uint32_t SMEM_BYTES = OFF_BAR + 256 + 1024;  // + slack for 1 KB alignment
-  static constexpr uint32_t TMEM_COLS = 2 * BN;
+  static constexpr uint32_t TMEM_COLS = 2 * BN;  // two accumulators: of two tiles, or NH = 2 of one
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
   static_assert(SMEM_BYTES <= 232448, "shared memory of one CTA");
 };
@@ -285,7 +288,7 @@ __device__ __forceinline__ void store_block16(const EpiCtx& e, const float (&v)[
 // Epi: struct with `Args` and `static void tile(const Args&, const GemmUnit&, const EpiCtx&)`, run
 // by every epilogue warp for each unit. A_MODE: 0 A is K-major, 1 MN-major, 2 K-major in product 0
 // and MN-major in product 1.
-template <class Epi, int CG, int BN, int A_MODE, bool B_MN, bool BF16>
+template <class Epi, int CG, int BN, int NH, int A_MODE, bool B_MN, bool BF16>
 __global__ void __launch_bounds__(320, 1)
     gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmA0,
                       const __grid_constant__ CUtensorMap tmB0,
@@ -294,7 +297,7 @@ __global__ void __launch_bounds__(320, 1)
                       const __grid_constant__ GemmWork work,
                       const __grid_constant__ typename Epi::Args ea0,
                       const __grid_constant__ typename Epi::Args ea1) {
-  using C = GemmCfg<CG, BN>;
+  using C = GemmCfg<CG, BN, NH>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -378,7 +381,7 @@ __global__ void __launch_bounds__(320, 1)
         const GemmUnit w = gemm_unit(g, u);
         const int m0 = (w.mt * CG + (int)rank) * C::BM;
         const int n0 = g.b_pair ? w.nt * (BN / 2) + (CG == 2 && rank ? g.b_pair : 0)
-                                : w.nt * BN + (int)rank * C::RB;
+                                : w.nt * BN * NH + (int)rank * C::HB;
         const int n1 = g.b_pair ? n0 + g.b_pair : n0 + BN / 2;  // CG = 1: second half of B
         int k = w.k0 * C::BK, kr = k;
         int to_jump = B_MN ? g.b_kjump_at - w.k0 : 0;
@@ -404,14 +407,19 @@ __global__ void __launch_bounds__(320, 1)
           } else {
             tma_load_2d<CG>(sa, ta, fb, k, m0);
           }
-          if constexpr (B_MN) {
 #pragma unroll
-            for (int j = 0; j < C::RB / 64; ++j) tma_load_2d<CG>(sb + j * 8192, tb, fb, n0 + j * 64, kr);
-            kr = --to_jump == 0 ? g.b_kjump : kr + C::BK;
-          } else {
-            tma_load_2d<CG>(sb, tb, fb, k, n0);
-            if constexpr (CG == 1) tma_load_2d<CG>(sb + C::B_BYTES / 2, tb, fb, k, n1);
+          for (int h = 0; h < NH; ++h) {
+            const uint32_t sh = sb + h * (C::HB * 128);
+            if constexpr (B_MN) {
+#pragma unroll
+              for (int j = 0; j < C::HB / 64; ++j)
+                tma_load_2d<CG>(sh + j * 8192, tb, fb, n0 + h * BN + j * 64, kr);
+            } else {
+              tma_load_2d<CG>(sh, tb, fb, k, n0 + h * BN);
+              if constexpr (CG == 1) tma_load_2d<CG>(sh + C::B_BYTES / 2, tb, fb, k, n1);
+            }
           }
+          if constexpr (B_MN) kr = --to_jump == 0 ? g.b_kjump : kr + C::BK;
           k += C::BK;
           if (++st == C::STAGES) st = 0, ++round;
         }
@@ -436,36 +444,82 @@ __global__ void __launch_bounds__(320, 1)
       const uint32_t a_first = sdesc_lo(sbase, 16), b_first = sdesc_lo(sbase + C::A_BYTES, B_MN ? LBO : 16);
       uint32_t st = 0, ph = 0;
       bool ok = true;
-      // The MMAs of one K block in stage st, then its release.
-      auto block = [&](uint32_t acc, bool a_mn, uint32_t keep) {
-        const uint32_t a_lo = a_first + st * (C::STAGE >> 4) + (a_mn ? ((LBO - 16) >> 4) << 16 : 0u);
-        const uint32_t b_lo = b_first + st * (C::STAGE >> 4);
+      // The MMAs of one K block in stage `at` into accumulator `acc`, with half h of B.
+      auto mmas = [&](uint32_t acc, uint32_t at, int h, bool a_mn, uint32_t keep) {
+        const uint32_t a_lo = a_first + at * (C::STAGE >> 4) + (a_mn ? ((LBO - 16) >> 4) << 16 : 0u);
+        const uint32_t b_lo = b_first + at * (C::STAGE >> 4) + (uint32_t)h * (C::HB * 128 >> 4);
         const uint32_t idesc = A_MODE == 2 && a_mn ? IDESC | (1u << 15) : IDESC;
         const uint32_t ka = a_mn ? 2048 >> 4 : 2;
 #pragma unroll
         for (int kk = 0; kk < C::BK / 16; ++kk)
           mma_cg<CG>(acc, a_lo + kk * ka, b_lo + kk * KB, idesc, kk ? 1u : keep);
+      };
+      auto release = [&]() {
         mma_commit_cg<CG>(empty((int)st));
         if (++st == C::STAGES) st = 0, ph ^= 1;
       };
       for (int i = 0; ok && i < count; ++i) {
-        const uint32_t acc = tmem + (uint32_t)((i & 1) * BN);
-        if (i >= 2) ok = mbar_wait(tempty(i & 1), ((i >> 1) - 1) & 1, work.status);
-        if (ok) ok = mbar_wait(full((int)st), ph, work.status) && !*abort_flag;
-        if (!ok) break;
-        tc_fence_after();
-        const int n = unit_slot[i & 7];
-        const bool a_mn = A_MODE == 1 || (A_MODE == 2 && n < 0);
-        block(acc, a_mn, 0u);
-        for (int kb = abs(n) - 1; kb > 0; --kb) {
-          if (!mbar_wait(full((int)st), ph, work.status)) {
-            ok = false;
-            break;
-          }
+        int left = 0;
+        bool a_mn = false;
+        if constexpr (NH == 1) {
+          const uint32_t acc = tmem + (uint32_t)((i & 1) * BN);
+          if (i >= 2) ok = mbar_wait(tempty(i & 1), ((i >> 1) - 1) & 1, work.status);
+          if (ok) ok = mbar_wait(full((int)st), ph, work.status) && !*abort_flag;
+          if (!ok) break;
           tc_fence_after();
-          block(acc, a_mn, 1u);
+          const int n = unit_slot[i & 7];
+          a_mn = A_MODE == 1 || (A_MODE == 2 && n < 0);
+          mmas(acc, st, 0, a_mn, 0u);
+          release();
+          for (left = abs(n) - 1; left > 0; --left) {
+            if (!mbar_wait(full((int)st), ph, work.status)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            mmas(acc, st, 0, a_mn, 1u);
+            release();
+          }
+        } else {
+          // Both accumulators are one tile's. The epilogue frees the first half of the columns
+          // before the second: the first K blocks go into the first half alone, up to one stage
+          // short of the ring, and are kept for the second.
+          if (i >= 1) ok = mbar_wait(tempty(0), (i - 1) & 1, work.status);
+          if (ok) ok = mbar_wait(full((int)st), ph, work.status) && !*abort_flag;
+          if (!ok) break;
+          tc_fence_after();
+          const int n = unit_slot[i & 7];
+          a_mn = A_MODE == 1 || (A_MODE == 2 && n < 0);
+          const int lead = min(abs(n), C::STAGES - 1);
+          uint32_t at = st, pt = ph;
+          for (int j = 0; j < lead; ++j) {
+            if (j > 0) {
+              ok = mbar_wait(full((int)at), pt, work.status);
+              if (!ok) break;
+              tc_fence_after();
+            }
+            mmas(tmem, at, 0, a_mn, j ? 1u : 0u);
+            if (++at == C::STAGES) at = 0, pt ^= 1;
+          }
+          if (ok && i >= 1) ok = mbar_wait(tempty(1), (i - 1) & 1, work.status);
+          if (!ok) break;
+          tc_fence_after();
+          for (int j = 0; j < lead; ++j) {
+            mmas(tmem + BN, st, 1, a_mn, j ? 1u : 0u);
+            release();
+          }
+          for (left = abs(n) - lead; left > 0; --left) {
+            if (!mbar_wait(full((int)st), ph, work.status)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            mmas(tmem, st, 0, a_mn, 1u);
+            mmas(tmem + BN, st, 1, a_mn, 1u);
+            release();
+          }
         }
-        if (ok) mma_commit_cg<CG>(tfull(i & 1));
+        if (ok) mma_commit_cg<CG>(tfull(NH == 1 ? i & 1 : 0));
       }
       if (!ok) *abort_flag = 1;
       mma_commit_cg<CG>(bar_end);  // every MMA retires before TMEM and shared memory are released
@@ -487,22 +541,29 @@ __global__ void __launch_bounds__(320, 1)
       const bool second = A_MODE == 2 && which == 1;
       const GemmUnit w = gemm_unit(work.g[second ? 1 : 0], u);
       if (!e.failed) {
-        const bool ok = mbar_wait(tfull(i & 1), (i >> 1) & 1, work.status);
+        const bool ok = NH == 1 ? mbar_wait(tfull(i & 1), (i >> 1) & 1, work.status)
+                                : mbar_wait(tfull(0), i & 1, work.status);
         if (!__all_sync(0xffffffffu, ok && !*abort_flag)) {
           e.failed = true;
           *abort_flag = 1;
         }
         tc_fence_after();
       }
-      e.taddr = tmem + ((uint32_t)(e.quad * 32) << 16) + (uint32_t)((i & 1) * BN);
       e.turn = i;
       e.row0 = (w.mt * CG + (int)rank) * C::BM + e.quad * 32;
-      Epi::tile(second ? ea1 : ea0, w, e);
-      tc_fence_before();
-      __syncwarp();
-      if (!e.failed && lane == 0) {
-        if constexpr (CG == 2) mbar_arrive_cluster(map_rank(tempty(i & 1), 0));
-        else mbar_arrive(tempty(i & 1));
+#pragma unroll 1
+      for (int h = 0; h < NH; ++h) {
+        const int buf = NH == 1 ? i & 1 : h;
+        e.taddr = tmem + ((uint32_t)(e.quad * 32) << 16) + (uint32_t)(buf * BN);
+        GemmUnit wh = w;
+        wh.nt = w.nt * NH + h;
+        Epi::tile(second ? ea1 : ea0, wh, e);
+        tc_fence_before();
+        __syncwarp();
+        if (!e.failed && lane == 0) {
+          if constexpr (CG == 2) mbar_arrive_cluster(map_rank(tempty(buf), 0));
+          else mbar_arrive(tempty(buf));
+        }
       }
     }
   }
@@ -569,9 +630,9 @@ struct GemmProduct {
   typename Epi::Args ea;
 };
 
-template <class Epi, int CG, int BN, int A_MODE, bool B_MN, bool BF16>
+template <class Epi, int CG, int BN, int NH, int A_MODE, bool B_MN, bool BF16>
 int launch_gemm(const GemmProduct<Epi>& p0, const GemmProduct<Epi>* p1, cudaStream_t st) {
-  using C = GemmCfg<CG, BN>;
+  using C = GemmCfg<CG, BN, NH>;
   static_assert(A_MODE == 2 || A_MODE == 0 || A_MODE == 1, "layout of A");
   constexpr int dtype = BF16 ? SSA_DTYPE_BF16 : SSA_DTYPE_F16;
   CUtensorMap t[4];
@@ -602,7 +663,7 @@ int launch_gemm(const GemmProduct<Epi>& p0, const GemmProduct<Epi>* p1, cudaStre
   }
   w.status = device_status_ptr();
   if (!w.status) return abi_error(SSA_ERR_CUDA, "cannot resolve the device status word");
-  auto kern = gemm_sm100_kernel<Epi, CG, BN, A_MODE, B_MN, BF16>;
+  auto kern = gemm_sm100_kernel<Epi, CG, BN, NH, A_MODE, B_MN, BF16>;
   if (set_smem_limit_once(reinterpret_cast<const void*>(kern), (int)C::SMEM_BYTES) != SSA_OK)
     return abi_error(SSA_ERR_CUDA, "cannot raise the shared memory limit");
   const int most = device_sm_count() / CG;
@@ -629,15 +690,29 @@ int launch_gemm(const GemmProduct<Epi>& p0, const GemmProduct<Epi>* p1, cudaStre
 inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 inline size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// Tile form: the pair's 256 x 256 tiles once they fill the clusters, else 128 x 128 tiles. Measured
-// on B200: see the callers.
+// Tile form of the products with a fused epilogue: the pair's 256 x 256 tiles once they fill the
+// clusters, else 128 x 128 tiles.
 struct GemmForm {
   bool pair;
   int bm, bn, workers;
+  bool wide;  // gradients: 256 x 512 tiles
 };
 inline GemmForm gemm_form(int64_t tiles_256) {
   const bool pair = tiles_256 >= kPlanSms / 2;
-  return pair ? GemmForm{true, 256, 256, kPlanSms / 2} : GemmForm{false, 128, 128, kPlanSms};
+  return pair ? GemmForm{true, 256, 256, kPlanSms / 2, false}
+              : GemmForm{false, 128, 128, kPlanSms, false};
+}
+
+// Tile form of dx [rows, hidden] (kx K blocks) and dW [cols, hidden] (kw K blocks): 256 x 512 tiles,
+// which read a quarter less per operation, when they fill the clusters and their K loop is long
+// against an epilogue that no longer runs under the next tile's MMAs.
+inline GemmForm gradient_form(int64_t rows, int64_t cols, int hidden, int kx, int kw) {
+  const int64_t dx = (int64_t)cdiv(rows, 256) * cdiv(hidden, 256);
+  const int64_t dw = (int64_t)cdiv(cols, 256) * cdiv(hidden, 256);
+  GemmForm f = gemm_form(dx > dw ? dx : dw);
+  f.wide = f.pair && hidden > 256 && dx + dw >= 2 * f.workers && kx >= 64 && kw >= 64;
+  if (f.wide) f.bn = 512;
+  return f;
 }
 
 // Row tiles walked before the column advances: all of them while that operand's panel stays in L2
@@ -687,8 +762,8 @@ struct StoreProduct {
 };
 
 // dx = d W (d K-major) and dW = d^T x (d MN-major), B MN-major in both: one launch for both, or either
-// alone where the other is nullptr. `pair`: the tile form (GemmForm::pair).
-int launch_gradients(bool bf16, bool pair, const StoreProduct* dx, const StoreProduct* dw,
+// alone where the other is nullptr.
+int launch_gradients(bool bf16, const GemmForm& form, const StoreProduct* dx, const StoreProduct* dw,
                      cudaStream_t st);
 
 // out[row, col] = scale * (the splits' sums [splits][rows][cols], added in split order).

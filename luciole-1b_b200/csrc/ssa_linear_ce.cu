@@ -256,9 +256,7 @@ CePlan ce_plan(const ssa_linear_ce_t* p) {
   q.pieces = cdiv(all, cols);
   q.ldd = (int64_t)cdiv(all / 256, q.pieces) * 256;  // pieces of about equal width
   q.pieces = cdiv(all, q.ldd);
-  const int64_t dx256 = (int64_t)cdiv(rows, 256) * cdiv(p->hidden, 256);
-  const int64_t dw256 = (q.ldd / 256) * cdiv(p->hidden, 256);
-  q.bwd = gemm_form(dx256 > dw256 ? dx256 : dw256);
+  q.bwd = gradient_form(rows, q.ldd, p->hidden, (int)(q.ldd / 64), cdiv(rows, 64));
   const int64_t dx_tiles = (int64_t)cdiv(rows, q.bwd.bm) * cdiv(p->hidden, q.bwd.bn);
   const int64_t dw_tiles = (int64_t)cdiv(q.ldd, q.bwd.bm) * cdiv(p->hidden, q.bwd.bn);
   q.dx_splits = split_count(dx_tiles, (int)(q.ldd / 64), dw_tiles * (cdiv(rows, 64) + kTileCost),
@@ -303,8 +301,8 @@ int ce_logits(const ssa_linear_ce_t* p, const GemmForm& f, const void* w, int64_
   const GemmOperand B{w, cols, p->hidden, p->w_stride, "w"};
   const GemmShape g = plain_shape(cdiv(p->rows, f.bm), tiles_n, cdiv(p->hidden, 64),
                                   2 * (int64_t)p->rows * p->hidden);
-  return f.pair ? launch_gemm<Epi256, 2, 256, 0, false, BF16>({A, B, g, a}, nullptr, st)
-                : launch_gemm<Epi128, 1, 128, 0, false, BF16>({A, B, g, a}, nullptr, st);
+  return f.pair ? launch_gemm<Epi256, 2, 256, 1, 0, false, BF16>({A, B, g, a}, nullptr, st)
+                : launch_gemm<Epi128, 1, 128, 1, 0, false, BF16>({A, B, g, a}, nullptr, st);
 }
 
 template <bool BF16>
@@ -373,7 +371,7 @@ int ce_bwd(const ssa_linear_ce_t* p, const CePlan& q, const float* lse, const fl
     const GemmOperand wb{w0, p->hidden, cols, p->w_stride, "w"};
     const GemmOperand xb{p->x, p->hidden, p->rows, p->x_stride, "x"};
     const StoreProduct px{dk, wb, gx, sx}, pw{dmn, xb, gw, sw};
-    rc = launch_gradients(BF16, q.bwd.pair, dx ? &px : nullptr, dw ? &pw : nullptr, st);
+    rc = launch_gradients(BF16, q.bwd, dx ? &px : nullptr, dw ? &pw : nullptr, st);
     if (rc != SSA_OK) return rc;
   }
   if (dx && q.dx_splits > 1)
