@@ -19,50 +19,62 @@ int device_sm_count() {
 
 namespace {
 
+// The epilogue is kept short: in the 256 x 512 form the next tile's MMAs wait for half of it. The next
+// 32 columns are on their way from TMEM while the last ones are stored; 16-bit results are rounded
+// before the exchange; a later piece's sum goes out as fp32 reductions, which wait for nothing (one
+// addition per element and launch: the order, and so the sum, is fixed by the stream).
 template <int BN, bool BF16>
 struct EpiStore {
   using Args = StoreArgs;
   __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, const EpiCtx& e) {
     const float sc = a.scale ? __ldg(a.scale) : 1.f;
     const int col0 = w.nt * BN + e.half * (BN / 2);
+    const int n = min(BN / 2, ((a.cols - col0 + 31) >> 5) << 5);  // columns of this warp, whole 32s
+    if (n <= 0) return;
+    uint32_t x[32];
+    e.fetch(e.half * (BN / 2), x);
 #pragma unroll 1
-    for (int c = 0; c < BN / 2; c += 32) {
+    for (int c = 0; c < n; c += 32) {
       const int col = col0 + c;
-      if (col >= a.cols) break;
       float v[32];
-      e.read(e.half * (BN / 2) + c, v);
+      e.settle(x, v);
+      if (c + 32 < n) e.fetch(e.half * (BN / 2) + c + 32, x);
+      if (a.out) {
 #pragma unroll
-      for (int p = 0; p < 8; ++p)
-        *exch32(e.exch, e.lane, p) = make_float4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
-      __syncwarp();
-      // four lanes per row, 8 columns each
-      const int q = e.lane & 3, my = col + 8 * q;
+        for (int i = 0; i < 32; ++i) v[i] *= sc;
+        put_row16<BF16>(e, v);
+        __syncwarp();
+        const int p = e.lane & 3, my = col + 8 * p;
 #pragma unroll
-      for (int it = 0; it < 4; ++it) {
-        const int r = it * 8 + (e.lane >> 2);
-        const int64_t row = (int64_t)e.row0 + r;
-        float4 x = *exch32(e.exch, r, 2 * q), y = *exch32(e.exch, r, 2 * q + 1);
-        bool ok = row < a.rows && my < a.cols;
-        int64_t orow = row;
-        if (a.jump_at) {
-          const int64_t in = row < a.jump_at ? row : row - a.jump_at;
-          ok = ok && in < a.jump_rows;
-          orow = row < a.jump_at ? row : a.jump + in;
+        for (int it = 0; it < 4; ++it) {
+          const int r = it * 8 + (e.lane >> 2);
+          const int row = e.row0 + r;
+          int64_t orow = row;
+          bool ok = row < a.rows && my < a.cols;
+          if (a.jump_at) {
+            const int in = row < a.jump_at ? row : row - a.jump_at;
+            ok = ok && in < a.jump_rows;
+            orow = row < a.jump_at ? row : (int64_t)a.jump + in;
+          }
+          if (ok)
+            *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + orow * a.ldo + my) =
+                *exch16(e.exch, r, p);
         }
-        if (!ok) continue;
-        float4* sp = reinterpret_cast<float4*>(
-            a.sum + ((int64_t)w.sp * a.rows + row) * a.cols + my);
-        if (a.add_prev) {
-          const float4 b = sp[0], d = sp[1];
-          x.x += b.x, x.y += b.y, x.z += b.z, x.w += b.w;
-          y.x += d.x, y.y += d.y, y.z += d.z, y.w += d.w;
+      } else {
+#pragma unroll
+        for (int p = 0; p < 8; ++p)
+          *exch32(e.exch, e.lane, p) = make_float4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
+        __syncwarp();
+        const int p = e.lane & 7, my = col + 4 * p;
+#pragma unroll
+        for (int it = 0; it < 8; ++it) {
+          const int r = it * 4 + (e.lane >> 3);
+          const int row = e.row0 + r;
+          if (row >= a.rows || my >= a.cols) continue;
+          float4* to = reinterpret_cast<float4*>(a.sum + ((int64_t)w.sp * a.rows + row) * a.cols + my);
+          if (a.add_prev) atomicAdd(to, *exch32(e.exch, r, p));
+          else *to = *exch32(e.exch, r, p);
         }
-        if (a.out)
-          *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + orow * a.ldo + my) =
-              make_uint4(pack2<BF16>(x.x * sc, x.y * sc), pack2<BF16>(x.z * sc, x.w * sc),
-                         pack2<BF16>(y.x * sc, y.y * sc), pack2<BF16>(y.z * sc, y.w * sc));
-        else
-          sp[0] = x, sp[1] = y;
       }
       __syncwarp();
     }

@@ -225,6 +225,16 @@ struct EpiCtx {
   int lane, quad, half, turn;
   int row0;         // global row of lane 0
 
+  // The same in two steps, with other work between them.
+  __device__ __forceinline__ void fetch(int col, uint32_t (&r)[32]) const {
+    if (!failed) tmem_ld32(taddr + (uint32_t)col, r);
+  }
+  __device__ __forceinline__ void settle(uint32_t (&r)[32], float (&v)[32]) const {
+    if (!failed) tmem_ld_wait(r);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = failed ? nan_f32() : __uint_as_float(r[i]);
+  }
+
   // Accumulator columns [col, col + 32) of this lane's row (every lane of the warp calls it).
   __device__ __forceinline__ void read(int col, float (&v)[32]) const {
     if (failed) {
@@ -742,15 +752,15 @@ inline int split_count(int64_t tiles, int kblocks, int64_t other, int workers) {
 }
 
 // ------------------------------------------------------------------------- plain store epilogue
-// out = (acc + earlier partial sum) * scale in 16 bits, or the running fp32 sum itself. `sum` holds
-// one [rows, cols] fp32 matrix per split; adding to it across launches is ordered by the stream.
+// out = acc * scale in 16 bits, or with out == nullptr the fp32 sum: one [rows, cols] matrix per split,
+// written, or added to (a later piece of the same contraction).
 struct StoreArgs {
-  void* out;             // 16-bit [.., ldo], or nullptr: keep the sum in fp32
+  void* out;             // 16-bit [.., ldo], or nullptr
   float* sum;            // fp32 [splits][rows][cols], or nullptr
   const float* scale;    // device scalar, or nullptr (1)
   int64_t ldo;
   int rows, cols;        // cols: a multiple of 8
-  int add_prev;          // add the matching element of sum
+  int add_prev;          // add to sum
   int jump_at, jump;     // rows >= jump_at are stored at jump + row - jump_at; rows in
   int jump_rows;         //   [jump_rows, jump_at) and past jump_at + jump_rows are dropped
 };

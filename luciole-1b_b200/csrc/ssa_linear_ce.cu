@@ -352,7 +352,7 @@ int ce_bwd(const ssa_linear_ce_t* p, const CePlan& q, const float* lse, const fl
     if (rc != SSA_OK) return rc;
 
     StoreArgs sx{}, sw{};
-    sx.out = q.dx_splits == 1 && i == q.pieces - 1 ? dx : nullptr;
+    sx.out = q.dx_splits == 1 && q.pieces == 1 ? dx : nullptr;
     sx.sum = sum;
     sx.scale = sw.scale = inv;
     sx.rows = p->rows;
@@ -374,7 +374,7 @@ int ce_bwd(const ssa_linear_ce_t* p, const CePlan& q, const float* lse, const fl
     rc = launch_gradients(BF16, q.bwd, dx ? &px : nullptr, dw ? &pw : nullptr, st);
     if (rc != SSA_OK) return rc;
   }
-  if (dx && q.dx_splits > 1)
+  if (dx && (q.dx_splits > 1 || q.pieces > 1))
     return launch_sum_splits(BF16, sum, dx, inv, p->rows, p->hidden, p->hidden, q.dx_splits, st);
   return SSA_OK;
 }
