@@ -16,8 +16,10 @@ __all__ = ["SSAQKNormRopeFunc", "ssa_qk_norm_rope"]
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """`t` if its last dimension is contiguous and its base and other strides are 16-byte aligned,
+    """`t` [.., D] if its last dimension is contiguous and its base and other strides are 16-byte aligned,
     else a copy in fresh storage."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t  # D is a multiple of 16
     if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
             s * t.element_size() % 16 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
         return t
@@ -26,8 +28,8 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 def _tensor(t: torch.Tensor) -> _lib.SsaTensor:
     """[B, S, H, D] as the library's strided [B, H, S, D]; strides of extent 1 are never used."""
-    st = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
-    return _lib.SsaTensor(t.data_ptr(), st[0], st[2], st[1])
+    (b, s, h, _), (sb, ss, sh, _) = t.shape, t.stride()
+    return _lib.SsaTensor(t.data_ptr(), sb if b > 1 else 0, sh if h > 1 else 0, ss if s > 1 else 0)
 
 
 def _problem(x, hq, hkv, cos, sin, pos, pos_stride, wq, wk, eps):
@@ -44,7 +46,7 @@ def _forward(qkv, q_weight, k_weight, cos, sin, positions, hq, hkv, eps):
     """q, k, v, the tensors the backward needs, and the stride between sequences' positions."""
     d = cos.shape[1]
     lead = qkv.shape[:-1]
-    heads = qkv.unflatten(-1, (hq + 2 * hkv, d))
+    heads = qkv.view(*lead, hq + 2 * hkv, d)
     x = _aligned(heads if len(lead) == 2 else heads.unsqueeze(0))
     cos, sin = _lib.table(cos), _lib.table(sin)
     pos, pos_stride = positions, 0

@@ -5,7 +5,7 @@
 // Bound: memory. The norm reads every gradient once; the scaling needs the norm, so it reads them
 // again and writes once. The tensors' addresses and sizes travel in the kernels' parameter block
 // (no table copy to the device, nothing to keep alive, capturable as it is), up to kTable tensors
-// per launch. Work is cut into chunks of kChunk elements, one block each; the second pass walks the
+// per launch. Work is cut into chunks of 64 KB, one block each; the second pass walks the
 // chunks from the last to the first, so that what the first pass read last is still in L2.
 //
 // Squares are added in fp32 over a thread's few elements of a chunk and in fp64 from there on, in
@@ -23,9 +23,9 @@ namespace ssa {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kUnit = 8;                          // elements a thread takes at a time
-constexpr int kUnits = 4;                         // times it does so per chunk
-constexpr int kChunk = kThreads * kUnit * kUnits;
+constexpr int kLoads = 8;                         // 16-byte loads a thread has under way per chunk
+template <typename T>
+constexpr int kChunkOf = kThreads * kLoads * 16 / (int)sizeof(T);  // elements: 64 KB
 
 struct TableEntry {
   const void* in;
@@ -42,31 +42,22 @@ struct Table {
   TableEntry t[kTable];
 };
 
+// Four elements of a thread: 8 or 16 bytes, so that a warp's accesses are contiguous on both sides when
+// 16-bit gradients are written as fp32.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  } else {
-    const uint4 x = *reinterpret_cast<const uint4*>(p);
-    const T* h = reinterpret_cast<const T*>(&x);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(h[i]);
-  }
+struct Four {
+  T v[4];
+};
+template <typename T>
+__device__ __forceinline__ Four<T> load4(const T* p) {
+  using W = typename std::conditional<sizeof(T) == 4, uint4, uint2>::type;
+  const W x = *reinterpret_cast<const W*>(p);
+  return *reinterpret_cast<const Four<T>*>(&x);
 }
-
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-    uint4 x;
-    T* h = reinterpret_cast<T*>(&x);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = from_f32<T>(v[i]);
-    *reinterpret_cast<uint4*>(p) = x;
-  }
+__device__ __forceinline__ void store4(T* p, const Four<T>& f) {
+  using W = typename std::conditional<sizeof(T) == 4, uint4, uint2>::type;
+  __stcs(reinterpret_cast<W*>(p), *reinterpret_cast<const W*>(&f));  // not read again here
 }
 
 // The tensor of a chunk: the last entry whose first chunk is not past it.
@@ -81,78 +72,98 @@ __device__ __forceinline__ int find_tensor(const Table<kTable>& t, int chunk) {
   return lo;
 }
 
+// A thread's elements of a chunk again, in fp64 (from memory: the rare case costs no registers).
+template <typename T>
+__device__ __noinline__ double sum_squares_64(const T* in, int64_t first, int64_t n) {
+  constexpr int E = 16 / (int)sizeof(T);
+  double d = 0.0;
+  for (int u = 0; u < kLoads; ++u)
+    for (int i = 0; i < E; ++i) {
+      const int64_t at = first + (int64_t)u * kThreads * E + i;
+      if (at < n) d = fma((double)to_f32<T>(in[at]), (double)to_f32<T>(in[at]), d);
+    }
+  return d;
+}
+
 template <typename T, int kTable>
 __global__ void __launch_bounds__(kThreads)
     sum_squares_kernel(const __grid_constant__ Table<kTable> tab, double* part) {
+  constexpr int E = 16 / (int)sizeof(T);  // elements of a 16-byte load
   __shared__ double red[kThreads / 32];
   sm100::griddep_wait();
   sm100::griddep_launch_dependents();
   const TableEntry& e = tab.t[find_tensor(tab, (int)blockIdx.x)];
-  const int64_t base = (int64_t)((int)blockIdx.x - e.first) * kChunk;
+  const int64_t base = (int64_t)((int)blockIdx.x - e.first) * kChunkOf<T>;
   const T* in = reinterpret_cast<const T*>(e.in);
-  float v[kUnits][kUnit];
+  uint4 raw[kLoads];
+  if (e.vec && base + kChunkOf<T> <= e.n) {
+    const uint4* p = reinterpret_cast<const uint4*>(in + base) + threadIdx.x;
 #pragma unroll
-  for (int u = 0; u < kUnits; ++u) {
-    const int64_t at = base + ((int64_t)u * kThreads + threadIdx.x) * kUnit;
-    if (e.vec && at + kUnit <= e.n) {
-      load8(in + at, v[u]);
-    } else {
+    for (int u = 0; u < kLoads; ++u) raw[u] = p[u * kThreads];
+  } else {
 #pragma unroll
-      for (int i = 0; i < kUnit; ++i) v[u][i] = at + i < e.n ? to_f32<T>(in[at + i]) : 0.f;
+    for (int u = 0; u < kLoads; ++u) {
+      const int64_t at = base + (int64_t)(u * kThreads + (int)threadIdx.x) * E;
+      T* t = reinterpret_cast<T*>(&raw[u]);
+#pragma unroll
+      for (int i = 0; i < E; ++i) t[i] = at + i < e.n ? in[at + i] : from_f32<T>(0.f);
     }
   }
   float s = 0.f;
 #pragma unroll
-  for (int u = 0; u < kUnits; ++u)
+  for (int u = 0; u < kLoads; ++u) {
+    const T* t = reinterpret_cast<const T*>(&raw[u]);
+    float q = 0.f;
 #pragma unroll
-    for (int i = 0; i < kUnit; ++i) s = fmaf(v[u][i], v[u][i], s);
+    for (int i = 0; i < E; ++i) q = fmaf(to_f32<T>(t[i]), to_f32<T>(t[i]), q);
+    s += q;
+  }
   double d = (double)s;
-  // fp32 squares overflow above 1.8e19 and lose digits below 1e-18 or so
+  // fp32 squares overflow above 1.8e19 and lose digits below 1e-18 or so. All zero (rows of an
+  // embedding that no token reached): nothing to redo.
   if (!(s < 3.0e38f) || s < 1.0e-30f) {
-    d = 0.0;
-    float top = 0.f;  // all zero (rows of an embedding that no token reached): nothing to redo
+    uint32_t any = 0;
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u)
-#pragma unroll
-      for (int i = 0; i < kUnit; ++i) top = v[u][i] == 0.f ? top : 1.f;
-    if (top != 0.f) {
-#pragma unroll
-      for (int u = 0; u < kUnits; ++u)
-#pragma unroll
-        for (int i = 0; i < kUnit; ++i) d = fma((double)v[u][i], (double)v[u][i], d);
-    }
+    for (int u = 0; u < kLoads; ++u) any |= raw[u].x | raw[u].y | raw[u].z | raw[u].w;
+    if (any) d = sum_squares_64<T>(in, base + (int64_t)threadIdx.x * E, e.n);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = d;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < kThreads / 32; ++i) d += red[i];
-    part[blockIdx.x] = d;
+  if (threadIdx.x < 32) {
+    d = threadIdx.x < kThreads / 32 ? red[threadIdx.x] : 0.0;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+    if (threadIdx.x == 0) part[blockIdx.x] = d;
   }
 }
 
 // norm = sqrt of the chunks' sums, coef = min(1, max_norm / (norm + 1e-6)); NaN stays NaN.
 __global__ void __launch_bounds__(1024) norm_kernel(const double* part, int64_t n, float max_norm,
                                                     float* norm, float* coef) {
-  __shared__ double red[1024];
+  __shared__ double red[32];
   sm100::griddep_wait();
   sm100::griddep_launch_dependents();
-  double s[4] = {0.0, 0.0, 0.0, 0.0};
-  int64_t i = threadIdx.x;
-  for (; i + 3 * 1024 < n; i += 4 * 1024) {
+  double s[8] = {};
+  for (int64_t i = threadIdx.x; i < n; i += 8 * 1024) {
+    double x[8];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) s[k] += part[i + k * 1024];
+    for (int k = 0; k < 8; ++k) x[k] = i + k * 1024 < n ? part[i + k * 1024] : 0.0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s[k] += x[k];
   }
-  for (; i < n; i += 1024) s[0] += part[i];
-  red[threadIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
+  double d = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = d;
   __syncthreads();
-  for (int o = 512; o > 0; o >>= 1) {
-    if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
-    __syncthreads();
-  }
+  if (threadIdx.x >= 32) return;
+  d = red[threadIdx.x];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
   if (threadIdx.x == 0) {
-    const float r = (float)sqrt(red[0]);
+    const float r = (float)sqrt(d);
     *norm = r;
     if (coef) {
       const float c = max_norm / (r + 1e-6f);
@@ -170,36 +181,32 @@ __global__ void __launch_bounds__(kThreads)
   const int chunk = tab.chunks - 1 - (int)blockIdx.x;  // last chunk first: its data is still in L2
   const TableEntry& e = tab.t[find_tensor(tab, chunk)];
   if (c == 1.f && e.in == e.out) return;  // in place and nothing to scale
-  const int64_t base = (int64_t)(chunk - e.first) * kChunk;
+  const int64_t base = (int64_t)(chunk - e.first) * kChunkOf<T>;
   const T* in = reinterpret_cast<const T*>(e.in);
   O* out = reinterpret_cast<O*>(e.out);
-  float v[kUnits][kUnit];
+  constexpr int N = kChunkOf<T> / (4 * kThreads);
+  if (e.vec && base + kChunkOf<T> <= e.n) {
+    Four<T> x[N];
 #pragma unroll
-  for (int u = 0; u < kUnits; ++u) {
-    const int64_t at = base + ((int64_t)u * kThreads + threadIdx.x) * kUnit;
-    if (e.vec && at + kUnit <= e.n) {
-      load8(in + at, v[u]);
-    } else {
+    for (int u = 0; u < N; ++u) x[u] = load4(in + base + (u * kThreads + (int)threadIdx.x) * 4);
 #pragma unroll
-      for (int i = 0; i < kUnit; ++i) v[u][i] = at + i < e.n ? to_f32<T>(in[at + i]) : 0.f;
+    for (int u = 0; u < N; ++u) {
+      Four<O> y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y.v[i] = from_f32<O>(to_f32<T>(x[u].v[i]) * c);
+      store4(out + base + (u * kThreads + (int)threadIdx.x) * 4, y);
     }
-  }
-#pragma unroll
-  for (int u = 0; u < kUnits; ++u) {
-    const int64_t at = base + ((int64_t)u * kThreads + threadIdx.x) * kUnit;
-#pragma unroll
-    for (int i = 0; i < kUnit; ++i) v[u][i] *= c;
-    if (e.vec && at + kUnit <= e.n) {
-      store8(out + at, v[u]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kUnit; ++i)
-        if (at + i < e.n) out[at + i] = from_f32<O>(v[u][i]);
-    }
+  } else {
+    const int64_t end = base + kChunkOf<T> < e.n ? base + kChunkOf<T> : e.n;
+    for (int64_t i = base + threadIdx.x; i < end; i += kThreads)
+      out[i] = from_f32<O>(to_f32<T>(in[i]) * c);
   }
 }
 
-int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
+int64_t chunks_of(int dtype, int64_t n) {
+  const int64_t c = dtype == SSA_DTYPE_F32 ? kChunkOf<float> : kChunkOf<__half>;
+  return (n + c - 1) / c;
+}
 
 // One launch for tensors [i0, i1) of the list.
 template <typename T, typename O, int kTable, bool SCALE>
@@ -216,7 +223,7 @@ int launch_table(const ssa_grad_list_t* l, int i0, int i1, double* part, const f
     e.n = l->sizes[i];
     e.first = (int32_t)chunks;
     e.vec = ((uintptr_t)e.in | (SCALE ? (uintptr_t)e.out : 0)) % 16 == 0;
-    chunks += chunks_of(e.n);
+    chunks += chunks_of(l->dtype, e.n);
   }
   if (!chunks) return SSA_OK;
   tab.chunks = (int32_t)chunks;
@@ -247,7 +254,7 @@ int walk(const ssa_grad_list_t* l, double* part, const float* coef, cudaStream_t
                        : launch_table<T, O, 768, SCALE>(l, i0, i1, part + done, coef, st);
     if (rc != SSA_OK) return rc;
     if (!SCALE)
-      for (int i = i0; i < i1; ++i) done += chunks_of(l->sizes[i]);
+      for (int i = i0; i < i1; ++i) done += chunks_of(l->dtype, l->sizes[i]);
   }
   return SSA_OK;
 }
@@ -269,7 +276,7 @@ int walk_types(const ssa_grad_list_t* l, double* part, const float* coef, cudaSt
 
 int64_t total_chunks(const ssa_grad_list_t* l) {
   int64_t n = 0;
-  for (int i = 0; i < l->count; ++i) n += chunks_of(l->sizes[i]);
+  for (int i = 0; i < l->count; ++i) n += chunks_of(l->dtype, l->sizes[i]);
   return n;
 }
 

@@ -76,8 +76,15 @@ struct EpiCeFwd {
   }
 };
 
-// Joins the tiles' pairs: 32 rows per block (one per lane), 32 warps that each walk every 32nd
-// tile. lse in natural units; loss 0 where the target is ignored, NaN where it is out of range.
+__device__ __forceinline__ void join_pair(float& m, float& s, float2 p) {
+  const float mn = fmaxf(m, p.x);
+  s = s * ex2_approx((m - mn) * kLog2e) + p.y * ex2_approx((p.x - mn) * kLog2e);
+  m = mn;
+}
+
+// Joins the tiles' pairs: 32 rows per block (one per lane), 32 warps that each walk every 32nd tile
+// (four loads under way at a time), then a warp per row. lse in natural units; loss 0 where the
+// target is ignored, NaN where it is out of range.
 __global__ void __launch_bounds__(1024)
     ce_join_kernel(const float2* part, const float* target_logit, const int64_t* targets,
                    int64_t ignore_index, int rows, int vocab, int tiles, float* lse, float* loss) {
@@ -88,61 +95,74 @@ __global__ void __launch_bounds__(1024)
   const int row = blockIdx.x * 32 + lane;
   float m = kLowest, s = 0.f;
   if (row < rows)
-    for (int i = y; i < tiles; i += 32) {
-      const float2 p = part[(int64_t)i * rows + row];
-      const float mn = fmaxf(m, p.x);
-      s = s * ex2_approx((m - mn) * kLog2e) + p.y * ex2_approx((p.x - mn) * kLog2e);
-      m = mn;
+    for (int i = y; i < tiles; i += 128) {
+      float2 p[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        p[k] = i + 32 * k < tiles ? part[(int64_t)(i + 32 * k) * rows + row] : make_float2(kLowest, 0.f);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) join_pair(m, s, p[k]);
     }
   sh[y][lane] = make_float2(m, s);
   __syncthreads();
-  if (y == 0 && row < rows) {
-    for (int i = 1; i < 32; ++i) {
-      const float2 p = sh[i][lane];
-      const float mn = fmaxf(m, p.x);
-      s = s * ex2_approx((m - mn) * kLog2e) + p.y * ex2_approx((p.x - mn) * kLog2e);
-      m = mn;
-    }
+  const float2 p = sh[lane][y];
+  m = p.x, s = p.y;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float2 q = make_float2(__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
+    join_pair(m, s, q);
+  }
+  const int r = blockIdx.x * 32 + y;
+  if (lane == 0 && r < rows) {
     const float ls = logf(s);
-    lse[row] = m + ls;
-    const int64_t t = targets[row];
+    lse[r] = m + ls;
+    const int64_t t = targets[r];
     // (m - l_t) + log s: no cancellation between a large lse and a large logit
-    loss[row] = t == ignore_index ? 0.f
-                : (t < 0 || t >= vocab) ? nan_f32()
-                                        : (m - target_logit[row]) + ls;
+    loss[r] = t == ignore_index ? 0.f
+              : (t < 0 || t >= vocab) ? nan_f32()
+                                      : (m - target_logit[r]) + ls;
   }
 }
 
-// Sum over a block of 1024 threads in a fixed order.
+// Sum over a block of 1024 threads in a fixed order; the result in thread 0.
 __device__ __forceinline__ double block_sum_1024(double v, double* red) {
-  red[threadIdx.x] = v;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  for (int o = 512; o > 0; o >>= 1) {
-    if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
-    __syncthreads();
-  }
-  const double t = red[0];
+  v = threadIdx.x < 32 ? red[threadIdx.x] : 0.0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   __syncthreads();
-  return t;
+  return v;
 }
 
 // Sum of the rows' losses in 64 bits (mean: over the rows that are not ignored), and that count.
 __global__ void __launch_bounds__(1024)
     ce_total_kernel(const float* loss_rows, const int64_t* targets, int64_t ignore_index, int rows,
                     int mean, float* loss, float* count) {
-  __shared__ double red[1024];
+  __shared__ double red[32];
   griddep_wait();
   griddep_launch_dependents();
-  double s = 0.0, n = 0.0;
-  for (int i = threadIdx.x; i < rows; i += 1024) {
-    s += (double)loss_rows[i];
-    n += targets[i] != ignore_index ? 1.0 : 0.0;
+  double s = 0.0;
+  int n = 0;
+  for (int i = threadIdx.x; i < rows; i += 4096) {
+    float l[4];
+    int64_t t[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int at = i + 1024 * k;
+      l[k] = at < rows ? loss_rows[at] : 0.f;
+      t[k] = at < rows ? targets[at] : ignore_index;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s += (double)l[k], n += t[k] != ignore_index;
   }
   s = block_sum_1024(s, red);
-  n = block_sum_1024(n, red);
+  const double c = block_sum_1024((double)n, red);
   if (threadIdx.x == 0) {
-    *loss = (float)(mean ? s / n : s);
-    *count = (float)n;
+    *loss = (float)(mean ? s / c : s);
+    *count = (float)c;
   }
 }
 
@@ -159,22 +179,33 @@ __global__ void __launch_bounds__(1024)
   griddep_launch_dependents();
   const float n = mean ? *count : 1.f;
   float top = 0.f;
-  for (int i = threadIdx.x; i < rows; i += 1024)
-    if (targets[i] != ignore_index) top = fmaxf(top, fabsf(grad[per_row ? i : 0] / n));
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
-  __syncthreads();
-  top = red[threadIdx.x & 31];
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (per_row) {
+    for (int i = threadIdx.x; i < rows; i += 1024)
+      if (targets[i] != ignore_index) top = fmaxf(top, fabsf(grad[i] / n));
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+    __syncthreads();
+    top = red[threadIdx.x & 31];
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  } else {
+    top = fabsf(grad[0] / n);
+  }
   int e = 0;
   if (top > 0.f && top < INFINITY) e = max(-126, min(126, 11 - ilogbf(top)));
   const float up = ldexpf(1.f, e);
-  for (int i = threadIdx.x; i < rows; i += 1024) {
-    const int64_t t = targets[i];
-    float g = grad[per_row ? i : 0] / n * up;
-    if (t == ignore_index) g = 0.f;
-    else if (t < 0 || t >= vocab) g = nan_f32();
-    weight[i] = g;
+  for (int i = threadIdx.x; i < rows; i += 4096) {
+    int64_t t[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) t[k] = i + 1024 * k < rows ? targets[i + 1024 * k] : ignore_index;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int at = i + 1024 * k;
+      if (at >= rows) break;
+      float g = grad[per_row ? at : 0] / n * up;
+      if (t[k] == ignore_index) g = 0.f;
+      else if (t[k] < 0 || t[k] >= vocab) g = nan_f32();
+      weight[at] = g;
+    }
   }
   if (threadIdx.x == 0) *inv = ldexpf(1.f, -e);
 }

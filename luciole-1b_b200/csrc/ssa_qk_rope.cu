@@ -5,7 +5,7 @@
 //     dw = sum dn x r,  dx = r (dn w - x r mean(dn w x r))
 // Everything in fp32, one rounding at the end.
 //
-// Bound: memory. D / 16 lanes share a head; a lane holds 8 columns of the first half and the 8 they
+// Bound: memory. D / 8 lanes share a head; a lane holds 4 columns of the first half and the 4 they
 // rotate with, so the rotation needs no exchange and the norm a few shuffles. A lane walks kHeads
 // heads of one token with that token's cos and sin in registers (a table row is 4 to 8 times as wide
 // as a 16-bit head), all heads' loads issued before the first is used. Few tokens: one head each.
@@ -43,52 +43,44 @@ struct RopeArgs {
 };
 
 template <typename T>
-struct Row16 {  // a lane's 16 elements: 8 of each half
-  uint4 raw[sizeof(T) == 4 ? 4 : 2];
+using Words = typename std::conditional<sizeof(T) == 4, uint4, uint2>::type;  // four elements
+
+template <typename T>
+struct Row8 {  // a lane's elements of a head: 4 of each half
+  Words<T> a, b;
 };
 
 template <typename T>
-__device__ __forceinline__ Row16<T> load_row(const T* head, int lane, int D) {
-  Row16<T> r;
-  const uint4* a = reinterpret_cast<const uint4*>(head + lane * 8);
-  const uint4* b = reinterpret_cast<const uint4*>(head + D / 2 + lane * 8);
-  if constexpr (sizeof(T) == 4) {
-    r.raw[0] = __ldg(a), r.raw[1] = __ldg(a + 1), r.raw[2] = __ldg(b), r.raw[3] = __ldg(b + 1);
-  } else {
-    r.raw[0] = __ldg(a), r.raw[1] = __ldg(b);
-  }
-  return r;
+__device__ __forceinline__ Row8<T> load_row(const T* head, int lane, int D) {
+  return Row8<T>{__ldg(reinterpret_cast<const Words<T>*>(head + lane * 4)),
+                 __ldg(reinterpret_cast<const Words<T>*>(head + D / 2 + lane * 4))};
 }
 template <typename T>
-__device__ __forceinline__ void unpack(const Row16<T>& r, float (&a)[8], float (&b)[8]) {
-  const T* t = reinterpret_cast<const T*>(r.raw);
+__device__ __forceinline__ void unpack(const Row8<T>& r, float (&a)[4], float (&b)[4]) {
+  const T* x = reinterpret_cast<const T*>(&r.a);
+  const T* y = reinterpret_cast<const T*>(&r.b);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a[i] = to_f32<T>(t[i]), b[i] = to_f32<T>(t[8 + i]);
+  for (int i = 0; i < 4; ++i) a[i] = to_f32<T>(x[i]), b[i] = to_f32<T>(y[i]);
 }
 template <typename T>
-__device__ __forceinline__ void store_row(T* head, int lane, int D, const float (&a)[8],
-                                          const float (&b)[8]) {
-  Row16<T> r;
-  T* t = reinterpret_cast<T*>(r.raw);
+__device__ __forceinline__ void store_row(T* head, int lane, int D, const float (&a)[4],
+                                          const float (&b)[4]) {
+  Row8<T> r;
+  T* x = reinterpret_cast<T*>(&r.a);
+  T* y = reinterpret_cast<T*>(&r.b);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) t[i] = from_f32<T>(a[i]), t[8 + i] = from_f32<T>(b[i]);
-  uint4* pa = reinterpret_cast<uint4*>(head + lane * 8);
-  uint4* pb = reinterpret_cast<uint4*>(head + D / 2 + lane * 8);
-  if constexpr (sizeof(T) == 4) {
-    pa[0] = r.raw[0], pa[1] = r.raw[1], pb[0] = r.raw[2], pb[1] = r.raw[3];
-  } else {
-    pa[0] = r.raw[0], pb[0] = r.raw[1];
-  }
+  for (int i = 0; i < 4; ++i) x[i] = from_f32<T>(a[i]), y[i] = from_f32<T>(b[i]);
+  *reinterpret_cast<Words<T>*>(head + lane * 4) = r.a;
+  *reinterpret_cast<Words<T>*>(head + D / 2 + lane * 4) = r.b;
 }
 
-__device__ __forceinline__ void load8f(const float* p, float (&v)[8]) {
-  const float4 x = __ldg(reinterpret_cast<const float4*>(p)),
-               y = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+__device__ __forceinline__ void load4f(const float* p, float (&v)[4]) {
+  const float4 x = __ldg(reinterpret_cast<const float4*>(p));
+  v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
 }
 
 struct Angles {
-  float ca[8], cb[8], sa[8], sb[8];
+  float ca[4], cb[4], sa[4], sb[4];
 };
 
 // cos and sin of row (b, s) for this lane's columns.
@@ -102,22 +94,22 @@ __device__ __forceinline__ void load_angles(const RopeArgs& a, int b, int s, int
   }
   if (p < 0 || p >= a.table_rows) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t.ca[i] = t.cb[i] = t.sa[i] = t.sb[i] = nan_f32();
+    for (int i = 0; i < 4; ++i) t.ca[i] = t.cb[i] = t.sa[i] = t.sb[i] = nan_f32();
     return;
   }
-  const int64_t o = p * D + lane * 8;
-  load8f(a.cos + o, t.ca);
-  load8f(a.cos + o + D / 2, t.cb);
-  load8f(a.sin + o, t.sa);
-  load8f(a.sin + o + D / 2, t.sb);
+  const int64_t o = p * D + lane * 4;
+  load4f(a.cos + o, t.ca);
+  load4f(a.cos + o + D / 2, t.cb);
+  load4f(a.sin + o, t.sa);
+  load4f(a.sin + o + D / 2, t.sb);
 }
 
 template <typename T, int D>
-__device__ __forceinline__ void load_weight(const void* w, int f32, int lane, float (&a)[8],
-                                            float (&b)[8]) {
+__device__ __forceinline__ void load_weight(const void* w, int f32, int lane, float (&a)[4],
+                                            float (&b)[4]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int c = lane * 8 + i;
+  for (int i = 0; i < 4; ++i) {
+    const int c = lane * 4 + i;
     a[i] = f32 ? __ldg(reinterpret_cast<const float*>(w) + c)
                : to_f32<T>(reinterpret_cast<const T*>(w)[c]);
     b[i] = f32 ? __ldg(reinterpret_cast<const float*>(w) + D / 2 + c)
@@ -125,17 +117,17 @@ __device__ __forceinline__ void load_weight(const void* w, int f32, int lane, fl
   }
 }
 
-// Sum over the D / 16 lanes of a head.
+// Sum over the D / 8 lanes of a head.
 template <int D>
 __device__ __forceinline__ float head_sum(float v) {
 #pragma unroll
-  for (int o = D / 32; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = D / 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
 template <typename T, int D, int kHeads, bool NORM>
 __global__ void __launch_bounds__(kThreads) rope_fwd_kernel(const __grid_constant__ RopeArgs a) {
-  constexpr int L = D / 16, G = kThreads / L;
+  constexpr int L = D / 8, G = kThreads / L;
   __shared__ float wsh[NORM ? 2 * D : 1];
   sm100::griddep_wait();
   sm100::griddep_launch_dependents();
@@ -159,7 +151,7 @@ __global__ void __launch_bounds__(kThreads) rope_fwd_kernel(const __grid_constan
   const int h0 = (int)(item - tok * slots) * kHeads;
   const int b = (int)(tok / a.S), s = (int)(tok - (int64_t)b * a.S);
   const T* row = reinterpret_cast<const T*>(a.qkv.ptr) + (int64_t)b * a.qkv.sB + (int64_t)s * a.qkv.sN;
-  Row16<T> x[kHeads];
+  Row8<T> x[kHeads];
 #pragma unroll
   for (int j = 0; j < kHeads; ++j)
     x[j] = load_row<T>(row + (int64_t)min(h0 + j, heads - 1) * a.qkv.sH, lane, D);
@@ -168,20 +160,20 @@ __global__ void __launch_bounds__(kThreads) rope_fwd_kernel(const __grid_constan
 #pragma unroll
   for (int j = 0; j < kHeads; ++j) {
     const int h = h0 + j;
-    float u[8], v[8];
+    float u[4], v[4];
     unpack<T>(x[j], u, v);
     if constexpr (NORM) {
       float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(u[i], u[i], fmaf(v[i], v[i], ss));
+      for (int i = 0; i < 4; ++i) ss = fmaf(u[i], u[i], fmaf(v[i], v[i], ss));
       const float r = rsqrtf(head_sum<D>(ss) * (1.f / D) + a.eps);
-      const float* w = wsh + (h < a.Hq ? 0 : D) + lane * 8;
+      const float* w = wsh + (h < a.Hq ? 0 : D) + lane * 4;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) u[i] = u[i] * r * w[i], v[i] = v[i] * r * w[D / 2 + i];
+      for (int i = 0; i < 4; ++i) u[i] = u[i] * r * w[i], v[i] = v[i] * r * w[D / 2 + i];
     }
-    float ya[8], yb[8];
+    float ya[4], yb[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       ya[i] = fmaf(u[i], t.ca[i], -v[i] * t.sa[i]);
       yb[i] = fmaf(v[i], t.cb[i], u[i] * t.sb[i]);
     }
@@ -196,8 +188,8 @@ __global__ void __launch_bounds__(kThreads) rope_fwd_kernel(const __grid_constan
 // Blocks [0, bq) take queries, the next bk keys, the next bv copy the values' gradient.
 template <typename T, int D, int kHeads, bool NORM>
 __global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const __grid_constant__ RopeArgs a) {
-  constexpr int L = D / 16, G = kThreads / L;
-  __shared__ float red[NORM ? kThreads * 16 : 1];
+  constexpr int L = D / 8, G = kThreads / L;
+  __shared__ float red[NORM ? kThreads * 8 : 1];
   sm100::griddep_wait();
   sm100::griddep_launch_dependents();
   const int lane = threadIdx.x % L, group = threadIdx.x / L;
@@ -211,9 +203,9 @@ __global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const __grid_constan
   const int slots = (H + kHeads - 1) / kHeads;
   const int64_t items = (int64_t)a.B * a.S * slots;
   const int64_t C = (int64_t)(a.Hq + 2 * a.Hkv) * D;
-  float wa[8], wb[8], dwa[8], dwb[8];
+  float wa[4], wb[4], dwa[4], dwb[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) wa[i] = wb[i] = dwa[i] = dwb[i] = 0.f;
+  for (int i = 0; i < 4; ++i) wa[i] = wb[i] = dwa[i] = dwb[i] = 0.f;
   if (NORM && kind < 2) load_weight<T, D>(kind ? a.kw : a.qw, a.w_f32, lane, wa, wb);
   // every lane of the block makes the same number of turns: the shuffles need whole warps
   for (int64_t at = (int64_t)blk * G; at < items; at += (int64_t)nblk * G) {
@@ -227,7 +219,7 @@ __global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const __grid_constan
     const T* xrow = reinterpret_cast<const T*>(a.qkv.ptr) + (int64_t)b * a.qkv.sB +
                     (int64_t)s * a.qkv.sN + (int64_t)base * a.qkv.sH;
     T* orow = reinterpret_cast<T*>(a.dqkv) + tok * C + (int64_t)base * D;
-    Row16<T> gr[kHeads], xr[kHeads];
+    Row8<T> gr[kHeads], xr[kHeads];
 #pragma unroll
     for (int j = 0; j < kHeads; ++j) {
       gr[j] = load_row<T>(grow + (int64_t)min(h0 + j, H - 1) * g.sH, lane, D);
@@ -238,26 +230,26 @@ __global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const __grid_constan
 #pragma unroll
     for (int j = 0; j < kHeads; ++j) {
       const bool on = live && h0 + j < H;
-      float ga[8], gb[8], na[8], nb[8];
+      float ga[4], gb[4], na[4], nb[4];
       unpack<T>(gr[j], ga, gb);
       if (kind == 2) {
         if (on) store_row<T>(orow + (int64_t)(h0 + j) * D, lane, D, ga, gb);
         continue;
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 4; ++i) {
         na[i] = fmaf(ga[i], t.ca[i], gb[i] * t.sb[i]);
         nb[i] = fmaf(gb[i], t.cb[i], -ga[i] * t.sa[i]);
       }
       if constexpr (NORM) {
-        float xa[8], xb[8], ss = 0.f;
+        float xa[4], xb[4], ss = 0.f;
         unpack<T>(xr[j], xa, xb);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(xa[i], xa[i], fmaf(xb[i], xb[i], ss));
+        for (int i = 0; i < 4; ++i) ss = fmaf(xa[i], xa[i], fmaf(xb[i], xb[i], ss));
         const float r = rsqrtf(head_sum<D>(ss) * (1.f / D) + a.eps);
         float c = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
           xa[i] *= r, xb[i] *= r;
           if (on) dwa[i] = fmaf(na[i], xa[i], dwa[i]), dwb[i] = fmaf(nb[i], xb[i], dwb[i]);
           na[i] *= wa[i], nb[i] *= wb[i];
@@ -265,7 +257,7 @@ __global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const __grid_constan
         }
         c = head_sum<D>(c) * (1.f / D);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
           na[i] = r * fmaf(-xa[i], c, na[i]);
           nb[i] = r * fmaf(-xb[i], c, nb[i]);
         }
@@ -276,9 +268,9 @@ __global__ void __launch_bounds__(kThreads) rope_bwd_kernel(const __grid_constan
   if constexpr (NORM) {
     if (kind == 2) return;  // block-uniform
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      red[group * D + lane * 8 + i] = dwa[i];
-      red[group * D + D / 2 + lane * 8 + i] = dwb[i];
+    for (int i = 0; i < 4; ++i) {
+      red[group * D + lane * 4 + i] = dwa[i];
+      red[group * D + D / 2 + lane * 4 + i] = dwb[i];
     }
     __syncthreads();
     if ((int)threadIdx.x < D) {
@@ -299,7 +291,14 @@ __global__ void __launch_bounds__(1024)
   const int first = blockIdx.x ? bq : 0, n = blockIdx.x ? bk : bq;
   const int c = threadIdx.x % D, y = threadIdx.x / D, Y = 1024 / D;
   double s = 0.0;
-  for (int i = y; i < n; i += Y) s += (double)part[(int64_t)(first + i) * D + c];
+  for (int i = y; i < n; i += 8 * Y) {
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      x[k] = i + k * Y < n ? part[(int64_t)(first + i + k * Y) * D + c] : 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += (double)x[k];
+  }
   red[threadIdx.x] = s;
   __syncthreads();
   for (int o = Y / 2; o > 0; o >>= 1) {
@@ -314,7 +313,7 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-constexpr int kPlanBlocks = 148 * 6;  // most backward blocks
+constexpr int kPlanBlocks = 148 * 4;  // most backward blocks
 
 struct RopePlan {
   int bq, bk, bv;
@@ -327,7 +326,7 @@ bool many(const ssa_qk_rope_t* p) { return (int64_t)p->B * p->S * (p->Hq + p->Hk
 RopePlan rope_plan(const ssa_qk_rope_t* p) {
   RopePlan q{};
   const int kh = many(p) ? 4 : 1;
-  const int G = kThreads / (p->D / 16);
+  const int G = kThreads / (p->D / 8);
   auto blocks = [&](int H) {
     return ((int64_t)p->B * p->S * ((H + kh - 1) / kh) + G - 1) / G;
   };
@@ -389,7 +388,7 @@ RopeArgs rope_args(const ssa_qk_rope_t* p) {
 template <typename T, int D, int kHeads, bool NORM>
 int run_fwd(const RopeArgs& a, cudaStream_t st) {
   const int64_t items = (int64_t)a.B * a.S * ((a.Hq + a.Hkv + kHeads - 1) / kHeads);
-  const int G = kThreads / (D / 16);
+  const int G = kThreads / (D / 8);
   const cudaError_t e = sm100::launch_pdl(rope_fwd_kernel<T, D, kHeads, NORM>,
                                           dim3((unsigned)((items + G - 1) / G)), dim3(kThreads), 0, st, a);
   if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "qk_rope_fwd: %s", cudaGetErrorString(e));
