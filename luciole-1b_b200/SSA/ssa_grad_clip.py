@@ -22,11 +22,10 @@ __all__ = ["ssa_grad_norm", "ssa_clip_grad_norm"]
 def _check_list(ts, what, device=None):
     """A list of dense CUDA tensors of one device and one floating dtype."""
     ts = list(ts)
-    for t in ts:
-        if not isinstance(t, torch.Tensor) or t.layout is not torch.strided:
-            raise ValueError(f"{what} must be dense tensors")
+    if not all([isinstance(t, torch.Tensor) and t.layout is torch.strided for t in ts]):
+        raise ValueError(f"{what} must be dense tensors")
     dtypes = {t.dtype for t in ts}
-    devices = {t.device for t in ts}
+    devices = {t.get_device() for t in ts}  # -1: the CPU
     if device is not None and ts:
         devices.add(device)
     if len(dtypes) > 1 or len(devices) > 1:
@@ -95,15 +94,13 @@ def ssa_clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float,
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must be at least 0, got {max_norm}")
     if out is not None:
-        out = _check_list(out, "out", grads[0].device if grads else None)
+        out = _check_list(out, "out", grads[0].get_device() if grads else None)
         if len(out) != len(grads):
             raise ValueError(f"out has {len(out)} tensors for {len(grads)} gradients")
-        for g, o in zip(grads, out):
-            if g.shape != o.shape:
-                raise ValueError(f"out {tuple(o.shape)} does not have its gradient's shape "
-                                 f"{tuple(g.shape)}")
-            if not o.is_contiguous():
-                raise ValueError("out must be contiguous")
+        if [o.shape for o in out] != [g.shape for g in grads]:
+            raise ValueError("out must have the gradients' shapes")
+        if not all([o.is_contiguous() for o in out]):
+            raise ValueError("out must be contiguous")
         if out and out[0].dtype not in (torch.float32, grads[0].dtype):
             raise ValueError(f"out must be fp32 or of the gradients' dtype, got {out[0].dtype}")
     if not grads:

@@ -63,7 +63,7 @@ def _forward(qkv, q_weight, k_weight, cos, sin, positions, hq, hkv, eps):
             rc = _lib.load().ssa_qk_rope_fwd(ctypes.byref(prob), q.data_ptr(), k.data_ptr(),
                                              _lib.stream_ptr(qkv.device))
         _lib.check(rc)
-    return (q, k, heads[..., hq + hkv:, :]), (x, cos, sin, pos, wq, wk), pos_stride
+    return (q, k, heads.narrow(-2, hq + hkv, hkv)), (x, cos, sin, pos, wq, wk), pos_stride
 
 
 class SSAQKNormRopeFunc(Function):
@@ -117,16 +117,15 @@ def ssa_qk_norm_rope(qkv, num_heads, num_kv_heads, cos, sin, q_weight=None, k_we
     sequence has position s), or int32 / int64 of shape [S], [B, S] or [T], an index into the tables;
     one outside them gives NaN (nothing is read out of range). Returns q [..., Hq, D], k [..., Hkv, D]
     and v [..., Hkv, D], the last a view of qkv. Layouts the kernels cannot address are copied."""
-    dev = qkv.device if isinstance(qkv, torch.Tensor) else None
+    if qkv is None or cos is None or sin is None:
+        raise ValueError("qkv, cos and sin are required")
     for t in (qkv, cos, sin, q_weight, k_weight, positions):
         if t is None:
             continue
         if not isinstance(t, torch.Tensor):
             raise ValueError("qkv, cos, sin, the weights and positions must be tensors")
-        if not t.is_cuda or t.device != dev:
+        if not t.is_cuda or t.get_device() != qkv.get_device():
             raise ValueError("all tensors must be CUDA tensors (there is no CPU path) on one device")
-    if qkv is None or cos is None or sin is None:
-        raise ValueError("qkv, cos and sin are required")
     if qkv.dtype not in _lib.DTYPE_CODES:
         raise ValueError(f"unsupported dtype {qkv.dtype}")
     hq, hkv = int(num_heads), int(num_kv_heads)

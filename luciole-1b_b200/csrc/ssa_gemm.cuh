@@ -76,6 +76,7 @@ struct GemmWork {
   int units0, units1;  // of the leading product, of the other
   int lead;
   int extra;
+  int turn;            // the cluster at which the last round robin begins: the one with least to do
   unsigned int* status;
 };
 
@@ -86,22 +87,24 @@ __device__ __forceinline__ int gemm_deal(const GemmWork& w, int c, int workers, 
   which = w.lead;
   if (i < mine) return c + i * workers;
   which = w.lead ^ 1;
-  int j = i - mine, u;
-  const int first = rem ? (workers - rem) * w.extra : 0;
-  if (rem && c >= rem) {
-    if (j < w.extra) u = (c - rem) * w.extra + j;
-    else u = first + c + (j - w.extra) * workers;
-  } else {
-    u = first + c + j * workers;
+  int j = i - mine;
+  const int at = c >= w.turn ? c - w.turn : c - w.turn + workers;
+  int first = 0;
+  if (rem) {
+    first = (workers - rem) * w.extra;
+    if (c >= rem) {
+      if (j < w.extra) return (c - rem) * w.extra + j;
+      j -= w.extra;
+    }
   }
-  return u;
+  return first + at + j * workers;
 }
 
 // How many units cluster c has.
 __device__ __forceinline__ int gemm_count(const GemmWork& w, int c, int workers) {
   const int rem = w.units0 % workers;
   int n = w.units0 / workers + (c < rem ? 1 : 0);
-  int at = c;  // of the other product's round robin
+  int at = c >= w.turn ? c - w.turn : c - w.turn + workers;  // in the other product's round robin
   if (rem) {
     at += (workers - rem) * w.extra;
     if (c >= rem) n += max(0, min(w.extra, w.units1 - (c - rem) * w.extra));
@@ -658,26 +661,27 @@ int launch_gemm(const GemmProduct<Epi>& p0, const GemmProduct<Epi>* p1, cudaStre
     if (rc != SSA_OK) return rc;
   }
   if (!p1) t[2] = t[0], t[3] = t[1];
-  GemmWork w{};
-  w.g[0] = p0.g;
-  w.g[1] = q1.g;
   const int64_t u0 = (int64_t)p0.g.tiles_m * p0.g.tiles_n * p0.g.splits;
   const int64_t u1 = p1 ? (int64_t)q1.g.tiles_m * q1.g.tiles_n * q1.g.splits : 0;
   if (u0 + u1 > INT32_MAX / 2) return abi_error(SSA_ERR_BAD_SHAPE, "too many tiles");
+  const int most = device_sm_count() / CG;
+  const int workers = (int)(u0 + u1 < most ? u0 + u1 : most);
+  GemmWork w{};
+  w.g[0] = p0.g;
+  w.g[1] = q1.g;
   w.lead = p1 && q1.g.kb_split > p0.g.kb_split ? 1 : 0;
   w.units0 = (int)(w.lead ? u1 : u0);
   w.units1 = (int)(w.lead ? u0 : u1);
   if (p1) {
     const int a = w.g[w.lead].kb_split + kTileCost, b = w.g[w.lead ^ 1].kb_split + kTileCost;
     w.extra = (a + b / 2) / b;
+    w.turn = w.extra * b <= a ? w.units0 % workers : 0;
   }
   w.status = device_status_ptr();
   if (!w.status) return abi_error(SSA_ERR_CUDA, "cannot resolve the device status word");
   auto kern = gemm_sm100_kernel<Epi, CG, BN, NH, A_MODE, B_MN, BF16>;
   if (set_smem_limit_once(reinterpret_cast<const void*>(kern), (int)C::SMEM_BYTES) != SSA_OK)
     return abi_error(SSA_ERR_CUDA, "cannot raise the shared memory limit");
-  const int most = device_sm_count() / CG;
-  const int workers = (int)(u0 + u1 < most ? u0 + u1 : most);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(workers * CG));
   cfg.blockDim = dim3(C::THREADS);
