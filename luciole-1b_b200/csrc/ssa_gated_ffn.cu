@@ -104,14 +104,13 @@ struct EpiFfnBwd {
   }
 };
 
-// Few rows: a warp per output column, dot products on the CUDA cores. Bound: memory, every weight read
-// once. A 128-row tile would leave most of the tensor cores' work unused and, with 64 output columns
-// to a tile, a third of the multiprocessors idle. x is read through L1 (ROWS 16-byte loads beside 32
-// bytes of weights).
-template <typename T, int ROWS>
+// One row: a warp per output column, dot products on the CUDA cores. Bound: memory, every weight read
+// once. At hidden 2048, ffn 5632 (46 MB, from L2) 8.8 us against 13.3 us for 128-row tiles, of which
+// there are 88 for 148 multiprocessors; at two rows the conversions already cost more (12.2 us
+// and up).
+template <typename T>
 __global__ void __launch_bounds__(256)
-    ffn_rows_kernel(const T* x, int64_t ldx, const T* w, int64_t ldw, T* h, int64_t ldh, int rows,
-                    int hidden, int ffn) {
+    ffn_row_kernel(const T* x, const T* w, int64_t ldw, T* h, int hidden, int ffn) {
   griddep_wait();
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31;
@@ -119,9 +118,7 @@ __global__ void __launch_bounds__(256)
   if (col >= ffn) return;
   const T* wg = w + (int64_t)col * ldw;
   const T* wu = w + (int64_t)(ffn + col) * ldw;
-  float g[ROWS], u[ROWS];
-#pragma unroll
-  for (int r = 0; r < ROWS; ++r) g[r] = u[r] = 0.f;
+  float g = 0.f, u = 0.f;
   constexpr int U = 4;  // 16-byte loads of each weight row under way per lane
   for (int k0 = lane * 8; k0 < hidden; k0 += U * 256) {
     uint4 a[U], b[U];
@@ -136,32 +133,24 @@ __global__ void __launch_bounds__(256)
     for (int i = 0; i < U; ++i) {
       const int k = k0 + i * 256;
       if (k >= hidden) break;
+      const uint4 c = __ldg(reinterpret_cast<const uint4*>(x + k));
       const T* ta = reinterpret_cast<const T*>(&a[i]);
       const T* tb = reinterpret_cast<const T*>(&b[i]);
+      const T* tx = reinterpret_cast<const T*>(&c);
 #pragma unroll
-      for (int r = 0; r < ROWS; ++r) {
-        if (r >= rows) break;
-        const uint4 c = __ldg(reinterpret_cast<const uint4*>(x + (int64_t)r * ldx + k));
-        const T* tx = reinterpret_cast<const T*>(&c);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float v = to_f32<T>(tx[j]);
-          g[r] = fmaf(to_f32<T>(ta[j]), v, g[r]);
-          u[r] = fmaf(to_f32<T>(tb[j]), v, u[r]);
-        }
+      for (int j = 0; j < 8; ++j) {
+        const float v = to_f32<T>(tx[j]);
+        g = fmaf(to_f32<T>(ta[j]), v, g);
+        u = fmaf(to_f32<T>(tb[j]), v, u);
       }
     }
   }
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    if (r >= rows) break;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      g[r] += __shfl_xor_sync(0xffffffffu, g[r], o);
-      u[r] += __shfl_xor_sync(0xffffffffu, u[r], o);
-    }
-    if (lane == 0) h[(int64_t)r * ldh + col] = from_f32<T>(g[r] * sigmoid_approx(g[r]) * u[r]);
+  for (int o = 16; o > 0; o >>= 1) {
+    g += __shfl_xor_sync(0xffffffffu, g, o);
+    u += __shfl_xor_sync(0xffffffffu, u, o);
   }
+  if (lane == 0) h[col] = from_f32<T>(g * sigmoid_approx(g) * u);
 }
 
 }  // namespace sm100
@@ -170,24 +159,14 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kFewRows = 8;
-
-template <typename T, int ROWS>
-int launch_rows(const ssa_gated_ffn_t* p, void* h, int64_t ldh, cudaStream_t st) {
-  const cudaError_t e =
-      launch_pdl(ffn_rows_kernel<T, ROWS>, dim3((unsigned)cdiv(p->ffn, 8)), dim3(256), 0, st,
-                 static_cast<const T*>(p->x), p->x_stride, static_cast<const T*>(p->w), p->w_stride,
-                 static_cast<T*>(h), ldh, p->rows, p->hidden, p->ffn);
-  if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "ffn_rows: %s", cudaGetErrorString(e));
+template <typename T>
+int ffn_row(const ssa_gated_ffn_t* p, void* h, cudaStream_t st) {
+  const cudaError_t e = launch_pdl(ffn_row_kernel<T>, dim3((unsigned)cdiv(p->ffn, 8)), dim3(256), 0,
+                                   st, static_cast<const T*>(p->x), static_cast<const T*>(p->w),
+                                   p->w_stride, static_cast<T*>(h), p->hidden, p->ffn);
+  if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "ffn_row: %s", cudaGetErrorString(e));
   note_launches(1);
   return SSA_OK;
-}
-
-template <typename T>
-int ffn_rows(const ssa_gated_ffn_t* p, void* h, int64_t ldh, cudaStream_t st) {
-  if (p->rows == 1) return launch_rows<T, 1>(p, h, ldh, st);
-  if (p->rows <= 4) return launch_rows<T, 4>(p, h, ldh, st);
-  return launch_rows<T, kFewRows>(p, h, ldh, st);
 }
 
 struct FfnPlan {
@@ -199,7 +178,7 @@ struct FfnPlan {
 
 FfnPlan ffn_plan(const ssa_gated_ffn_t* p) {
   FfnPlan q{};
-  q.pair = gemm_form((int64_t)cdiv(p->rows, 256) * cdiv(p->ffn, 128));
+  q.pair = gemm_form(p->rows, 2 * (int64_t)p->ffn);
   q.wide = cdiv(p->ffn, q.pair.bn / 2) * (q.pair.bn / 2);
   q.bwd = gradient_form(p->rows, 2 * (int64_t)q.wide, p->hidden, 2 * q.wide / 64,
                         cdiv(p->rows, 64));
@@ -304,9 +283,8 @@ int ssa_gated_ffn_fwd(const ssa_gated_ffn_t* p, void* h, int64_t h_stride, void*
     return abi_error(SSA_ERR_BAD_STRIDE, "gated_ffn: h's row stride is below ffn");
   if ((rc = abi_bind_device(p->x, "x")) != SSA_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (p->rows <= kFewRows)
-    return p->dtype == SSA_DTYPE_BF16 ? ffn_rows<__nv_bfloat16>(p, h, h_stride, st)
-                                      : ffn_rows<__half>(p, h, h_stride, st);
+  if (p->rows == 1)
+    return p->dtype == SSA_DTYPE_BF16 ? ffn_row<__nv_bfloat16>(p, h, st) : ffn_row<__half>(p, h, st);
   const FfnPlan q = ffn_plan(p);
   const FfnFwdArgs a{h, h_stride, p->rows, p->ffn,
                      (uintptr_t)h % 16 == 0 && h_stride % 8 == 0 ? 1 : 0};

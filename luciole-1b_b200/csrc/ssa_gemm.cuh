@@ -47,6 +47,7 @@ struct GemmShape {
   int band;              // row tiles walked before the column advances (operand reuse in L2)
   int b_kjump_at;        // MN-major B: K blocks from here on read rows b_kjump + 64 (kb - at)
   int b_kjump;
+  int a_rows;            // rows of a K-major A's box: 128, or fewer where a lone row tile has fewer
   int b_pair;            // 0, or B is a pair of row blocks this far apart, BN / 2 rows of each
 };
 
@@ -412,7 +413,7 @@ __global__ void __launch_bounds__(320, 1)
             if (rank == 0) mbar_expect_tx(fb, CG * C::STAGE);
             fb = map_rank(fb, 0);
           } else {
-            mbar_expect_tx(fb, C::STAGE);
+            mbar_expect_tx(fb, a_mn ? C::STAGE : C::B_BYTES + (uint32_t)g.a_rows * 128u);
           }
           if (a_mn) {
             tma_load_2d<CG>(sa, ta, fb, m0, k);
@@ -650,11 +651,21 @@ int launch_gemm(const GemmProduct<Epi>& p0, const GemmProduct<Epi>* p1, cudaStre
   constexpr int dtype = BF16 ? SSA_DTYPE_BF16 : SSA_DTYPE_F16;
   CUtensorMap t[4];
   const GemmProduct<Epi>& q1 = p1 ? *p1 : p0;
+  GemmWork w{};
+  w.g[0] = p0.g;
+  w.g[1] = q1.g;
+  // A row of the result depends on its own row of A alone: a lone row tile loads the rows it has
+  // (whole 8-row groups of the swizzle) and leaves the rest of the stage as it is. Boxes that lie
+  // mostly outside the matrix are slow: 9 rows of the loss's head 79 us, 64 rows 59 us before.
+  for (GemmShape& g : w.g) g.a_rows = CG == 1 && g.tiles_m == 1 ? 0 : C::BM;
+  if (!w.g[0].a_rows) w.g[0].a_rows = p0.a.mn < C::BM ? (int)(p0.a.mn + 7) / 8 * 8 : C::BM;
+  if (!w.g[1].a_rows) w.g[1].a_rows = q1.a.mn < C::BM ? (int)(q1.a.mn + 7) / 8 * 8 : C::BM;
   for (int i = 0; i < (p1 ? 2 : 1); ++i) {
     const GemmProduct<Epi>& p = i ? q1 : p0;
     const bool a_mn = A_MODE == 1 || (A_MODE == 2 && i == 1);
     int rc = a_mn ? make_tmap_2d(&t[2 * i], p.a.ptr, dtype, p.a.mn, p.a.k, p.a.ld, 64, p.a.name)
-                  : make_tmap_2d(&t[2 * i], p.a.ptr, dtype, p.a.k, p.a.mn, p.a.ld, C::BM, p.a.name);
+                  : make_tmap_2d(&t[2 * i], p.a.ptr, dtype, p.a.k, p.a.mn, p.a.ld,
+                                 w.g[i].a_rows, p.a.name);
     if (rc != SSA_OK) return rc;
     rc = B_MN ? make_tmap_2d(&t[2 * i + 1], p.b.ptr, dtype, p.b.mn, p.b.k, p.b.ld, 64, p.b.name)
               : make_tmap_2d(&t[2 * i + 1], p.b.ptr, dtype, p.b.k, p.b.mn, p.b.ld, BN / 2, p.b.name);
@@ -666,9 +677,6 @@ int launch_gemm(const GemmProduct<Epi>& p0, const GemmProduct<Epi>* p1, cudaStre
   if (u0 + u1 > INT32_MAX / 2) return abi_error(SSA_ERR_BAD_SHAPE, "too many tiles");
   const int most = device_sm_count() / CG;
   const int workers = (int)(u0 + u1 < most ? u0 + u1 : most);
-  GemmWork w{};
-  w.g[0] = p0.g;
-  w.g[1] = q1.g;
   w.lead = p1 && q1.g.kb_split > p0.g.kb_split ? 1 : 0;
   w.units0 = (int)(w.lead ? u1 : u0);
   w.units1 = (int)(w.lead ? u0 : u1);
@@ -704,26 +712,38 @@ int launch_gemm(const GemmProduct<Epi>& p0, const GemmProduct<Epi>* p1, cudaStre
 inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 inline size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// Tile form of the products with a fused epilogue: the pair's 256 x 256 tiles once they fill the
-// clusters, else 128 x 128 tiles.
+// Tile form. A K block costs about 512 cycles in both: a 256 x 256 pair is bound by the MMAs, a 128 x
+// 128 tile by its 32 KB from L2. So the pairs are taken where they need fewer rounds than single CTAs
+// do, and where more than half of their rows are used. Feed-forward at 256 rows of 2048, ffn 5632:
+// 176 single tiles (two rounds) 22 us, 44 pairs 17 us; at 300 rows of 512, ffn 1024: 48 single tiles
+// 8 us, 16 pairs 10.5 us.
 struct GemmForm {
   bool pair;
   int bm, bn, workers;
   bool wide;  // gradients: 256 x 512 tiles
 };
-inline GemmForm gemm_form(int64_t tiles_256) {
-  const bool pair = tiles_256 >= kPlanSms / 2;
+inline GemmForm make_form(bool pair) {
   return pair ? GemmForm{true, 256, 256, kPlanSms / 2, false}
               : GemmForm{false, 128, 128, kPlanSms, false};
 }
 
-// Tile form of dx [rows, hidden] (kx K blocks) and dW [cols, hidden] (kw K blocks): 256 x 512 tiles,
-// which read a quarter less per operation, when they fill the clusters and their K loop is long
-// against an epilogue that no longer runs under the next tile's MMAs.
+// Of a product [rows, cols] with a fused epilogue.
+inline GemmForm gemm_form(int64_t rows, int64_t cols) {
+  const int pairs = cdiv((int64_t)cdiv(rows, 256) * cdiv(cols, 256), kPlanSms / 2);
+  const int singles = cdiv((int64_t)cdiv(rows, 128) * cdiv(cols, 128), kPlanSms);
+  return make_form(rows > 128 && pairs < singles);
+}
+
+// Of dx [rows, hidden] (kx K blocks) and dW [cols, hidden] (kw K blocks): pairs once one of the two
+// fills the clusters (few rows included: dW is then bound by its stores; at 64 rows of 2048,
+// vocabulary 32,768 loss and gradients take 153 us with pairs, 176 us without; with fewer tiles, 300
+// rows of 512, ffn 1024, 26 us without and 35 us with pairs); 256 x 512 tiles, which read a quarter
+// less per operation, when these fill the clusters and the K loops are long against an epilogue that
+// no longer runs under the next tile's MMAs.
 inline GemmForm gradient_form(int64_t rows, int64_t cols, int hidden, int kx, int kw) {
   const int64_t dx = (int64_t)cdiv(rows, 256) * cdiv(hidden, 256);
   const int64_t dw = (int64_t)cdiv(cols, 256) * cdiv(hidden, 256);
-  GemmForm f = gemm_form(dx > dw ? dx : dw);
+  GemmForm f = make_form((dx > dw ? dx : dw) >= kPlanSms / 2);
   f.wide = f.pair && hidden > 256 && dx + dw >= 2 * f.workers && kx >= 64 && kw >= 64;
   if (f.wide) f.bn = 512;
   return f;

@@ -124,6 +124,70 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
+// One row: the forward's logits on the CUDA cores, two vocabulary rows per warp at a time, each warp
+// keeping a running pair. Bound: memory, W read once. A 128-row tile would spend as long on its
+// unused rows: at hidden 2048, vocabulary 65,536 (268 MB) 50.5 us here, 59 us there; at two rows
+// this form's conversions already cost more (69 us).
+constexpr int kRowBlocks = 148 * 4;
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+    ce_row_kernel(const T* x, const T* w, int64_t ldw, int hidden, const CeFwdArgs a) {
+  __shared__ float2 sh[8];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t t = __ldg(a.targets);
+  float m = kLowest, s = 0.f;
+  for (int v0 = 2 * (blockIdx.x * 8 + warp); v0 < a.vocab; v0 += 2 * 8 * (int)gridDim.x) {
+    const int v1 = min(v0 + 1, a.vocab - 1);
+    const T* w0 = w + (int64_t)v0 * ldw;
+    const T* w1 = w + (int64_t)v1 * ldw;
+    float p = 0.f, q = 0.f;
+    constexpr int U = 4;  // 16-byte loads of each vocabulary row under way per lane
+    for (int k0 = lane * 8; k0 < hidden; k0 += U * 256) {
+      uint4 u0[U], u1[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int k = k0 + i * 256;
+        const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+        u0[i] = k < hidden ? __ldg(reinterpret_cast<const uint4*>(w0 + k)) : z;
+        u1[i] = k < hidden ? __ldg(reinterpret_cast<const uint4*>(w1 + k)) : z;
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int k = k0 + i * 256;
+        if (k >= hidden) break;
+        const uint4 c = __ldg(reinterpret_cast<const uint4*>(x + k));
+        const T* t0 = reinterpret_cast<const T*>(&u0[i]);
+        const T* t1 = reinterpret_cast<const T*>(&u1[i]);
+        const T* tx = reinterpret_cast<const T*>(&c);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float y = to_f32<T>(tx[j]);
+          p = fmaf(to_f32<T>(t0[j]), y, p);
+          q = fmaf(to_f32<T>(t1[j]), y, q);
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      p += __shfl_xor_sync(0xffffffffu, p, o);
+      q += __shfl_xor_sync(0xffffffffu, q, o);
+    }
+    if (lane == 0 && t == v0) *a.target_logit = p;
+    if (lane == 0 && t == v1) *a.target_logit = q;
+    join_pair(m, s, make_float2(p, 1.f));
+    if (v1 != v0) join_pair(m, s, make_float2(q, 1.f));
+  }
+  if (lane == 0) sh[warp] = make_float2(m, s);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 8; ++i) join_pair(m, s, sh[i]);
+    a.part[blockIdx.x] = make_float2(m, s);
+  }
+}
+
 // Sum over a block of 1024 threads in a fixed order; the result in thread 0.
 __device__ __forceinline__ double block_sum_1024(double v, double* red) {
 #pragma unroll
@@ -263,7 +327,7 @@ constexpr int64_t kPieceBytes = (int64_t)256 << 20;
 
 struct CePlan {
   GemmForm fwd, bwd;           // tiles of the logits, and of dx and dw
-  int fwd_tiles;               // column tiles of the forward
+  int fwd_tiles;               // column tiles of the forward (one row: blocks)
   int64_t ldd;                 // columns of a piece (a multiple of 256)
   int pieces;
   int dx_splits;
@@ -274,8 +338,10 @@ struct CePlan {
 CePlan ce_plan(const ssa_linear_ce_t* p) {
   CePlan q{};
   const int64_t rows = p->rows;
-  q.fwd = gemm_form((int64_t)cdiv(rows, 256) * cdiv(p->vocab, 256));
-  q.fwd_tiles = cdiv(p->vocab, q.fwd.bn);
+  q.fwd = gemm_form(rows, p->vocab);
+  q.fwd_tiles = rows > 1                            ? cdiv(p->vocab, q.fwd.bn)
+                : cdiv(p->vocab, 16) < kRowBlocks ? cdiv(p->vocab, 16)
+                                                  : kRowBlocks;
   q.off_target = up256(sizeof(float2) * (size_t)q.fwd_tiles * rows);
   q.off_rows = q.off_target + up256(sizeof(float) * rows);
   q.fwd_bytes = q.off_rows + up256(sizeof(float) * rows);
@@ -337,12 +403,25 @@ int ce_logits(const ssa_linear_ce_t* p, const GemmForm& f, const void* w, int64_
 }
 
 template <bool BF16>
+int ce_row(const ssa_linear_ce_t* p, int blocks, const CeFwdArgs& a, cudaStream_t st) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  const cudaError_t e = launch_pdl(ce_row_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st,
+                                   static_cast<const T*>(p->x), static_cast<const T*>(p->w),
+                                   p->w_stride, p->hidden, a);
+  if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "ce_row: %s", cudaGetErrorString(e));
+  note_launches(1);
+  return SSA_OK;
+}
+
+template <bool BF16>
 int ce_fwd(const ssa_linear_ce_t* p, const CePlan& q, float* loss, float* lse, float* count,
            uint8_t* ws, cudaStream_t st) {
   CeFwdArgs a{p->targets, reinterpret_cast<float2*>(ws),
               reinterpret_cast<float*>(ws + q.off_target), p->rows, p->vocab};
-  const int rc = ce_logits<EpiCeFwd<256>, EpiCeFwd<128>, BF16>(p, q.fwd, p->w, p->vocab, q.fwd_tiles,
-                                                               a, st);
+  const int rc = p->rows == 1
+                     ? ce_row<BF16>(p, q.fwd_tiles, a, st)
+                     : ce_logits<EpiCeFwd<256>, EpiCeFwd<128>, BF16>(p, q.fwd, p->w, p->vocab,
+                                                                     q.fwd_tiles, a, st);
   if (rc != SSA_OK) return rc;
   float* rows_loss = p->reduction ? reinterpret_cast<float*>(ws + q.off_rows) : loss;
   cudaError_t e = launch_pdl(ce_join_kernel, dim3((unsigned)cdiv(p->rows, 32)), dim3(1024), 0, st,
@@ -377,7 +456,7 @@ int ce_bwd(const ssa_linear_ce_t* p, const CePlan& q, const float* lse, const fl
     const int64_t wide = (int64_t)cdiv(cols, 256) * 256;                 // written to d
     const uint8_t* w0 = static_cast<const uint8_t*>(p->w) + 2 * v0 * p->w_stride;
     const CeBwdArgs a{p->targets, lse, weight, d, q.ldd, p->rows, (int)v0, p->vocab};
-    const GemmForm form = gemm_form((int64_t)cdiv(p->rows, 256) * (wide / 256));
+    const GemmForm form = gemm_form(p->rows, wide);
     int rc = ce_logits<EpiCeBwd<256, BF16>, EpiCeBwd<128, BF16>, BF16>(
         p, form, w0, cols, (int)(wide / form.bn), a, st);
     if (rc != SSA_OK) return rc;
