@@ -13,6 +13,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd.function import once_differentiable
 
 _PKG_ROOT = Path(__file__).resolve().parent.parent
 LIB_PATH = Path(os.environ.get("SSA_B200_LIB", str(_PKG_ROOT / "libssa_b200.so")))
@@ -207,6 +208,17 @@ def table(t: torch.Tensor) -> torch.Tensor:
     """A contiguous, 16-byte aligned table: `t` itself, or a copy in fresh storage."""
     ok = t.is_contiguous() and t.data_ptr() % 16 == 0
     return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def first_order(backward):
+    """A Function's backward that runs kernels autograd cannot see through: differentiating it again
+    raises (torch's once_differentiable, whose wrapper is entered only where a graph of the
+    backward is being built)."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 def workspace(size: int, device: torch.device) -> torch.Tensor:

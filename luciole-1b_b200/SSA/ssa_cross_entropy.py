@@ -12,7 +12,6 @@ import ctypes
 
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -63,7 +62,7 @@ class SSALinearCrossEntropyFunc(Function):
         return loss
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, grad_loss):
         x, w, t, stats = ctx.saved_tensors
         ignore_index, code, shape = ctx.args

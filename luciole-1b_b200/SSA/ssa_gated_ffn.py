@@ -11,7 +11,6 @@ import ctypes
 
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -50,7 +49,7 @@ class SSAGatedFFNFunc(Function):
         return h
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, grad):
         x, w = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad

@@ -8,7 +8,6 @@ import ctypes
 
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -78,7 +77,7 @@ class SSAQKNormRopeFunc(Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, dq, dk, dv):
         x, cos, sin, pos, wq, wk = ctx.saved_tensors
         hq, hkv, eps, pos_stride, shape = ctx.args

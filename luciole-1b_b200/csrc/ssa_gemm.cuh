@@ -767,12 +767,14 @@ inline GemmShape plain_shape(int tiles_m, int tiles_n, int kblocks, int64_t a_by
 
 // Splits of the contraction of `tiles` tiles of `kblocks` K blocks beside `other` K blocks of the
 // launch's other product, so that no unit is longer than a worker's share of everything; of at least
-// four blocks each. The same whether the other product is asked for or not: so are the bits.
+// four blocks each, and only where that shortens the longest unit by 32 blocks (9 us): the splits'
+// sums take another launch. The same whether the other product is asked for or not: so are the bits.
 inline int split_count(int64_t tiles, int kblocks, int64_t other, int workers) {
   const int64_t share = (tiles * kblocks + other) / workers;
   int64_t s = share > 0 ? (kblocks + share - 1) / share : kblocks;
   if (s > kblocks / 4) s = kblocks / 4;
-  return s > 1 ? cdiv(kblocks, cdiv(kblocks, s)) : 1;
+  if (s <= 1 || kblocks - kblocks / s < 32) return 1;
+  return cdiv(kblocks, cdiv(kblocks, s));
 }
 
 // ------------------------------------------------------------------------- plain store epilogue

@@ -168,3 +168,12 @@ def test_refusals(cuda_device):
                         ((x, w[:, :32]), r"\[2 F, H\]"), ((x.cpu(), w), "CUDA")):
         with pytest.raises(ValueError, match=match):
             f(*args)
+
+
+def test_second_derivative_is_refused(cuda_device):
+    from SSA.ssa_gated_ffn import ssa_gated_ffn
+    x, w, _ = _data(4, 64, 10, torch.bfloat16, 23, cuda_device)
+    x.requires_grad_(True)
+    (g,) = torch.autograd.grad(ssa_gated_ffn(x, w).float().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.float().sum().backward()
