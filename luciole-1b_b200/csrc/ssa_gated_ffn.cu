@@ -29,16 +29,27 @@ struct FfnFwdArgs {
 template <int BN, bool BF16>
 struct EpiFfnFwd {
   using Args = FfnFwdArgs;
-  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, const EpiCtx& e) {
+  struct Row {};
+  __device__ static __forceinline__ Row row(const Args&, int) { return Row{}; }
+  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, const Row&,
+                                              const EpiCtx& e) {
     const int off = e.half * (BN / 4);  // a warp's gate columns; the up projection's are BN / 2 on
     uint16_t* base = reinterpret_cast<uint16_t*>(a.h) + (int64_t)e.row0 * a.ldh;
+    uint32_t xg[32], xu[32];
+    e.fetch(off, xg);
+    e.fetch(BN / 2 + off, xu);
 #pragma unroll 1
     for (int c = 0; c < BN / 4; c += 32) {
       const int col = w.nt * (BN / 2) + off + c;
-      if (col >= a.ffn) break;
       float g[32], u[32];
-      e.read(off + c, g);
-      e.read(BN / 2 + off + c, u);
+      e.settle();
+      e.values(xg, g);
+      e.values(xu, u);
+      if (c + 32 < BN / 4) {
+        e.fetch(off + c + 32, xg);
+        e.fetch(BN / 2 + off + c + 32, xu);
+      }
+      if (col >= a.ffn) break;
 #pragma unroll
       for (int i = 0; i < 32; ++i) g[i] = g[i] * sigmoid_approx(g[i]) * u[i];
       store_block16<BF16>(e, g, base, a.ldh, a.rows - e.row0, col, a.ffn, a.vec);
@@ -58,12 +69,18 @@ template <int BN, bool BF16>
 struct EpiFfnBwd {
   using Args = FfnBwdArgs;
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, const EpiCtx& e) {
+  struct Row {};
+  __device__ static __forceinline__ Row row(const Args&, int) { return Row{}; }
+  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, const Row&,
+                                              const EpiCtx& e) {
     const int off = e.half * (BN / 4);
     const int rows = a.rows - e.row0;
     const uint16_t* dhbase = reinterpret_cast<const uint16_t*>(a.dh) + (int64_t)e.row0 * a.lddh;
     uint16_t* base = reinterpret_cast<uint16_t*>(a.d) + (int64_t)e.row0 * (2 * a.wide);
     uint8_t* in = e.exch + 2048;  // dh's block; the first half of the buffer carries d's
+    uint32_t xg[32], xu[32];
+    e.fetch(off, xg);
+    e.fetch(BN / 2 + off, xu);
 #pragma unroll 1
     for (int c = 0; c < BN / 4; c += 32) {
       const int col = w.nt * (BN / 2) + off + c;
@@ -77,14 +94,20 @@ struct EpiFfnBwd {
                                        : make_uint4(0u, 0u, 0u, 0u);
         }
       } else {
+#pragma unroll 8
         for (int r = 0; r < 32; ++r)
           reinterpret_cast<uint16_t*>(exch16(in, r, e.lane >> 3))[e.lane & 7] =
               r < rows && col + e.lane < a.ffn ? dhbase[(int64_t)r * a.lddh + col + e.lane] : 0;
       }
       __syncwarp();
       float g[32], u[32];
-      e.read(off + c, g);
-      e.read(BN / 2 + off + c, u);
+      e.settle();
+      e.values(xg, g);
+      e.values(xu, u);
+      if (c + 32 < BN / 4) {
+        e.fetch(off + c + 32, xg);
+        e.fetch(BN / 2 + off + c + 32, xu);
+      }
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
         const uint4 x = *exch16(in, e.lane, p);

@@ -26,7 +26,10 @@ namespace {
 template <int BN, bool BF16>
 struct EpiStore {
   using Args = StoreArgs;
-  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, const EpiCtx& e) {
+  struct Row {};
+  __device__ static __forceinline__ Row row(const Args&, int) { return Row{}; }
+  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, const Row&,
+                                              const EpiCtx& e) {
     const float sc = a.scale ? __ldg(a.scale) : 1.f;
     const int col0 = w.nt * BN + e.half * (BN / 2);
     const int n = min(BN / 2, ((a.cols - col0 + 31) >> 5) << 5);  // columns of this warp, whole 32s
@@ -37,12 +40,13 @@ struct EpiStore {
     for (int c = 0; c < n; c += 32) {
       const int col = col0 + c;
       float v[32];
-      e.settle(x, v);
+      e.settle();
+      e.values(x, v);
       if (c + 32 < n) e.fetch(e.half * (BN / 2) + c + 32, x);
       if (a.out) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] *= sc;
-        put_row16<BF16>(e, v);
+        put_row16<BF16>(e, v, 0xffffffffu);
         __syncwarp();
         const int p = e.lane & 3, my = col + 8 * p;
 #pragma unroll

@@ -38,6 +38,22 @@
 namespace ssa {
 namespace sm100 {
 
+// Division of 0 <= n < 2^31 by a fixed d >= 1 as a multiplication (Granlund and Montgomery, "Division
+// by invariant integers using multiplication", 1994): with 2^s >= d, n / d = (hi(n m) + n) >> s for
+// m = floor(2^32 (2^s - d) / d) + 1.
+struct FastDiv {
+  uint32_t d, m, s;
+};
+inline FastDiv fast_div(int d) {
+  FastDiv f{(uint32_t)d, 0, 0};
+  while ((1ull << f.s) < f.d) ++f.s;
+  f.m = (uint32_t)(((1ull << 32) * ((1ull << f.s) - f.d)) / f.d + 1);
+  return f;
+}
+__device__ __forceinline__ int div_by(int n, const FastDiv& f) {
+  return (int)((__umulhi((uint32_t)n, f.m) + (uint32_t)n) >> f.s);
+}
+
 // One product of a launch (plain data, passed by value).
 struct GemmShape {
   int tiles_m, tiles_n;  // tiles of 128 CG rows and BN columns
@@ -49,6 +65,15 @@ struct GemmShape {
   int b_kjump;
   int a_rows;            // rows of a K-major A's box: 128, or fewer where a lone row tile has fewer
   int b_pair;            // 0, or B is a pair of row blocks this far apart, BN / 2 rows of each
+  FastDiv by_splits, by_band, by_rows, by_last;  // splits, tiles of a band, rows of a band, of the last
+
+  void set_divisors() {
+    const int last = tiles_m % band;
+    by_splits = fast_div(splits);
+    by_band = fast_div(band * tiles_n);
+    by_rows = fast_div(band);
+    by_last = fast_div(last ? last : band);
+  }
 };
 
 struct GemmUnit {
@@ -57,12 +82,12 @@ struct GemmUnit {
 
 __device__ __forceinline__ GemmUnit gemm_unit(const GemmShape& g, int u) {
   GemmUnit w;
-  const int t = u / g.splits;
+  const int t = div_by(u, g.by_splits);
   w.sp = u - t * g.splits;
-  const int per_band = g.band * g.tiles_n;
-  const int bd = t / per_band, r = t - bd * per_band;
-  const int rows = min(g.band, g.tiles_m - bd * g.band);
-  w.nt = r / rows;
+  const int bd = div_by(t, g.by_band), r = t - bd * (g.band * g.tiles_n);
+  const bool last = (bd + 1) * g.band > g.tiles_m;
+  const int rows = last ? (int)g.by_last.d : g.band;
+  w.nt = div_by(r, last ? g.by_last : g.by_rows);
   w.mt = bd * g.band + (r - w.nt * rows);
   w.k0 = w.sp * g.kb_split;
   w.k1 = min(g.kblocks, w.k0 + g.kb_split);
@@ -75,6 +100,7 @@ __device__ __forceinline__ GemmUnit gemm_unit(const GemmShape& g, int u) {
 struct GemmWork {
   GemmShape g[2];
   int units0, units1;  // of the leading product, of the other
+  int rem, whole;      // units0 over the clusters: part-filled last round, whole rounds
   int lead;
   int extra;
   int turn;            // the cluster at which the last round robin begins: the one with least to do
@@ -83,8 +109,7 @@ struct GemmWork {
 
 // The i-th unit of cluster c (below gemm_count): its product in `which`, its index returned.
 __device__ __forceinline__ int gemm_deal(const GemmWork& w, int c, int workers, int i, int& which) {
-  const int rem = w.units0 % workers;
-  const int mine = w.units0 / workers + (c < rem ? 1 : 0);
+  const int rem = w.rem, mine = w.whole + (c < rem ? 1 : 0);
   which = w.lead;
   if (i < mine) return c + i * workers;
   which = w.lead ^ 1;
@@ -103,8 +128,8 @@ __device__ __forceinline__ int gemm_deal(const GemmWork& w, int c, int workers, 
 
 // How many units cluster c has.
 __device__ __forceinline__ int gemm_count(const GemmWork& w, int c, int workers) {
-  const int rem = w.units0 % workers;
-  int n = w.units0 / workers + (c < rem ? 1 : 0);
+  const int rem = w.rem;
+  int n = w.whole + (c < rem ? 1 : 0);
   int at = c >= w.turn ? c - w.turn : c - w.turn + workers;  // in the other product's round robin
   if (rem) {
     at += (workers - rem) * w.extra;
@@ -146,8 +171,10 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// What the arrival guards is TMEM, which the tcgen05 fence before it orders: a release at cluster scope
+// would also wait for the warp's global stores (a quarter of the stalls of an epilogue warp).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // The pair forms of the TMEM and MMA instructions (both CTAs of the cluster take part).
@@ -225,30 +252,25 @@ struct EpiCtx {
   uint32_t taddr;   // TMEM address of the accumulator's column 0 in this warp's lanes
   bool failed;
   uint8_t* exch;    // this warp's 4 KB of shared memory
-  uint8_t* exch0;   // the 4 KB of epilogue warp 0
   int lane, quad, half, turn;
   int row0;         // global row of lane 0
 
-  // The same in two steps, with other work between them.
+  // Accumulator columns [col, col + 32) of this lane's row, in two steps with other work between them
+  // (every lane of the warp calls both): start the read, then wait for all reads started.
   __device__ __forceinline__ void fetch(int col, uint32_t (&r)[32]) const {
-    if (!failed) tmem_ld32(taddr + (uint32_t)col, r);
-  }
-  __device__ __forceinline__ void settle(uint32_t (&r)[32], float (&v)[32]) const {
-    if (!failed) tmem_ld_wait(r);
+    if (!failed) {
+      tmem_ld32(taddr + (uint32_t)col, r);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = failed ? nan_f32() : __uint_as_float(r[i]);
-  }
-
-  // Accumulator columns [col, col + 32) of this lane's row (every lane of the warp calls it).
-  __device__ __forceinline__ void read(int col, float (&v)[32]) const {
-    if (failed) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = nan_f32();
-      return;
+      for (int i = 0; i < 32; ++i) r[i] = 0x7FC00000u;
     }
-    uint32_t r[32];
-    tmem_ld32(taddr + (uint32_t)col, r);
-    tmem_ld_wait(r);
+  }
+  __device__ __forceinline__ void settle() const {
+    if (!failed) tmem_ld_wait_only();
+  }
+  // The values of a read that settle() has waited for.
+  __device__ __forceinline__ static void values(uint32_t (&r)[32], float (&v)[32]) {
+    tmem_pin(r);
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
   }
@@ -266,21 +288,22 @@ __device__ __forceinline__ float4* exch32(uint8_t* buf, int row, int piece) {
 }
 
 template <bool BF16>
-__device__ __forceinline__ void put_row16(const EpiCtx& e, const float (&v)[32]) {
+__device__ __forceinline__ void put_row16(const EpiCtx& e, const float (&v)[32], uint32_t mask) {
 #pragma unroll
   for (int p = 0; p < 4; ++p)
-    *exch16(e.exch, e.lane, p) =
-        make_uint4(pack2<BF16>(v[8 * p], v[8 * p + 1]), pack2<BF16>(v[8 * p + 2], v[8 * p + 3]),
-                   pack2<BF16>(v[8 * p + 4], v[8 * p + 5]), pack2<BF16>(v[8 * p + 6], v[8 * p + 7]));
+    *exch16(e.exch, e.lane, p) = make_uint4(
+        pack2<BF16>(v[8 * p], v[8 * p + 1]) & mask, pack2<BF16>(v[8 * p + 2], v[8 * p + 3]) & mask,
+        pack2<BF16>(v[8 * p + 4], v[8 * p + 5]) & mask, pack2<BF16>(v[8 * p + 6], v[8 * p + 7]) & mask);
 }
 
 // Stores the warp's block of 16-bit values (one row of 32 per lane) to rows base + r * ld of
 // columns [col, col + 32), rows and columns below the limits only. base: row 0, column 0.
-// vec: base and ld are multiples of 16 bytes.
+// vec: base and ld are multiples of 16 bytes. mask: 0 makes this lane's row zeros, whatever its values.
 template <bool BF16>
 __device__ __forceinline__ void store_block16(const EpiCtx& e, const float (&v)[32], uint16_t* base,
-                                              int64_t ld, int rows, int col, int cols, bool vec) {
-  put_row16<BF16>(e, v);
+                                              int64_t ld, int rows, int col, int cols, bool vec,
+                                              uint32_t mask = 0xffffffffu) {
+  put_row16<BF16>(e, v, mask);
   __syncwarp();
   if (vec && col + 32 <= cols) {
     const int p = e.lane & 3;
@@ -292,6 +315,7 @@ __device__ __forceinline__ void store_block16(const EpiCtx& e, const float (&v)[
     }
   } else if (col + e.lane < cols) {
     const int n = min(rows, 32);
+#pragma unroll 8
     for (int r = 0; r < n; ++r)
       base[(int64_t)r * ld + col + e.lane] =
           reinterpret_cast<const uint16_t*>(exch16(e.exch, r, e.lane >> 3))[e.lane & 7];
@@ -299,8 +323,10 @@ __device__ __forceinline__ void store_block16(const EpiCtx& e, const float (&v)[
   __syncwarp();
 }
 
-// Epi: struct with `Args` and `static void tile(const Args&, const GemmUnit&, const EpiCtx&)`, run
-// by every epilogue warp for each unit. A_MODE: 0 A is K-major, 1 MN-major, 2 K-major in product 0
+// Epi: struct with `Args`, `Row`, `static Row row(const Args&, int row)`, which reads what a lane needs
+// to know of its row, and `static void tile(const Args&, const GemmUnit&, const Row&, const EpiCtx&)`,
+// run by every epilogue warp for each unit; the next unit's rows are read before this one's
+// tile. A_MODE: 0 A is K-major, 1 MN-major, 2 K-major in product 0
 // and MN-major in product 1.
 template <class Epi, int CG, int BN, int NH, int A_MODE, bool B_MN, bool BF16>
 __global__ void __launch_bounds__(320, 1)
@@ -547,13 +573,24 @@ __global__ void __launch_bounds__(320, 1)
     e.lane = lane;
     e.quad = warp & 3;  // the 32 TMEM lanes this warp can read
     e.half = (warp - 2) >> 2;
-    e.exch0 = smem + C::OFF_EXCH;
-    e.exch = e.exch0 + (warp - 2) * 4096;
-    for (int i = 0; i < count; ++i) {
+    e.exch = smem + C::OFF_EXCH + (warp - 2) * 4096;
+    const int row_in = (int)rank * C::BM + e.quad * 32;
+    GemmUnit next;
+    bool next_second = false;
+    typename Epi::Row next_row{};
+    auto look = [&](int i) {
       int which;
       const int u = gemm_deal(work, worker, workers, i, which);
-      const bool second = A_MODE == 2 && which == 1;
-      const GemmUnit w = gemm_unit(work.g[second ? 1 : 0], u);
+      next_second = A_MODE == 2 && which == 1;
+      next = gemm_unit(work.g[next_second ? 1 : 0], u);
+      next_row = Epi::row(next_second ? ea1 : ea0, next.mt * CG * C::BM + row_in + lane);
+    };
+    look(0);
+    for (int i = 0; i < count; ++i) {
+      const GemmUnit w = next;
+      const bool second = next_second;
+      const typename Epi::Row row = next_row;
+      if (i + 1 < count) look(i + 1);
       if (!e.failed) {
         const bool ok = NH == 1 ? mbar_wait(tfull(i & 1), (i >> 1) & 1, work.status)
                                 : mbar_wait(tfull(0), i & 1, work.status);
@@ -564,14 +601,14 @@ __global__ void __launch_bounds__(320, 1)
         tc_fence_after();
       }
       e.turn = i;
-      e.row0 = (w.mt * CG + (int)rank) * C::BM + e.quad * 32;
+      e.row0 = w.mt * CG * C::BM + row_in;
 #pragma unroll 1
       for (int h = 0; h < NH; ++h) {
         const int buf = NH == 1 ? i & 1 : h;
         e.taddr = tmem + ((uint32_t)(e.quad * 32) << 16) + (uint32_t)(buf * BN);
         GemmUnit wh = w;
         wh.nt = w.nt * NH + h;
-        Epi::tile(second ? ea1 : ea0, wh, e);
+        Epi::tile(second ? ea1 : ea0, wh, row, e);
         tc_fence_before();
         __syncwarp();
         if (!e.failed && lane == 0) {
@@ -657,6 +694,7 @@ int launch_gemm(const GemmProduct<Epi>& p0, const GemmProduct<Epi>* p1, cudaStre
   // A row of the result depends on its own row of A alone: a lone row tile loads the rows it has
   // (whole 8-row groups of the swizzle) and leaves the rest of the stage as it is. Boxes that lie
   // mostly outside the matrix are slow: 9 rows of the loss's head 79 us, 64 rows 59 us before.
+  for (GemmShape& g : w.g) g.set_divisors();
   for (GemmShape& g : w.g) g.a_rows = CG == 1 && g.tiles_m == 1 ? 0 : C::BM;
   if (!w.g[0].a_rows) w.g[0].a_rows = p0.a.mn < C::BM ? (int)(p0.a.mn + 7) / 8 * 8 : C::BM;
   if (!w.g[1].a_rows) w.g[1].a_rows = q1.a.mn < C::BM ? (int)(q1.a.mn + 7) / 8 * 8 : C::BM;
@@ -680,10 +718,12 @@ int launch_gemm(const GemmProduct<Epi>& p0, const GemmProduct<Epi>* p1, cudaStre
   w.lead = p1 && q1.g.kb_split > p0.g.kb_split ? 1 : 0;
   w.units0 = (int)(w.lead ? u1 : u0);
   w.units1 = (int)(w.lead ? u0 : u1);
+  w.rem = w.units0 % workers;
+  w.whole = w.units0 / workers;
   if (p1) {
     const int a = w.g[w.lead].kb_split + kTileCost, b = w.g[w.lead ^ 1].kb_split + kTileCost;
     w.extra = (a + b / 2) / b;
-    w.turn = w.extra * b <= a ? w.units0 % workers : 0;
+    w.turn = w.extra * b <= a ? w.rem : 0;
   }
   w.status = device_status_ptr();
   if (!w.status) return abi_error(SSA_ERR_CUDA, "cannot resolve the device status word");

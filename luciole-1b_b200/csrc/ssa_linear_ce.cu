@@ -16,7 +16,7 @@
 namespace ssa {
 namespace sm100 {
 
-constexpr float kLowest = -3.0e38f;  // start of a running maximum: finite, so that max - max is 0
+constexpr float kLowest = -1.0e38f;  // start of a running maximum: finite, so that max - max is 0
 
 struct CeFwdArgs {
   const int64_t* targets;
@@ -25,41 +25,69 @@ struct CeFwdArgs {
   int rows, vocab;
 };
 
+// A row's target column, -1 where there is none in the vocabulary.
+__device__ __forceinline__ int ce_target(const int64_t* targets, int row, int rows, int vocab) {
+  const int64_t t = row < rows ? __ldg(targets + row) : -1;
+  return t >= 0 && t < vocab ? (int)t : -1;
+}
+
 template <int BN>
 struct EpiCeFwd {
   using Args = CeFwdArgs;
-  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, const EpiCtx& e) {
+  struct Row {
+    int t;
+  };
+  __device__ static __forceinline__ Row row(const Args& a, int row) {
+    return Row{ce_target(a.targets, row, a.rows, a.vocab)};
+  }
+  // A lane holds its half row, BN / 2 columns, in registers: one maximum, then the exponentials in
+  // eight independent sums.
+  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, const Row& rw,
+                                              const EpiCtx& e) {
+    constexpr int NC = BN / 64;  // 32-column pieces of the half
     const int row = e.row0 + e.lane;
     const int off = e.half * (BN / 2), col0 = w.nt * BN + off;
     const bool ok = row < a.rows;
-    const int64_t t = ok ? __ldg(a.targets + row) : -1;
     float m = kLowest, s = 0.f;
-#pragma unroll 1
-    for (int c = 0; c < BN / 2; c += 32) {
-      if (col0 + c >= a.vocab) break;
-      float v[32];
-      e.read(off + c, v);
-      if (col0 + c + 32 > a.vocab) {
+    if (col0 < a.vocab) {  // warp-uniform
+      uint32_t x[NC][32];
+      float v[NC][32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (col0 + c + i >= a.vocab) v[i] = -INFINITY;
+      for (int c = 0; c < NC; ++c) e.fetch(off + 32 * c, x[c]);
+      e.settle();
+#pragma unroll
+      for (int c = 0; c < NC; ++c) e.values(x[c], v[c]);
+      if (col0 + 32 * NC > a.vocab) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (col0 + 32 * c + i >= a.vocab) v[c][i] = -INFINITY;
       }
-      float m4[4] = {m, m, m, m};
+      float m8[8], s8[8];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], v[i]);
-      const float mn = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-      const float b = -mn * kLog2e;
-      float s4[4] = {s * ex2_approx((m - mn) * kLog2e), 0.f, 0.f, 0.f};
+      for (int i = 0; i < 8; ++i) m8[i] = kLowest, s8[i] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) s4[i & 3] += ex2_approx(fmaf(v[i], kLog2e, b));
-      s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
-      m = mn;
-      const int64_t at = t - (col0 + c);
-      if (at >= 0 && at < 32 && t < a.vocab) {
-        float x = 0.f;
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int i = 0; i < 32; ++i) x = at == i ? v[i] : x;
-        a.target_logit[row] = x;
+        for (int i = 0; i < 32; ++i) m8[i & 7] = fmaxf(m8[i & 7], v[c][i]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = fmaxf(m, m8[i]);
+      const float b = -m * kLog2e;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) s8[i & 7] += ex2_approx(fmaf(v[c][i], kLog2e, b));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += s8[i];
+      const int at = rw.t - col0;
+      if (at >= 0 && at < 32 * NC) {
+        float y = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) y = at == 32 * c + i ? v[c][i] : y;
+        a.target_logit[row] = y;
       }
     }
     // The row's other half is in the warp with the same lanes: its pair comes through shared
@@ -290,32 +318,43 @@ struct CeBwdArgs {
 template <int BN, bool BF16>
 struct EpiCeBwd {
   using Args = CeBwdArgs;
-  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, const EpiCtx& e) {
-    const int row = e.row0 + e.lane;
+  struct Row {
+    float g, b;
+    int t;
+  };
+  __device__ static __forceinline__ Row row(const Args& a, int row) {
     const bool ok = row < a.rows;
-    const float g = ok ? __ldg(a.weight + row) : 0.f;
-    const float b = ok ? -__ldg(a.lse + row) * kLog2e : 0.f;
-    const int64_t t = ok ? __ldg(a.targets + row) : -1;
+    return Row{ok ? __ldg(a.weight + row) : 0.f, ok ? -__ldg(a.lse + row) * kLog2e : 0.f,
+               ce_target(a.targets, row, a.rows, a.vocab)};
+  }
+  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, const Row& rw,
+                                              const EpiCtx& e) {
     const int off = e.half * (BN / 2);
     uint16_t* base = reinterpret_cast<uint16_t*>(a.d) + (int64_t)e.row0 * a.ldd + w.nt * BN + off;
+    const float g = rw.g, b = rw.b;
+    const uint32_t mask = g == 0.f ? 0u : 0xffffffffu;  // an ignored row adds nothing, whatever it holds
+    uint32_t x[32];
+    e.fetch(off, x);
 #pragma unroll 1
     for (int c = 0; c < BN / 2; c += 32) {
       const int col = a.piece0 + w.nt * BN + off + c;
       float v[32];
-      e.read(off + c, v);
+      e.settle();
+      e.values(x, v);
+      if (c + 32 < BN / 2) e.fetch(off + c + 32, x);
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = ex2_approx(fmaf(v[i], kLog2e, b)) * g;
-      const int64_t at = t - col;
+      const int at = rw.t - col;
       if (at >= 0 && at < 32) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = at == i ? v[i] - g : v[i];
       }
-      if (g == 0.f || col + 32 > a.vocab) {  // an ignored row adds nothing, whatever its logits
+      if (col + 32 > a.vocab) {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
-          if (g == 0.f || col + i >= a.vocab) v[i] = 0.f;
+          if (col + i >= a.vocab) v[i] = 0.f;
       }
-      store_block16<BF16>(e, v, base, a.ldd, a.rows - e.row0, c, BN / 2, true);
+      store_block16<BF16>(e, v, base, a.ldd, a.rows - e.row0, c, BN / 2, true, mask);
     }
   }
 };
