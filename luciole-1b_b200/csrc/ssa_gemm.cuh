@@ -688,6 +688,9 @@ int launch_gemm(const GemmProduct<Epi>& p0, const GemmProduct<Epi>* p1, cudaStre
   constexpr int dtype = BF16 ? SSA_DTYPE_BF16 : SSA_DTYPE_F16;
   CUtensorMap t[4];
   const GemmProduct<Epi>& q1 = p1 ? *p1 : p0;
+  const int64_t u0 = (int64_t)p0.g.tiles_m * p0.g.tiles_n * p0.g.splits;
+  const int64_t u1 = p1 ? (int64_t)q1.g.tiles_m * q1.g.tiles_n * q1.g.splits : 0;
+  if (u0 + u1 > INT32_MAX / 2) return abi_error(SSA_ERR_BAD_SHAPE, "too many tiles");
   GemmWork w{};
   w.g[0] = p0.g;
   w.g[1] = q1.g;
@@ -710,9 +713,6 @@ int launch_gemm(const GemmProduct<Epi>& p0, const GemmProduct<Epi>* p1, cudaStre
     if (rc != SSA_OK) return rc;
   }
   if (!p1) t[2] = t[0], t[3] = t[1];
-  const int64_t u0 = (int64_t)p0.g.tiles_m * p0.g.tiles_n * p0.g.splits;
-  const int64_t u1 = p1 ? (int64_t)q1.g.tiles_m * q1.g.tiles_n * q1.g.splits : 0;
-  if (u0 + u1 > INT32_MAX / 2) return abi_error(SSA_ERR_BAD_SHAPE, "too many tiles");
   const int most = device_sm_count() / CG;
   const int workers = (int)(u0 + u1 < most ? u0 + u1 : most);
   w.lead = p1 && q1.g.kb_split > p0.g.kb_split ? 1 : 0;

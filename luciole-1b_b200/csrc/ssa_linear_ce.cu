@@ -265,13 +265,28 @@ __global__ void __launch_bounds__(1024)
 // the gradients of 8192 rows before). One gradient per row: grad_r times the power of two that
 // brings the largest to [2^14, 2^15), and its exact inverse. The power of two keeps the small
 // probabilities of a large vocabulary normal numbers in fp16. Ignored rows: 0.
+//
+// Blocks after the first copy x with ignored rows as zeros, for the product that sums over rows: what
+// an ignored row holds (padding, an infinity) must not reach dW as 0 times it.
 __global__ void __launch_bounds__(1024)
     ce_row_weights_kernel(const float* grad, int per_row, const int64_t* targets,
                           int64_t ignore_index, int rows, int vocab, const float* count, int mean,
-                          float* weight, float* inv) {
+                          float* weight, float* inv, const uint16_t* x, int64_t ldx, int hidden,
+                          uint16_t* x_kept) {
   __shared__ float red[32];
   griddep_wait();
   griddep_launch_dependents();
+  if (blockIdx.x > 0) {
+    const int chunks = hidden / 8;  // of 16 bytes, per row
+    const int64_t total = (int64_t)rows * chunks, step = (int64_t)(gridDim.x - 1) * 1024;
+    for (int64_t i = (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x; i < total; i += step) {
+      const int row = (int)(i / chunks), c = (int)(i - (int64_t)row * chunks);
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(x + (int64_t)row * ldx) + c);
+      reinterpret_cast<uint4*>(x_kept)[i] =
+          __ldg(targets + row) == ignore_index ? make_uint4(0u, 0u, 0u, 0u) : v;
+    }
+    return;
+  }
   float up = 16384.f;
   if (per_row) {
     float top = 0.f;
@@ -375,7 +390,7 @@ struct CePlan {
   int pieces;
   int dx_splits;
   size_t off_target, off_rows, fwd_bytes;
-  size_t off_inv, off_d, off_sum, bwd_bytes;
+  size_t off_inv, off_x, off_d, off_sum, bwd_bytes;
 };
 
 CePlan ce_plan(const ssa_linear_ce_t* p) {
@@ -402,7 +417,8 @@ CePlan ce_plan(const ssa_linear_ce_t* p) {
   q.dx_splits = split_count(dx_tiles, (int)(q.ldd / 64), dw_tiles * (cdiv(rows, 64) + kTileCost),
                             q.bwd.workers);
   q.off_inv = up256(sizeof(float) * rows);
-  q.off_d = q.off_inv + 256;
+  q.off_x = q.off_inv + 256;
+  q.off_d = q.off_x + up256(2 * (size_t)rows * p->hidden);
   q.off_sum = q.off_d + up256(2 * (size_t)rows * q.ldd);
   q.bwd_bytes = q.off_sum;
   if (q.pieces > 1 || q.dx_splits > 1)
@@ -488,9 +504,14 @@ int ce_bwd(const ssa_linear_ce_t* p, const CePlan& q, const float* lse, const fl
   float* inv = reinterpret_cast<float*>(ws + q.off_inv);
   uint8_t* d = ws + q.off_d;
   float* sum = reinterpret_cast<float*>(ws + q.off_sum);
-  const cudaError_t e = launch_pdl(ce_row_weights_kernel, dim3(1), dim3(1024), 0, st, grad,
-                                   (int)(p->reduction == 0), p->targets, p->ignore_index, p->rows,
-                                   p->vocab, count, (int)(p->reduction == 1), weight, inv);
+  uint16_t* x_kept = reinterpret_cast<uint16_t*>(ws + q.off_x);
+  int copies = dw ? cdiv((int64_t)p->rows * (p->hidden / 8), 4 * 1024) : 0;
+  if (copies > 2 * device_sm_count()) copies = 2 * device_sm_count();
+  const cudaError_t e =
+      launch_pdl(ce_row_weights_kernel, dim3((unsigned)(1 + copies)), dim3(1024), 0, st, grad,
+                 (int)(p->reduction == 0), p->targets, p->ignore_index, p->rows, p->vocab, count,
+                 (int)(p->reduction == 1), weight, inv, static_cast<const uint16_t*>(p->x),
+                 p->x_stride, p->hidden, x_kept);
   if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "ce_row_weights: %s", cudaGetErrorString(e));
   note_launches(1);
   for (int i = 0; i < q.pieces; ++i) {
@@ -522,7 +543,7 @@ int ce_bwd(const ssa_linear_ce_t* p, const CePlan& q, const float* lse, const fl
                                      2 * (int64_t)p->rows * q.ldd);
     const GemmOperand dk{d, p->rows, wide, q.ldd, "d"}, dmn{d, wide, p->rows, q.ldd, "d"};
     const GemmOperand wb{w0, p->hidden, cols, p->w_stride, "w"};
-    const GemmOperand xb{p->x, p->hidden, p->rows, p->x_stride, "x"};
+    const GemmOperand xb{x_kept, p->hidden, p->rows, p->hidden, "x"};
     const StoreProduct px{dk, wb, gx, sx}, pw{dmn, xb, gw, sw};
     rc = launch_gradients(BF16, q.bwd, dx ? &px : nullptr, dw ? &pw : nullptr, st);
     if (rc != SSA_OK) return rc;

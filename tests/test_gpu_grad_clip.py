@@ -162,3 +162,9 @@ def test_refusals(cuda_device):
         with pytest.raises(ValueError, match=match):
             ssa_clip_grad_norm(grads, **kw)
     assert torch.equal(a, torch.ones(8, device=dev))
+
+
+def test_only_empty_tensors(cuda_device):
+    from SSA.ssa_grad_clip import ssa_clip_grad_norm, ssa_grad_norm
+    empty = [torch.zeros(0, 3, device=cuda_device), torch.zeros(0, device=cuda_device)]
+    assert float(ssa_grad_norm(empty)) == 0.0 and float(ssa_clip_grad_norm(empty, 1.0)) == 0.0

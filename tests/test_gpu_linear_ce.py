@@ -235,3 +235,68 @@ def test_refusals(cuda_device):
             ((x.cpu(), w, t), {}, "CUDA")):
         with pytest.raises(ValueError, match=match):
             f(*args, **kw)
+
+
+def test_what_an_ignored_row_holds_reaches_nothing(cuda_device):
+    """Infinities and NaN in the hidden states of ignored rows (padding): the other rows' losses and
+    every gradient are as without them."""
+    x, w, t = _data(200, 128, 777, torch.bfloat16, 43, 0.3, cuda_device)
+    want = _check(x, w, t)
+    dirty = x.clone()
+    skip = t == -100
+    dirty[skip] = float("nan")
+    dirty[skip.nonzero()[0, 0]] = float("inf")
+    from SSA.ssa_cross_entropy import ssa_linear_cross_entropy
+    xl, wl = dirty.requires_grad_(True), w.clone().requires_grad_(True)
+    loss = ssa_linear_cross_entropy(xl, wl, t)
+    assert torch.equal(loss, want[0])
+    grad = torch.rand(loss.shape, device=x.device) + 0.5
+    gx, gw = torch.autograd.grad(loss, (xl, wl), grad)
+    clean = x.clone().requires_grad_(True)
+    a, b = torch.autograd.grad(ssa_linear_cross_entropy(clean, wl, t), (clean, wl), grad)
+    assert torch.equal(gx, a) and torch.equal(gw, b) and not gx[skip].any()
+
+
+def test_two_streams_at_once(cuda_device):
+    from SSA.ssa_cross_entropy import ssa_linear_cross_entropy
+    sets = [_data(700, 256, 9001, torch.bfloat16, 50 + i, 0.1, cuda_device) for i in range(2)]
+
+    def step(x, w, t):
+        x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        loss = ssa_linear_cross_entropy(x, w, t)
+        return [loss.detach(), *torch.autograd.grad(loss, (x, w))]
+
+    want = [step(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(4):
+        for i, (st, s) in enumerate(zip(streams, sets)):
+            with torch.cuda.stream(st):
+                got[i] = step(*s)
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_device_timeout_shows_as_nan(cuda_device):
+    """With the device status set (a self-test wait that runs out), the tensor-core products write NaN;
+    once it is read, results are back."""
+    from SSA import _lib, check_device_status
+    from SSA.ssa_cross_entropy import ssa_linear_cross_entropy
+    from SSA.ssa_gated_ffn import ssa_gated_ffn
+    x, w, t = _data(300, 128, 2000, torch.bfloat16, 61, 0.1, cuda_device)
+    xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    good = ssa_linear_cross_entropy(xl, wl, t)
+    fw = w[:1000].detach()
+    h = ssa_gated_ffn(x, fw)
+    lib = _lib.load()
+    _lib.check(lib.ssa_selftest_device_timeout(1_000_000, _lib.stream_ptr(cuda_device)))
+    bad = ssa_linear_cross_entropy(xl, wl, t)
+    gx, gw = torch.autograd.grad(good, (xl, wl), retain_graph=True)
+    assert torch.isnan(bad) and torch.isnan(gx[t != -100]).all() and torch.isnan(gw).all()
+    assert torch.isnan(ssa_gated_ffn(x, fw)).all()
+    with pytest.raises(_lib.SSAKernelError):
+        check_device_status()
+    assert torch.equal(ssa_linear_cross_entropy(xl, wl, t), good)
+    assert torch.equal(ssa_gated_ffn(x, fw), h)
