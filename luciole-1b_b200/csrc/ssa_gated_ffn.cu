@@ -281,7 +281,7 @@ int ffn_bwd(const ssa_gated_ffn_t* p, const FfnPlan& q, const void* dh, int64_t 
   rc = launch_gradients(BF16, q.bwd, dx ? &px : nullptr, dw ? &pw : nullptr, st);
   if (rc != SSA_OK) return rc;
   if (dx && q.dx_splits > 1)
-    return launch_sum_splits(BF16, sum, dx, nullptr, p->rows, p->hidden, p->hidden, q.dx_splits, st);
+    return launch_sum_splits(BF16, sum, dx, nullptr, nullptr, p->rows, p->hidden, p->hidden, q.dx_splits, st);
   return SSA_OK;
 }
 

@@ -26,11 +26,15 @@ namespace {
 template <int BN, bool BF16>
 struct EpiStore {
   using Args = StoreArgs;
-  struct Row {};
-  __device__ static __forceinline__ Row row(const Args&, int) { return Row{}; }
-  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, const Row&,
+  struct Row {
+    float scale;
+  };
+  __device__ static __forceinline__ Row row(const Args& a, int row) {
+    return Row{a.row_scale && row < a.rows ? __ldg(a.row_scale + row) : 1.f};
+  }
+  __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, const Row& rw,
                                               const EpiCtx& e) {
-    const float sc = a.scale ? __ldg(a.scale) : 1.f;
+    const float sc = (a.scale ? __ldg(a.scale) : 1.f) * rw.scale;
     const int col0 = w.nt * BN + e.half * (BN / 2);
     const int n = min(BN / 2, ((a.cols - col0 + 31) >> 5) << 5);  // columns of this warp, whole 32s
     if (n <= 0) return;
@@ -88,17 +92,19 @@ struct EpiStore {
 // out[row, col] = scale * sum over splits, in split order (deterministic).
 template <bool BF16>
 __global__ void __launch_bounds__(256) sum_splits_kernel(const float* sum, void* out,
-                                                         const float* scale, int64_t rows, int cols,
-                                                         int64_t ldo, int splits) {
+                                                         const float* scale, const float* row_scale,
+                                                         int64_t rows, int cols, int64_t ldo,
+                                                         int splits) {
   griddep_wait();
   griddep_launch_dependents();
-  const float sc = scale ? __ldg(scale) : 1.f;
+  const float all = scale ? __ldg(scale) : 1.f;
   const int per_row = cols / 4;
   const int64_t total = rows * per_row, plane = rows * (int64_t)cols;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t row = i / per_row;
     const int col = (int)(i - row * per_row) * 4;
     const float* p = sum + row * cols + col;
+    const float sc = row_scale ? all * __ldg(row_scale + row) : all;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int k = 0; k < splits; ++k) {
       const float4 x = *reinterpret_cast<const float4*>(p + k * plane);
@@ -133,16 +139,17 @@ int launch_gradients(bool bf16, const GemmForm& form, const StoreProduct* dx, co
   return bf16 ? gradients_form<true>(form, dx, dw, st) : gradients_form<false>(form, dx, dw, st);
 }
 
-int launch_sum_splits(bool bf16, const float* sum, void* out, const float* scale, int64_t rows,
-                      int cols, int64_t ldo, int splits, cudaStream_t st) {
+int launch_sum_splits(bool bf16, const float* sum, void* out, const float* scale,
+                      const float* row_scale, int64_t rows, int cols, int64_t ldo, int splits,
+                      cudaStream_t st) {
   const int64_t blocks = (rows * (cols / 4) + 255) / 256;
   const int64_t most = (int64_t)device_sm_count() * 8;
   const dim3 grid((unsigned)(blocks < most ? blocks : most));
   const cudaError_t e =
-      bf16 ? launch_pdl(sum_splits_kernel<true>, grid, dim3(256), 0, st, sum, out, scale, rows, cols,
-                        ldo, splits)
-           : launch_pdl(sum_splits_kernel<false>, grid, dim3(256), 0, st, sum, out, scale, rows, cols,
-                        ldo, splits);
+      bf16 ? launch_pdl(sum_splits_kernel<true>, grid, dim3(256), 0, st, sum, out, scale,
+                        row_scale, rows, cols, ldo, splits)
+           : launch_pdl(sum_splits_kernel<false>, grid, dim3(256), 0, st, sum, out, scale,
+                        row_scale, rows, cols, ldo, splits);
   if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "sum_splits: %s", cudaGetErrorString(e));
   note_launches(1);
   return SSA_OK;

@@ -824,6 +824,7 @@ struct StoreArgs {
   void* out;             // 16-bit [.., ldo], or nullptr
   float* sum;            // fp32 [splits][rows][cols], or nullptr
   const float* scale;    // device scalar, or nullptr (1)
+  const float* row_scale;  // one factor per row (out only), or nullptr
   int64_t ldo;
   int rows, cols;        // cols: a multiple of 8
   int add_prev;          // add to sum
@@ -842,9 +843,11 @@ struct StoreProduct {
 int launch_gradients(bool bf16, const GemmForm& form, const StoreProduct* dx, const StoreProduct* dw,
                      cudaStream_t st);
 
-// out[row, col] = scale * (the splits' sums [splits][rows][cols], added in split order).
-int launch_sum_splits(bool bf16, const float* sum, void* out, const float* scale, int64_t rows,
-                      int cols, int64_t ldo, int splits, cudaStream_t st);
+// out[row, col] = scale * row_scale[row] * (the splits' sums [splits][rows][cols], added in split
+// order); either factor may be nullptr.
+int launch_sum_splits(bool bf16, const float* sum, void* out, const float* scale,
+                      const float* row_scale, int64_t rows, int cols, int64_t ldo, int splits,
+                      cudaStream_t st);
 
 }  // namespace sm100
 }  // namespace ssa

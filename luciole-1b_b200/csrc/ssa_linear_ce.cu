@@ -73,13 +73,14 @@ struct EpiCeFwd {
         for (int i = 0; i < 32; ++i) m8[i & 7] = fmaxf(m8[i & 7], v[c][i]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) m = fmaxf(m, m8[i]);
-      const float b = -m * kLog2e;
+      const float b = -m * kLog2e, lost = fmaf(-m, kLog2e, -b);  // b's rounding: 2^lost on every term
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int i = 0; i < 32; ++i) s8[i & 7] += ex2_approx(fmaf(v[c][i], kLog2e, b));
 #pragma unroll
       for (int i = 0; i < 8; ++i) s += s8[i];
+      s = fmaf(s, lost * kLn2, s);
       const int at = rw.t - col0;
       if (at >= 0 && at < 32 * NC) {
         float y = 0.f;
@@ -258,21 +259,33 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// What the backward multiplies (p - [v = t]) by before it is rounded to 16 bits, and the factor `inv` of
-// the products' epilogues. One gradient for all rows (mean, sum): 2^14 and grad / count 2^-14, so that
+// A gradient as +- 2^e times the rest in [0.5, 1); one that is 0 or not finite is its own factor.
+__device__ __forceinline__ float split_power(float g, float& rest) {
+  rest = 1.f;
+  if (g == 0.f || !(fabsf(g) < INFINITY)) return g;
+  int e;
+  rest = fabsf(frexpf(g, &e));
+  return copysignf(ldexpf(1.f, min(e, 127)), g) * (e > 127 ? 2.f : 1.f);
+}
+
+// What the backward multiplies (p - [v = t]) by before it is rounded to 16 bits: a power of two, so that
 // the target's p - 1, which weighs most, is rounded as a number just below a power of two and not
-// times an arbitrary factor that would put the same error, up to 2^-8 in bf16, on every row (0.4% of
-// the gradients of 8192 rows before). One gradient per row: grad_r times the power of two that
-// brings the largest to [2^14, 2^15), and its exact inverse. The power of two keeps the small
-// probabilities of a large vocabulary normal numbers in fp16. Ignored rows: 0.
+// times an arbitrary factor that would put one error, up to 2^-8 in bf16, on a whole row (0.4% of the
+// gradients of 8192 rows before). The rest of each gradient enters elsewhere:
+//   one for all rows (mean, sum): the power is 2^14, `inv` = grad / count 2^-14 in the epilogues;
+//   one per row: grad_r = +- 2^e rest_r. The powers are brought to at most 2^14 by another that `inv`
+//   undoes; rest_r multiplies row r of dx in its epilogue, and row r of the copy of x for dW.
+// 2^14 keeps the small probabilities of a large vocabulary normal numbers in fp16. Ignored rows: 0.
 //
-// Blocks after the first copy x with ignored rows as zeros, for the product that sums over rows: what
-// an ignored row holds (padding, an infinity) must not reach dW as 0 times it.
+// Blocks after the first make that copy of x, with ignored rows as zeros, for the product that sums over
+// rows: what an ignored row holds (padding, an infinity) must not reach dW as 0 times it.
+template <bool BF16>
 __global__ void __launch_bounds__(1024)
     ce_row_weights_kernel(const float* grad, int per_row, const int64_t* targets,
                           int64_t ignore_index, int rows, int vocab, const float* count, int mean,
-                          float* weight, float* inv, const uint16_t* x, int64_t ldx, int hidden,
-                          uint16_t* x_kept) {
+                          float* weight, float* rest, float* inv, const uint16_t* x, int64_t ldx,
+                          int hidden, uint16_t* x_kept) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   __shared__ float red[32];
   griddep_wait();
   griddep_launch_dependents();
@@ -281,7 +294,14 @@ __global__ void __launch_bounds__(1024)
     const int64_t total = (int64_t)rows * chunks, step = (int64_t)(gridDim.x - 1) * 1024;
     for (int64_t i = (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x; i < total; i += step) {
       const int row = (int)(i / chunks), c = (int)(i - (int64_t)row * chunks);
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(x + (int64_t)row * ldx) + c);
+      uint4 v = __ldg(reinterpret_cast<const uint4*>(x + (int64_t)row * ldx) + c);
+      if (per_row) {
+        float r;
+        split_power(__ldg(grad + row), r);
+        T* t = reinterpret_cast<T*>(&v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t[k] = from_f32<T>(to_f32<T>(t[k]) * r);
+      }
       reinterpret_cast<uint4*>(x_kept)[i] =
           __ldg(targets + row) == ignore_index ? make_uint4(0u, 0u, 0u, 0u) : v;
     }
@@ -298,7 +318,7 @@ __global__ void __launch_bounds__(1024)
     top = red[threadIdx.x & 31];
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     int e = 0;
-    if (top > 0.f && top < INFINITY) e = max(-126, min(126, 14 - ilogbf(top)));
+    if (top > 0.f && top < INFINITY) e = max(-126, min(126, 13 - ilogbf(top)));
     up = ldexpf(1.f, e);
     if (threadIdx.x == 0) *inv = ldexpf(1.f, -e);
   } else if (threadIdx.x == 0) {
@@ -313,7 +333,9 @@ __global__ void __launch_bounds__(1024)
     for (int k = 0; k < 4; ++k) {
       const int at = i + 1024 * k;
       if (at >= rows) break;
-      float g = per_row ? grad[at] * up : up;
+      float g = up, r = 1.f;
+      if (per_row) g = split_power(grad[at], r) * up;
+      if (per_row) rest[at] = r;
       if (t[k] == ignore_index) g = 0.f;
       else if (t[k] < 0 || t[k] >= vocab) g = nan_f32();
       weight[at] = g;
@@ -390,7 +412,7 @@ struct CePlan {
   int pieces;
   int dx_splits;
   size_t off_target, off_rows, fwd_bytes;
-  size_t off_inv, off_x, off_d, off_sum, bwd_bytes;
+  size_t off_rest, off_inv, off_x, off_d, off_sum, bwd_bytes;
 };
 
 CePlan ce_plan(const ssa_linear_ce_t* p) {
@@ -416,7 +438,8 @@ CePlan ce_plan(const ssa_linear_ce_t* p) {
   const int64_t dw_tiles = (int64_t)cdiv(q.ldd, q.bwd.bm) * cdiv(p->hidden, q.bwd.bn);
   q.dx_splits = split_count(dx_tiles, (int)(q.ldd / 64), dw_tiles * (cdiv(rows, 64) + kTileCost),
                             q.bwd.workers);
-  q.off_inv = up256(sizeof(float) * rows);
+  q.off_rest = up256(sizeof(float) * rows);
+  q.off_inv = 2 * q.off_rest;
   q.off_x = q.off_inv + 256;
   q.off_d = q.off_x + up256(2 * (size_t)rows * p->hidden);
   q.off_sum = q.off_d + up256(2 * (size_t)rows * q.ldd);
@@ -501,16 +524,18 @@ template <bool BF16>
 int ce_bwd(const ssa_linear_ce_t* p, const CePlan& q, const float* lse, const float* count,
            const float* grad, void* dx, void* dw, uint8_t* ws, cudaStream_t st) {
   float* weight = reinterpret_cast<float*>(ws);
+  float* rest = reinterpret_cast<float*>(ws + q.off_rest);
   float* inv = reinterpret_cast<float*>(ws + q.off_inv);
+  const bool per_row = p->reduction == 0;
   uint8_t* d = ws + q.off_d;
   float* sum = reinterpret_cast<float*>(ws + q.off_sum);
   uint16_t* x_kept = reinterpret_cast<uint16_t*>(ws + q.off_x);
   int copies = dw ? cdiv((int64_t)p->rows * (p->hidden / 8), 4 * 1024) : 0;
   if (copies > 2 * device_sm_count()) copies = 2 * device_sm_count();
   const cudaError_t e =
-      launch_pdl(ce_row_weights_kernel, dim3((unsigned)(1 + copies)), dim3(1024), 0, st, grad,
-                 (int)(p->reduction == 0), p->targets, p->ignore_index, p->rows, p->vocab, count,
-                 (int)(p->reduction == 1), weight, inv, static_cast<const uint16_t*>(p->x),
+      launch_pdl(ce_row_weights_kernel<BF16>, dim3((unsigned)(1 + copies)), dim3(1024), 0, st, grad,
+                 (int)per_row, p->targets, p->ignore_index, p->rows, p->vocab, count,
+                 (int)(p->reduction == 1), weight, rest, inv, static_cast<const uint16_t*>(p->x),
                  p->x_stride, p->hidden, x_kept);
   if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "ce_row_weights: %s", cudaGetErrorString(e));
   note_launches(1);
@@ -529,6 +554,7 @@ int ce_bwd(const ssa_linear_ce_t* p, const CePlan& q, const float* lse, const fl
     sx.out = q.dx_splits == 1 && q.pieces == 1 ? dx : nullptr;
     sx.sum = sum;
     sx.scale = sw.scale = inv;
+    sx.row_scale = per_row ? rest : nullptr;
     sx.rows = p->rows;
     sx.ldo = sx.cols = sw.ldo = sw.cols = p->hidden;
     sx.add_prev = i > 0;
@@ -549,7 +575,8 @@ int ce_bwd(const ssa_linear_ce_t* p, const CePlan& q, const float* lse, const fl
     if (rc != SSA_OK) return rc;
   }
   if (dx && (q.dx_splits > 1 || q.pieces > 1))
-    return launch_sum_splits(BF16, sum, dx, inv, p->rows, p->hidden, p->hidden, q.dx_splits, st);
+    return launch_sum_splits(BF16, sum, dx, inv, per_row ? rest : nullptr, p->rows, p->hidden,
+                             p->hidden, q.dx_splits, st);
   return SSA_OK;
 }
 

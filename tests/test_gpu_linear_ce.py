@@ -5,7 +5,10 @@ instructions, each adding with an error of at most a few steps of 2^-23 relative
 magnitudes A = sum |x||w|; DL = (H / 8 + 8) 2^-23 A bounds it. A row's loss is off by at most
 2 DL plus a few fp32 roundings of the loss. d is rounded once to 16 bits (u = eps / 2 relative) after
 exponentials whose argument is off by up to 2 DL, the sums over it run in fp32, and the result is
-rounded once: |dx error| <= (u + 2 DL + 2^-16) |d| |W| + u |dx|, elementwise."""
+rounded once: |dx error| <= (u + 2 DL + 2^-16) |d| |W| + u |dx|, elementwise. With one gradient per
+row (reduction "none") its fraction multiplies x in the sum for dW and that product is rounded to 16
+bits as well: each term is a product of two rounded factors, so dW's bound has 2 u (and u^2, inside
+2^-16) where the others have u."""
 
 import math
 
@@ -51,7 +54,7 @@ def _reference(x, w, t, reduction, grad, ignore_index=-100):
     D[torch.arange(len(t), device=t.device), at] += 2 * dl * gr.abs()
     tiny = torch.finfo(x.dtype).tiny * torch.finfo(x.dtype).eps  # subnormal results: half a step
     bdx = e * (D @ W.abs()) + u * dx.abs() + tiny
-    bdw = e * (D.t() @ X.abs()) + u * dw.abs() + tiny
+    bdw = (e + (u if reduction == "none" else 0.0)) * (D.t() @ X.abs()) + u * dw.abs() + tiny
     return loss, dx, dw, 2 * dl, bdx, bdw
 
 
