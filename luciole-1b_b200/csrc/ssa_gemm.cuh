@@ -325,9 +325,8 @@ __device__ __forceinline__ void store_block16(const EpiCtx& e, const float (&v)[
 
 // Epi: struct with `Args`, `Row`, `static Row row(const Args&, int row)`, which reads what a lane needs
 // to know of its row, and `static void tile(const Args&, const GemmUnit&, const Row&, const EpiCtx&)`,
-// run by every epilogue warp for each unit; the next unit's rows are read before this one's
-// tile. A_MODE: 0 A is K-major, 1 MN-major, 2 K-major in product 0
-// and MN-major in product 1.
+// run by every epilogue warp for each unit; the next unit's rows are read before this one's tile.
+// A_MODE: 0 A is K-major, 1 MN-major, 2 K-major in product 0 and MN-major in product 1.
 template <class Epi, int CG, int BN, int NH, int A_MODE, bool B_MN, bool BF16>
 __global__ void __launch_bounds__(320, 1)
     gemm_sm100_kernel(const __grid_constant__ CUtensorMap tmA0,
@@ -401,7 +400,7 @@ __global__ void __launch_bounds__(320, 1)
   // Warps 0 and 1 share their schedulers with epilogue warps and get few issue slots beside them, so
   // their loops are kept to what each K block needs: running stage and phase, no division, the
   // abort flag looked at once per unit, the unit's decoding left to the producer (which runs
-  // ahead). Measured on B200, see below.
+  // ahead). Loss forward of 8192 x 2048, vocabulary 65,536: 1647 us before, 1528 us so.
   const int count = gemm_count(work, worker, workers);
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
@@ -684,7 +683,6 @@ struct GemmProduct {
 template <class Epi, int CG, int BN, int NH, int A_MODE, bool B_MN, bool BF16>
 int launch_gemm(const GemmProduct<Epi>& p0, const GemmProduct<Epi>* p1, cudaStream_t st) {
   using C = GemmCfg<CG, BN, NH>;
-  static_assert(A_MODE == 2 || A_MODE == 0 || A_MODE == 1, "layout of A");
   constexpr int dtype = BF16 ? SSA_DTYPE_BF16 : SSA_DTYPE_F16;
   CUtensorMap t[4];
   const GemmProduct<Epi>& q1 = p1 ? *p1 : p0;

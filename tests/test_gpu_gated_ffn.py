@@ -59,7 +59,8 @@ def _check(x, w, dh):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("n,h,f", [(1, 8, 1), (1, 64, 63), (2, 72, 200), (5, 256, 129), (9, 64, 64),
                                    (127, 64, 65), (128, 128, 128), (129, 136, 127), (300, 512, 1365),
-                                   (1, 2048, 5632), (2500, 64, 1000)])
+                                   (1, 2048, 5632), (2500, 64, 1000), (200, 512, 2001),
+                                   (4111, 264, 9001)])
 def test_forward_and_gradients(cuda_device, dtype, n, h, f):
     _check(*_data(n, h, f, dtype, n + f, cuda_device))
 

@@ -102,6 +102,13 @@ def test_many_pieces_equal_one(cuda_device):
     _check(x, w, t)
 
 
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_long_contractions(cuda_device, reduction):
+    """Sizes at which dx and dW take the 256 x 512 tiles, none of them a multiple of a tile."""
+    x, w, t = _data(4300, 520, 16001, torch.bfloat16, 15, 0.1, cuda_device)
+    _check(x, w, t, reduction)
+
+
 def test_row_weights_of_widely_different_size(cuda_device):
     x, w, t = _data(96, 128, 999, torch.float16, 11, 0.1, cuda_device)
     grad = torch.logspace(-3, 3, 96, device=cuda_device)
