@@ -358,10 +358,8 @@ __global__ void __launch_bounds__(320, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
   const int worker = (int)blockIdx.x / CG, workers = (int)gridDim.x / CG;
-  // Launched programmatically: nothing global is touched before the previous kernel is done.
-  griddep_wait();
-  griddep_launch_dependents();
-
+  // Launched programmatically: the set-up of this CTA may run while the previous kernel still does;
+  // nothing global is touched before that is done.
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(full(s), 1);
@@ -373,13 +371,17 @@ __global__ void __launch_bounds__(320, 1)
     }
     mbar_init(bar_end, 1);
     *abort_flag = 0;
-    *status_slot = *reinterpret_cast<const volatile unsigned int*>(work.status);
     fence_mbar_init();
+    prefetch_tmap(&tmA0);
+    prefetch_tmap(&tmB0);
   }
   if (warp == 1) {
     __syncwarp();
     tmem_alloc_cg<CG>(smem_u32(tmem_slot), C::TMEM_COLS);
   }
+  griddep_wait();
+  griddep_launch_dependents();
+  if (threadIdx.x == 0) *status_slot = *reinterpret_cast<const volatile unsigned int*>(work.status);
   tc_fence_before();
   __syncthreads();
   if constexpr (CG == 2) cluster_sync();  // both CTAs' barriers are initialised
@@ -405,8 +407,6 @@ __global__ void __launch_bounds__(320, 1)
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0 && !dead) {
-      prefetch_tmap(&tmA0);
-      prefetch_tmap(&tmB0);
       int st = 0, round = 0;
       bool ok = true;
       for (int i = 0; ok && i < count; ++i) {
