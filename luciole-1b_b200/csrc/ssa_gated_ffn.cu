@@ -10,7 +10,7 @@
 // as one 16-bit matrix d = [dg | du]; then dx = d W and dW = d^T x are two plain products. Bound:
 // the tensor cores, 16 rows hidden ffn operations for forward and backward against the 12 that
 // kept pre-activations would need (at 8 bytes of memory per row and ffn column, held over the whole
-// forward).
+// forward). A forward of few rows has a kernel of its own, bound by memory.
 #include "ssa_gemm.cuh"
 
 namespace ssa {
@@ -127,53 +127,92 @@ struct EpiFfnBwd {
   }
 };
 
-// One row: a warp per output column, dot products on the CUDA cores. Bound: memory, every weight read
-// once. At hidden 2048, ffn 5632 (46 MB, from L2) 8.8 us against 13.3 us for 128-row tiles, of which
-// there are 88 for 148 multiprocessors; at two rows the conversions already cost more (12.2 us
-// and up).
+// mma m16n8k16, fp32 accumulators: c[0], c[1] are row lane / 4, c[2], c[3] row lane / 4 + 8.
 template <typename T>
-__global__ void __launch_bounds__(256)
-    ffn_row_kernel(const T* x, const T* w, int64_t ldw, T* h, int hidden, int ffn) {
+__device__ __forceinline__ void mma_16x8(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+                 "{%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+                 "{%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Few rows: KW warps share the contraction of 8 output columns and 8 NT rows; a block has 8 / KW such
+// groups. The 16 rows of a warp's matrix instruction are 8 gate and 8 up columns, its 8 columns are
+// rows of x, so g and u of an output meet in one thread. A sum does not mind the order of its terms:
+// lane (r, t) takes the 16 bytes k = 8 t .. 8 t + 7 of weight row r as they lie in memory and hands
+// them to two instructions, x in the same order. The partial sums are joined in a fixed order. Bound:
+// memory, every weight read once per 16 rows with 16 16-byte loads per lane under way; the tensor
+// cores only save the conversions, which cost more than the reads from two rows on.
+template <typename T, int NT, int KW>
+__global__ void __launch_bounds__(256, 2)
+    ffn_rows_kernel(const T* x, int64_t ldx, const T* w, int64_t ldw, T* h, int64_t ldh, int rows,
+                    int hidden, int ffn) {
+  constexpr int kCols = 64 / KW, kLd = 20;  // a joined row: 8 gate sums, 8 up sums, 4 to part banks
+  __shared__ float part[8][8 * NT][kLd];
   griddep_wait();
   griddep_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int col = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (col >= ffn) return;
-  const T* wg = w + (int64_t)col * ldw;
-  const T* wu = w + (int64_t)(ffn + col) * ldw;
-  float g = 0.f, u = 0.f;
-  constexpr int U = 4;  // 16-byte loads of each weight row under way per lane
-  for (int k0 = lane * 8; k0 < hidden; k0 += U * 256) {
-    uint4 a[U], b[U];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, t = lane & 3;
+  const int row0 = blockIdx.y * (8 * NT), col0 = blockIdx.x * kCols;
+  const int wcol = col0 + warp / KW * 8 + r;
+  const bool live = wcol < ffn;
+  rows -= row0;
+  x += row0 * ldx;
+  h += row0 * ldh;
+  const T* wg = w + (int64_t)(live ? wcol : 0) * ldw + 8 * t;
+  const T* wu = w + (int64_t)(live ? ffn + wcol : 0) * ldw + 8 * t;
+  const T* xr = x + r * ldx + 8 * t;
+  float c[NT][4] = {};
+  constexpr int U = 4, kStep = KW * 64;  // U 64-wide pieces of the contraction under way per warp
+  for (int k0 = warp % KW * 64; k0 < hidden; k0 += U * kStep) {
+    uint4 g[U][2], u[U][2], b[U][2][NT];
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int k = k0 + i * 256;
-      const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-      a[i] = k < hidden ? __ldg(reinterpret_cast<const uint4*>(wg + k)) : z;
-      b[i] = k < hidden ? __ldg(reinterpret_cast<const uint4*>(wu + k)) : z;
-    }
+    for (int i = 0; i < U; ++i)
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int k = k0 + i * 256;
-      if (k >= hidden) break;
-      const uint4 c = __ldg(reinterpret_cast<const uint4*>(x + k));
-      const T* ta = reinterpret_cast<const T*>(&a[i]);
-      const T* tb = reinterpret_cast<const T*>(&b[i]);
-      const T* tx = reinterpret_cast<const T*>(&c);
+      for (int j = 0; j < 2; ++j) {
+        const int k = k0 + i * kStep + j * 32;
+        const bool in = k + 8 * t < hidden;
+        const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+        g[i][j] = in && live ? __ldg(reinterpret_cast<const uint4*>(wg + k)) : z;
+        u[i][j] = in && live ? __ldg(reinterpret_cast<const uint4*>(wu + k)) : z;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float v = to_f32<T>(tx[j]);
-        g = fmaf(to_f32<T>(ta[j]), v, g);
-        u = fmaf(to_f32<T>(tb[j]), v, u);
+        for (int n = 0; n < NT; ++n)
+          b[i][j][n] = in && 8 * n + r < rows
+                           ? __ldg(reinterpret_cast<const uint4*>(xr + 8 * n * ldx + k)) : z;
       }
-    }
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint4 v = b[i][j][n];
+          mma_16x8<T>(c[n], g[i][j].x, u[i][j].x, g[i][j].y, u[i][j].y, v.x, v.y);
+          mma_16x8<T>(c[n], g[i][j].z, u[i][j].z, g[i][j].w, u[i][j].w, v.z, v.w);
+        }
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    g += __shfl_xor_sync(0xffffffffu, g, o);
-    u += __shfl_xor_sync(0xffffffffu, u, o);
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) part[warp][8 * n + 2 * t + (j & 1)][r + 8 * (j >> 1)] = c[n][j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < kCols * 8 * NT; i += 256) {
+    const int row = i / kCols, col = i % kCols;
+    if (row >= rows || col0 + col >= ffn) continue;
+    float g = 0.f, u = 0.f;
+#pragma unroll
+    for (int s = 0; s < KW; ++s) {
+      g += part[col / 8 * KW + s][row][col % 8];
+      u += part[col / 8 * KW + s][row][8 + col % 8];
+    }
+    h[(int64_t)row * ldh + col0 + col] = from_f32<T>(g * sigmoid_approx(g) * u);
   }
-  if (lane == 0) h[col] = from_f32<T>(g * sigmoid_approx(g) * u);
 }
 
 }  // namespace sm100
@@ -182,14 +221,43 @@ namespace {
 
 using namespace sm100;
 
-template <typename T>
-int ffn_row(const ssa_gated_ffn_t* p, void* h, cudaStream_t st) {
-  const cudaError_t e = launch_pdl(ffn_row_kernel<T>, dim3((unsigned)cdiv(p->ffn, 8)), dim3(256), 0,
-                                   st, static_cast<const T*>(p->x), static_cast<const T*>(p->w),
-                                   p->w_stride, static_cast<T*>(h), p->hidden, p->ffn);
-  if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "ffn_row: %s", cudaGetErrorString(e));
+template <typename T, int NT, int KW>
+int ffn_rows(const ssa_gated_ffn_t* p, void* h, int64_t ldh, cudaStream_t st) {
+  const dim3 grid((unsigned)cdiv(p->ffn, 64 / KW), (unsigned)cdiv(p->rows, 8 * NT));
+  const cudaError_t e = launch_pdl(ffn_rows_kernel<T, NT, KW>, grid, dim3(256), 0, st,
+                                   static_cast<const T*>(p->x), p->x_stride,
+                                   static_cast<const T*>(p->w), p->w_stride, static_cast<T*>(h), ldh,
+                                   p->rows, p->hidden, p->ffn);
+  if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "ffn_rows: %s", cudaGetErrorString(e));
   note_launches(1);
   return SSA_OK;
+}
+
+// Warps per contraction: as few as take it with one batch of loads each.
+int few_rows_warps(const ssa_gated_ffn_t* p) {
+  return p->hidden <= 512 ? 2 : p->hidden <= 1024 ? 4 : 8;
+}
+
+// Up to 16 rows, and as long as all blocks of 16 rows take one round of the multiprocessors (two where
+// the contraction is long): 128-row tiles wait for one tile's whole contraction, so that few tiles are
+// slow however small the product. Hidden 2048, ffn 5632 (46 MB, from L2): 1 row 5.8 us, 8 rows 6.9,
+// 16 rows 9.6 against 12.8 on tiles, 32 rows would take 15.7; 180 MB of weights from memory, 8 rows
+// 28.9 us (6.2 TB/s) against 47.8. Hidden 2048, ffn 1024: 64 rows 7.2 us against 12.0.
+bool few_rows(const ssa_gated_ffn_t* p) {
+  const int64_t blocks = (int64_t)cdiv(p->ffn, 64 / few_rows_warps(p)) * cdiv(p->rows, 16);
+  return p->rows <= 16 || blocks <= (p->hidden <= 512 ? 2 : 4) * device_sm_count();
+}
+
+template <typename T>
+int ffn_few_rows(const ssa_gated_ffn_t* p, void* h, int64_t ldh, cudaStream_t st) {
+  const int kw = few_rows_warps(p);
+  if (p->rows <= 8)
+    return kw == 2   ? ffn_rows<T, 1, 2>(p, h, ldh, st)
+           : kw == 4 ? ffn_rows<T, 1, 4>(p, h, ldh, st)
+                     : ffn_rows<T, 1, 8>(p, h, ldh, st);
+  return kw == 2   ? ffn_rows<T, 2, 2>(p, h, ldh, st)
+         : kw == 4 ? ffn_rows<T, 2, 4>(p, h, ldh, st)
+                   : ffn_rows<T, 2, 8>(p, h, ldh, st);
 }
 
 struct FfnPlan {
@@ -306,8 +374,9 @@ int ssa_gated_ffn_fwd(const ssa_gated_ffn_t* p, void* h, int64_t h_stride, void*
     return abi_error(SSA_ERR_BAD_STRIDE, "gated_ffn: h's row stride is below ffn");
   if ((rc = abi_bind_device(p->x, "x")) != SSA_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (p->rows == 1)
-    return p->dtype == SSA_DTYPE_BF16 ? ffn_row<__nv_bfloat16>(p, h, st) : ffn_row<__half>(p, h, st);
+  if (few_rows(p))
+    return p->dtype == SSA_DTYPE_BF16 ? ffn_few_rows<__nv_bfloat16>(p, h, h_stride, st)
+                                      : ffn_few_rows<__half>(p, h, h_stride, st);
   const FfnPlan q = ffn_plan(p);
   const FfnFwdArgs a{h, h_stride, p->rows, p->ffn,
                      (uintptr_t)h % 16 == 0 && h_stride % 8 == 0 ? 1 : 0};

@@ -7,6 +7,7 @@ rounding u = eps / 2. The gradient d = [dg | du] is off by DL |dh| (0.5 |u| + 2.
 the sums over it run in fp32, and the results are rounded once. 2^-18 relative covers the
 exponential's and reciprocal's approximations and the fp32 sums."""
 
+import ctypes
 import math
 
 import pytest
@@ -63,6 +64,40 @@ def _check(x, w, dh):
                                    (4111, 264, 9001)])
 def test_forward_and_gradients(cuda_device, dtype, n, h, f):
     _check(*_data(n, h, f, dtype, n + f, cuda_device))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,h,f", [
+    # few rows, or few blocks of 16 rows: contractions of one batch of loads and just beyond
+    (8, 504, 40), (16, 520, 65), (17, 1016, 33), (15, 1032, 31), (9, 2056, 17), (33, 4104, 9),
+    (600, 2048, 8), (4700, 8, 3),
+    # few rows, more blocks than that: tiles
+    (127, 64, 3001), (17, 72, 5000), (100, 520, 2500), (65, 1032, 4800)])
+def test_few_rows_and_lone_row_tiles(cuda_device, dtype, n, h, f):
+    _check(*_data(n, h, f, dtype, n + f, cuda_device))
+
+
+@pytest.mark.parametrize("n", [1, 7, 8, 16, 40])
+def test_a_row_depends_on_itself_alone(cuda_device, n):
+    """Infinities and NaN in one row reach no other; a row alone gives what it gives among others;
+    nothing is written beyond the rows and columns of h."""
+    from SSA import _lib
+    from SSA.ssa_gated_ffn import _problem, ssa_gated_ffn
+    x, w, _ = _data(n, 264, 45, torch.bfloat16, 29, cuda_device)
+    h = ssa_gated_ffn(x, w)
+    bad = x.clone()
+    bad[n // 2, 3], bad[n // 2, 200] = float("inf"), float("nan")
+    got = ssa_gated_ffn(bad, w)
+    other = torch.arange(n, device=cuda_device) != n // 2
+    assert torch.equal(got[other], h[other]) and got[n // 2].isnan().all()
+    assert torch.equal(ssa_gated_ffn(x[n // 2:n // 2 + 1], w)[0], h[n // 2])
+    wide = torch.full((n + 2, 53), 7.0, dtype=x.dtype, device=cuda_device)
+    prob = _problem(x, w)
+    _lib.check(_lib.load().ssa_gated_ffn_fwd(ctypes.byref(prob), wide[1, 4:].data_ptr(), 53,
+                                             _lib.stream_ptr(x.device)))
+    assert torch.equal(wide[1:-1, 4:49], h)
+    wide[1:-1, 4:49] = 7.0
+    assert (wide == 7.0).all()
 
 
 def test_large_preactivations(cuda_device):
