@@ -127,22 +127,6 @@ struct EpiFfnBwd {
   }
 };
 
-// mma m16n8k16, fp32 accumulators: c[0], c[1] are row lane / 4, c[2], c[3] row lane / 4 + 8.
-template <typename T>
-__device__ __forceinline__ void mma_16x8(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                         uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same<T, __half>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-                 "{%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-                 "{%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
 // Few rows: KW warps share the contraction of 8 output columns and 8 NT rows; a block has 8 / KW such
 // groups. The 16 rows of a warp's matrix instruction are 8 gate and 8 up columns, its 8 columns are
 // rows of x, so g and u of an output meet in one thread. A sum does not mind the order of its terms:
@@ -245,7 +229,7 @@ int few_rows_warps(const ssa_gated_ffn_t* p) {
 // 28.9 us (6.2 TB/s) against 47.8. Hidden 2048, ffn 1024: 64 rows 7.2 us against 12.0.
 bool few_rows(const ssa_gated_ffn_t* p) {
   const int64_t blocks = (int64_t)cdiv(p->ffn, 64 / few_rows_warps(p)) * cdiv(p->rows, 16);
-  return p->rows <= 16 || blocks <= (p->hidden <= 512 ? 2 : 4) * device_sm_count();
+  return p->rows <= 16 || blocks <= (p->hidden <= 512 ? 2 : 4) * kPlanSms;
 }
 
 template <typename T>

@@ -153,67 +153,98 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// One row: the forward's logits on the CUDA cores, two vocabulary rows per warp at a time, each warp
-// keeping a running pair. Bound: memory, W read once. A 128-row tile would spend as long on its
-// unused rows: at hidden 2048, vocabulary 65,536 (268 MB) 50.5 us here, 59 us there; at two rows
-// this form's conversions already cost more (69 us).
-constexpr int kRowBlocks = 148 * 4;
-
-template <typename T>
-__global__ void __launch_bounds__(256)
-    ce_row_kernel(const T* x, const T* w, int64_t ldw, int hidden, const CeFwdArgs a) {
-  __shared__ float2 sh[8];
+// Few rows: the forward without tiles. KW warps share the contraction of 16 vocabulary rows with
+// 8 NT rows of x, 8 / KW such groups a block; blocks walk the vocabulary. The 16 x 8 matrix
+// instruction takes W's rows as they lie in memory: lane (r, t) hands the 16 bytes k = 8 t .. 8 t + 7
+// of rows r and r + 8 to two instructions, x in the same order, which changes only the order of the
+// sum's terms. Every thread keeps the running pair of a row over its share of the columns. Bound:
+// memory, W read once per 16 rows.
+template <typename T, int NT, int KW>
+__global__ void __launch_bounds__(256, 2)
+    ce_rows_kernel(const T* x, int64_t ldx, const T* w, int64_t ldw, int hidden, const CeFwdArgs a) {
+  constexpr int kCols = 128 / KW, kLd = 20;  // a joined row: 16 logits, 4 to part the banks
+  constexpr int kOut = kCols * 8 * NT, kPer = (kOut + 255) / 256;  // logits of a step, and per thread
+  static_assert(kCols == 16 || kCols == 32, "a row's columns are lanes of one warp");
+  __shared__ float part[2][8][8 * NT][kLd];
   griddep_wait();
   griddep_launch_dependents();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t t = __ldg(a.targets);
-  float m = kLowest, s = 0.f;
-  for (int v0 = 2 * (blockIdx.x * 8 + warp); v0 < a.vocab; v0 += 2 * 8 * (int)gridDim.x) {
-    const int v1 = min(v0 + 1, a.vocab - 1);
-    const T* w0 = w + (int64_t)v0 * ldw;
-    const T* w1 = w + (int64_t)v1 * ldw;
-    float p = 0.f, q = 0.f;
-    constexpr int U = 4;  // 16-byte loads of each vocabulary row under way per lane
-    for (int k0 = lane * 8; k0 < hidden; k0 += U * 256) {
-      uint4 u0[U], u1[U];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, t = lane & 3;
+  const int row0 = blockIdx.y * (8 * NT), rows = a.rows - row0;
+  const T* xr = x + (row0 + r) * ldx + 8 * t;
+  const int cc = threadIdx.x % kCols;
+  float m[kPer], s[kPer];
+  int target[kPer];
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int k = k0 + i * 256;
-        const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-        u0[i] = k < hidden ? __ldg(reinterpret_cast<const uint4*>(w0 + k)) : z;
-        u1[i] = k < hidden ? __ldg(reinterpret_cast<const uint4*>(w1 + k)) : z;
-      }
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int k = k0 + i * 256;
-        if (k >= hidden) break;
-        const uint4 c = __ldg(reinterpret_cast<const uint4*>(x + k));
-        const T* t0 = reinterpret_cast<const T*>(&u0[i]);
-        const T* t1 = reinterpret_cast<const T*>(&u1[i]);
-        const T* tx = reinterpret_cast<const T*>(&c);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float y = to_f32<T>(tx[j]);
-          p = fmaf(to_f32<T>(t0[j]), y, p);
-          q = fmaf(to_f32<T>(t1[j]), y, q);
-        }
-      }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      p += __shfl_xor_sync(0xffffffffu, p, o);
-      q += __shfl_xor_sync(0xffffffffu, q, o);
-    }
-    if (lane == 0 && t == v0) *a.target_logit = p;
-    if (lane == 0 && t == v1) *a.target_logit = q;
-    join_pair(m, s, make_float2(p, 1.f));
-    if (v1 != v0) join_pair(m, s, make_float2(q, 1.f));
+  for (int q = 0; q < kPer; ++q) {
+    m[q] = kLowest, s[q] = 0.f;
+    target[q] = ce_target(a.targets, row0 + (threadIdx.x + 256 * q) / kCols, a.rows, a.vocab);
   }
-  if (lane == 0) sh[warp] = make_float2(m, s);
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 8; ++i) join_pair(m, s, sh[i]);
-    a.part[blockIdx.x] = make_float2(m, s);
+  int turn = 0;
+  for (int v0 = blockIdx.x * kCols; v0 < a.vocab; v0 += gridDim.x * kCols) {
+    const int v = v0 + warp / KW * 16 + r;
+    const bool live0 = v < a.vocab, live1 = v + 8 < a.vocab;
+    const T* w0 = w + (int64_t)(live0 ? v : 0) * ldw + 8 * t;
+    const T* w1 = w + (int64_t)(live1 ? v + 8 : 0) * ldw + 8 * t;
+    float c[NT][4] = {};
+    constexpr int U = 4, kStep = KW * 64;  // U 64-wide pieces of the contraction under way per warp
+    for (int k0 = warp % KW * 64; k0 < hidden; k0 += U * kStep) {
+      uint4 u0[U][2], u1[U][2], b[U][2][NT];
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int k = k0 + i * kStep + j * 32;
+          const bool in = k + 8 * t < hidden;
+          const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+          u0[i][j] = in && live0 ? __ldg(reinterpret_cast<const uint4*>(w0 + k)) : z;
+          u1[i][j] = in && live1 ? __ldg(reinterpret_cast<const uint4*>(w1 + k)) : z;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            b[i][j][n] = in && 8 * n + r < rows
+                             ? __ldg(reinterpret_cast<const uint4*>(xr + 8 * n * ldx + k)) : z;
+        }
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint4 y = b[i][j][n];
+            mma_16x8<T>(c[n], u0[i][j].x, u1[i][j].x, u0[i][j].y, u1[i][j].y, y.x, y.y);
+            mma_16x8<T>(c[n], u0[i][j].z, u1[i][j].z, u0[i][j].w, u1[i][j].w, y.z, y.w);
+          }
+    }
+    // The partial sums meet in two places in turn, so that one barrier per step is enough.
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        part[turn][warp][8 * n + 2 * t + (j & 1)][r + 8 * (j >> 1)] = c[n][j];
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+      const int i = threadIdx.x + 256 * q, row = i / kCols;
+      if (i < kOut && row < rows && v0 + cc < a.vocab) {
+        float l = 0.f;
+#pragma unroll
+        for (int k = 0; k < KW; ++k) l += part[turn][cc / 16 * KW + k][row][cc % 16];
+        if (target[q] == v0 + cc) a.target_logit[row0 + row] = l;
+        join_pair(m[q], s[q], make_float2(l, 1.f));
+      }
+    }
+    turn ^= 1;
+  }
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) {
+#pragma unroll
+    for (int o = kCols / 2; o > 0; o >>= 1) {
+      const float2 y = make_float2(__shfl_xor_sync(0xffffffffu, m[q], o),
+                                   __shfl_xor_sync(0xffffffffu, s[q], o));
+      join_pair(m[q], s[q], y);
+    }
+    const int i = threadIdx.x + 256 * q, row = i / kCols;
+    if (i < kOut && row < rows && cc == 0)
+      a.part[(int64_t)blockIdx.x * a.rows + row0 + row] = make_float2(m[q], s[q]);
   }
 }
 
@@ -405,9 +436,23 @@ using namespace sm100;
 // d of one piece; the larger, the fewer passes over the fp32 sums of dx
 constexpr int64_t kPieceBytes = (int64_t)256 << 20;
 
+// Warps per contraction: as few as take it with one batch of loads each, but a row's columns must
+// be lanes of one warp.
+int few_rows_warps(const ssa_linear_ce_t* p) { return p->hidden <= 1024 ? 4 : 8; }
+
+// Up to 8 rows, and as long as all steps of 16 rows take one round of the multiprocessors (two where
+// the contraction is long); 128-row tiles otherwise, with their join. Hidden 2048, vocabulary 65,536
+// (268 MB): 1 to 8 rows 45-46 us (6.2 TB/s without the join) against 56 on tiles, 16 rows would take
+// 58. Hidden 2048, vocabulary 1024: 64 rows 7.4 us against 14.1.
+bool few_rows(const ssa_linear_ce_t* p) {
+  const int64_t steps = (int64_t)cdiv(p->vocab, 128 / few_rows_warps(p)) * cdiv(p->rows, 16);
+  return p->rows <= 8 || steps <= (p->hidden <= 512 ? 2 : 4) * kPlanSms;
+}
+
 struct CePlan {
   GemmForm fwd, bwd;           // tiles of the logits, and of dx and dw
-  int fwd_tiles;               // column tiles of the forward (one row: blocks)
+  bool few;                    // forward without tiles
+  int fwd_tiles;               // column tiles of the forward, or blocks that share the columns
   int64_t ldd;                 // columns of a piece (a multiple of 256)
   int pieces;
   int dx_splits;
@@ -419,9 +464,9 @@ CePlan ce_plan(const ssa_linear_ce_t* p) {
   CePlan q{};
   const int64_t rows = p->rows;
   q.fwd = gemm_form(rows, p->vocab);
-  q.fwd_tiles = rows > 1                            ? cdiv(p->vocab, q.fwd.bn)
-                : cdiv(p->vocab, 16) < kRowBlocks ? cdiv(p->vocab, 16)
-                                                  : kRowBlocks;
+  q.few = few_rows(p);
+  q.fwd_tiles = cdiv(p->vocab, q.few ? 128 / few_rows_warps(p) : q.fwd.bn);
+  if (q.few && q.fwd_tiles > 2 * kPlanSms) q.fwd_tiles = 2 * kPlanSms;
   q.off_target = up256(sizeof(float2) * (size_t)q.fwd_tiles * rows);
   q.off_rows = q.off_target + up256(sizeof(float) * rows);
   q.fwd_bytes = q.off_rows + up256(sizeof(float) * rows);
@@ -484,15 +529,23 @@ int ce_logits(const ssa_linear_ce_t* p, const GemmForm& f, const void* w, int64_
                 : launch_gemm<Epi128, 1, 128, 1, 0, false, BF16>({A, B, g, a}, nullptr, st);
 }
 
-template <bool BF16>
-int ce_row(const ssa_linear_ce_t* p, int blocks, const CeFwdArgs& a, cudaStream_t st) {
-  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-  const cudaError_t e = launch_pdl(ce_row_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st,
-                                   static_cast<const T*>(p->x), static_cast<const T*>(p->w),
-                                   p->w_stride, p->hidden, a);
-  if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "ce_row: %s", cudaGetErrorString(e));
+template <typename T, int NT, int KW>
+int ce_rows(const ssa_linear_ce_t* p, int blocks, const CeFwdArgs& a, cudaStream_t st) {
+  const dim3 grid((unsigned)blocks, (unsigned)cdiv(p->rows, 8 * NT));
+  const cudaError_t e = launch_pdl(ce_rows_kernel<T, NT, KW>, grid, dim3(256), 0, st,
+                                   static_cast<const T*>(p->x), p->x_stride,
+                                   static_cast<const T*>(p->w), p->w_stride, p->hidden, a);
+  if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "ce_rows: %s", cudaGetErrorString(e));
   note_launches(1);
   return SSA_OK;
+}
+
+template <bool BF16>
+int ce_few_rows(const ssa_linear_ce_t* p, int blocks, const CeFwdArgs& a, cudaStream_t st) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  const bool four = few_rows_warps(p) == 4;
+  if (p->rows <= 8) return four ? ce_rows<T, 1, 4>(p, blocks, a, st) : ce_rows<T, 1, 8>(p, blocks, a, st);
+  return four ? ce_rows<T, 2, 4>(p, blocks, a, st) : ce_rows<T, 2, 8>(p, blocks, a, st);
 }
 
 template <bool BF16>
@@ -500,8 +553,8 @@ int ce_fwd(const ssa_linear_ce_t* p, const CePlan& q, float* loss, float* lse, f
            uint8_t* ws, cudaStream_t st) {
   CeFwdArgs a{p->targets, reinterpret_cast<float2*>(ws),
               reinterpret_cast<float*>(ws + q.off_target), p->rows, p->vocab};
-  const int rc = p->rows == 1
-                     ? ce_row<BF16>(p, q.fwd_tiles, a, st)
+  const int rc = q.few
+                     ? ce_few_rows<BF16>(p, q.fwd_tiles, a, st)
                      : ce_logits<EpiCeFwd<256>, EpiCeFwd<128>, BF16>(p, q.fwd, p->w, p->vocab,
                                                                      q.fwd_tiles, a, st);
   if (rc != SSA_OK) return rc;

@@ -86,6 +86,38 @@ def test_loss_and_gradients(cuda_device, dtype, n, h, v):
     _check(x, w, t)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,h,v", [
+    # few rows, or few steps of 16 rows: contractions of one batch of loads and beyond, blocks of one
+    # step and of several
+    (2, 520, 300), (8, 1032, 1000), (9, 64, 33), (16, 1024, 4000), (17, 2056, 700), (60, 264, 500),
+    (300, 512, 16), (5, 64, 20001), (8, 1032, 10007), (16, 1032, 9000),
+    # few rows, more steps than that: tiles
+    (17, 72, 20000), (100, 520, 20001), (9, 2056, 10000)])
+def test_few_rows_and_lone_row_tiles(cuda_device, dtype, n, h, v):
+    _check(*_data(n, h, v, dtype, n + v, 0.2 if n > 2 else 0.0, cuda_device))
+
+
+@pytest.mark.parametrize("n", [3, 8, 11, 40])
+def test_a_row_depends_on_itself_alone(cuda_device, n):
+    """Infinities and NaN in one row reach no other row's loss, and every target of the vocabulary's
+    ends and steps is found."""
+    from SSA.ssa_cross_entropy import ssa_linear_cross_entropy
+    x, w, t = _data(n, 264, 1003, torch.bfloat16, 31, 0.0, cuda_device)
+    ends = torch.tensor([0, 1002, 15, 16, 31, 32, 1000, 991, 7, 8], device=cuda_device)
+    t[:min(n, 10)] = ends[:n]
+    loss = ssa_linear_cross_entropy(x, w, t, reduction="none")
+    logits = x.double() @ w.double().t()
+    want = torch.logsumexp(logits, 1) - logits.gather(1, t[:, None])[:, 0]
+    dl = (264 / 8 + 8) * 2.0 ** -23 * float((x.double().abs() @ w.double().abs().t()).max())
+    assert ((loss.double() - want).abs() <= 2 * dl + 2.0 ** -20 * (want.abs() + 1)).all()
+    bad = x.clone()
+    bad[n // 2, 3], bad[n // 2, 200] = float("inf"), float("nan")
+    got = ssa_linear_cross_entropy(bad, w, t, reduction="none")
+    other = torch.arange(n, device=cuda_device) != n // 2
+    assert torch.equal(got[other], loss[other]) and got[n // 2].isnan()
+
+
 @pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
 def test_reductions_and_leading_shape(cuda_device, reduction):
     from SSA.ssa_cross_entropy import ssa_linear_cross_entropy
