@@ -94,10 +94,20 @@ struct EpiFfnBwd {
                                        : make_uint4(0u, 0u, 0u, 0u);
         }
       } else {
-#pragma unroll 8
-        for (int r = 0; r < 32; ++r)
-          reinterpret_cast<uint16_t*>(exch16(in, r, e.lane >> 3))[e.lane & 7] =
-              r < rows && col + e.lane < a.ffn ? dhbase[(int64_t)r * a.lddh + col + e.lane] : 0;
+        // All of a batch is read before any of it is written: 4096 x 1024, ffn 2815, forward and
+        // backward 272 us element by element, 180 us so, 164 us with aligned rows (ffn 2816).
+#pragma unroll 1
+        for (int r0 = 0; r0 < 32; r0 += 8) {
+          uint16_t y[8];
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            y[r] = r0 + r < rows && col + e.lane < a.ffn
+                       ? __ldg(reinterpret_cast<const unsigned short*>(dhbase) +
+                               (int64_t)(r0 + r) * a.lddh + col + e.lane) : 0;
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            reinterpret_cast<uint16_t*>(exch16(in, r0 + r, e.lane >> 3))[e.lane & 7] = y[r];
+        }
       }
       __syncwarp();
       float g[32], u[32];
