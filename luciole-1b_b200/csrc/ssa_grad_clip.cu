@@ -100,6 +100,18 @@ __global__ void __launch_bounds__(kThreads)
     const uint4* p = reinterpret_cast<const uint4*>(in + base) + threadIdx.x;
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) raw[u] = p[u * kThreads];
+  } else if (e.vec) {  // a tensor's end: one load may reach past it
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int64_t at = base + (int64_t)(u * kThreads + (int)threadIdx.x) * E;
+      raw[u] = at + E <= e.n ? *reinterpret_cast<const uint4*>(in + at) : make_uint4(0u, 0u, 0u, 0u);
+      if (at < e.n && at + E > e.n) {
+        T* t = reinterpret_cast<T*>(&raw[u]);
+#pragma unroll
+        for (int i = 0; i < E - 1; ++i)
+          if (at + i < e.n) t[i] = in[at + i];
+      }
+    }
   } else {
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
@@ -197,9 +209,34 @@ __global__ void __launch_bounds__(kThreads)
       store4(out + base + (u * kThreads + (int)threadIdx.x) * 4, y);
     }
   } else {
+    // The end of a tensor, or one no vector access fits. A batch is read before any of it is written:
+    // in and out may be one, so that the compiler cannot move a read up by itself.
+    constexpr int B = 8;
     const int64_t end = base + kChunkOf<T> < e.n ? base + kChunkOf<T> : e.n;
-    for (int64_t i = base + threadIdx.x; i < end; i += kThreads)
-      out[i] = from_f32<O>(to_f32<T>(in[i]) * c);
+    const int64_t whole = e.vec ? base + (end - base) / 4 * 4 : base;  // in vectors of four up to here
+    for (int64_t i0 = base + 4 * (int)threadIdx.x; i0 < whole; i0 += 4 * B * kThreads) {
+      Four<T> x[B];
+#pragma unroll
+      for (int u = 0; u < B; ++u)
+        if (i0 + 4 * u * kThreads < whole) x[u] = load4(in + i0 + 4 * u * kThreads);
+#pragma unroll
+      for (int u = 0; u < B; ++u) {
+        if (i0 + 4 * u * kThreads >= whole) break;
+        Four<O> y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y.v[i] = from_f32<O>(to_f32<T>(x[u].v[i]) * c);
+        store4(out + i0 + 4 * u * kThreads, y);
+      }
+    }
+    for (int64_t i0 = whole + (int)threadIdx.x; i0 < end; i0 += B * kThreads) {
+      T x[B];
+#pragma unroll
+      for (int u = 0; u < B; ++u)
+        if (i0 + u * kThreads < end) x[u] = in[i0 + u * kThreads];
+#pragma unroll
+      for (int u = 0; u < B; ++u)
+        if (i0 + u * kThreads < end) out[i0 + u * kThreads] = from_f32<O>(to_f32<T>(x[u]) * c);
+    }
   }
 }
 

@@ -111,6 +111,27 @@ def test_layouts(cuda_device):
     _check([flat[1:10001].float()], 0.01, [out[1:]])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("start", [0, 1, 8])
+def test_ends_of_tensors(cuda_device, dtype, start):
+    """Sizes around the vectors, the batches and the 64 KB chunks the kernels walk in, from aligned and
+    unaligned starts; what lies before and behind a tensor stays as it was."""
+    chunk = 65536 // torch.finfo(dtype).bits * 8
+    sizes = [1, 3, 4, 5, 7, 8, 9, 2047, 2049, 4099, chunk - 9, chunk - 8, chunk - 1, chunk + 1,
+             chunk + 8, chunk + 2051, 2 * chunk - 3]
+    flats = _grads([(start + n + 16,) for n in sizes], dtype, cuda_device, seed=start + 1)
+    views = [f[start:start + n] for f, n in zip(flats, sizes)]
+    whole = [f.clone() for f in flats]
+    for o in {torch.float32, dtype}:
+        outs = [torch.full((start + n + 16,), 7.0, dtype=o, device=cuda_device) for n in sizes]
+        _check(views, 0.05, [t[start:start + n] for t, n in zip(outs, sizes)])
+        for t, n in zip(outs, sizes):
+            assert (t[:start] == 7.0).all() and (t[start + n:] == 7.0).all()
+    _check(views, 0.05)
+    for f, w, n in zip(flats, whole, sizes):
+        assert torch.equal(f[:start], w[:start]) and torch.equal(f[start + n:], w[start + n:])
+
+
 def test_repeatable_and_captured(cuda_device):
     from SSA.ssa_grad_clip import ssa_clip_grad_norm
     grads = _grads([(100000,), (3, 7), (511,)], torch.bfloat16, cuda_device)
