@@ -234,7 +234,7 @@ int ssa_grad_norm(const ssa_grad_list_t* list, float* norm, void* workspace, siz
                   void* stream);
 /* The same, then every element times min(1, max_norm / (norm + 1e-6)). Written tensors must not
  * share memory. */
-int ssa_grad_clip(const ssa_grad_list_t* list, float max_norm, float* norm, void* workspace,
+int ssa_grad_clip(const ssa_grad_list_t* list, double max_norm, float* norm, void* workspace,
                   size_t workspace_bytes, void* stream);
 size_t ssa_grad_clip_workspace_size(const ssa_grad_list_t* list);
 

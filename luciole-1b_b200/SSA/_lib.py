@@ -145,7 +145,7 @@ def load() -> ctypes.CDLL:
         lib.ssa_qk_rope_fwd.argtypes = [QK, vp, vp, vp]
         lib.ssa_qk_rope_bwd.argtypes = [QK, T, T, T, vp, vp, vp, vp, sz, vp]
         lib.ssa_grad_norm.argtypes = [GL, vp, vp, sz, vp]
-        lib.ssa_grad_clip.argtypes = [GL, ctypes.c_float, vp, vp, sz, vp]
+        lib.ssa_grad_clip.argtypes = [GL, ctypes.c_double, vp, vp, sz, vp]
         for fn in (lib.ssa_linear_ce_fwd, lib.ssa_linear_ce_bwd, lib.ssa_gated_ffn_fwd,
                    lib.ssa_gated_ffn_bwd, lib.ssa_qk_rope_fwd, lib.ssa_qk_rope_bwd,
                    lib.ssa_grad_norm, lib.ssa_grad_clip):

@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // norm = sqrt of the chunks' sums, coef = min(1, max_norm / (norm + 1e-6)); NaN stays NaN.
-__global__ void __launch_bounds__(1024) norm_kernel(const double* part, int64_t n, float max_norm,
+__global__ void __launch_bounds__(1024) norm_kernel(const double* part, int64_t n, double max_norm,
                                                     float* norm, float* coef) {
   __shared__ double red[32];
   sm100::griddep_wait();
@@ -175,10 +175,11 @@ __global__ void __launch_bounds__(1024) norm_kernel(const double* part, int64_t 
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
   if (threadIdx.x == 0) {
-    const float r = (float)sqrt(d);
+    const double root = sqrt(d);
+    const float r = (float)root;
     *norm = r;
-    if (coef) {
-      const float c = max_norm / (r + 1e-6f);
+    if (coef) {  // rounded once; a norm that fp32 shows as infinite gives 0 (and infinity over it NaN)
+      const float c = (float)(max_norm / (isinf(r) ? (double)r : root + 1e-6));
       *coef = c > 1.f ? 1.f : c;
     }
   }
@@ -386,7 +387,7 @@ int first_tensor(const ssa_grad_list_t* l) {
   return -1;
 }
 
-int norm_into(const ssa_grad_list_t* l, double* part, float max_norm, float* norm, float* coef,
+int norm_into(const ssa_grad_list_t* l, double* part, double max_norm, float* norm, float* coef,
               cudaStream_t st) {
   int rc = walk_types<false>(l, part, nullptr, st);
   if (rc != SSA_OK) return rc;
@@ -425,13 +426,13 @@ int ssa_grad_norm(const ssa_grad_list_t* list, float* norm, void* workspace, siz
                    norm, nullptr, static_cast<cudaStream_t>(stream));
 }
 
-int ssa_grad_clip(const ssa_grad_list_t* list, float max_norm, float* norm, void* workspace,
+int ssa_grad_clip(const ssa_grad_list_t* list, double max_norm, float* norm, void* workspace,
                   size_t workspace_bytes, void* stream) {
   abi_clear_error();
   int rc = list_check(list, true);
   if (rc != SSA_OK) return rc;
   if (!norm) return abi_error(SSA_ERR_NULL, "grad_clip: norm is NULL");
-  if (!(max_norm >= 0.f))
+  if (!(max_norm >= 0.0))
     return abi_error(SSA_ERR_BAD_SHAPE, "grad_clip: max_norm must not be negative or NaN");
   const size_t need = 256 + sizeof(double) * (size_t)(total_chunks(list) + 1);
   if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256)

@@ -71,6 +71,18 @@ def test_matches_torch(cuda_device):
         assert torch.allclose(p.grad, m, rtol=2e-5, atol=0)
 
 
+def test_the_factor_is_rounded_once(cuda_device):
+    """max_norm and the norm's root stay in 64 bits up to the factor: all elements carry its one
+    rounding, 2^-24 at most, and the norm's squares here are exact (a power of two times integers)."""
+    from SSA.ssa_grad_clip import ssa_clip_grad_norm
+    g = torch.full((4096,), 0.5, device=cuda_device)  # norm 32
+    for max_norm in (0.1, 0.3, 1.7, 3.3, 1 / 3, 31.9):
+        out = torch.empty_like(g)
+        assert float(ssa_clip_grad_norm([g], max_norm, out=[out])) == 32.0
+        want = max_norm / (32.0 + 1e-6)
+        assert abs(float(out[0]) / 0.5 - want) <= 2.0 ** -24 * want and (out == out[0]).all()
+
+
 def test_range_of_squares(cuda_device):
     """Squares that overflow or underflow fp32."""
     from SSA.ssa_grad_clip import ssa_grad_norm
