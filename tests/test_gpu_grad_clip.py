@@ -1,7 +1,7 @@
 """Global gradient norm and clipping (SSA.ssa_grad_clip) against the same sums in 64 bits.
 
-Bounds. A thread adds 32 squares in fp32 (33 steps of 2^-24), everything above that in fp64, and the
-norm is rounded once: 20 steps of 2^-24 relative after the square root. An element is multiplied in
+Bounds. A thread adds at most 32 squares in fp32 (33 steps of 2^-24), everything above that in fp64,
+and the norm is rounded once: 20 steps of 2^-24 relative after the square root. An element is multiplied in
 fp32 by a coefficient off by that and three more roundings, and rounded once to its type."""
 
 import math
