@@ -8,9 +8,9 @@
 // per launch. Work is cut into chunks of 64 KB, one block each; the second pass walks the
 // chunks from the last to the first, so that what the first pass read last is still in L2.
 //
-// Squares are added in fp32 over a thread's few elements of a chunk and in fp64 from there on, in
-// a fixed order: the norm is the same from run to run. A thread whose fp32 sum overflowed, or is so
-// small that squares may have been lost, adds its elements again in fp64.
+// Squares are added in fp32 over the elements of a 16-byte load and in fp64 from there on, in a fixed
+// order: the norm is the same from run to run. A thread whose sum overflowed, or is so small that
+// squares may have been lost, adds its elements again in fp64.
 #include <algorithm>
 #include <cmath>
 #include <exception>
