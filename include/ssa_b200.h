@@ -142,8 +142,8 @@ int ssa_attn_bwd_noalloc(const ssa_problem_t* prob,
 
 /* Linear cross entropy: loss of the logits x W^T against targets, without keeping the logits.
  * x [rows, hidden] and w [vocab, hidden] are fp16 or bf16 with unit column stride and 16-byte
- * aligned rows; hidden is a multiple of 8. targets: int64, a row whose target equals ignore_index
- * has loss 0 and no gradient, and one outside [0, vocab) gives NaN. */
+ * aligned rows; hidden is a multiple of 8; no size exceeds 2^24. targets: int64, a row whose target
+ * equals ignore_index has loss 0 and no gradient, and one outside [0, vocab) gives NaN. */
 typedef struct {
   int32_t dtype; /* ssa_dtype_t */
   int32_t rows, hidden, vocab;

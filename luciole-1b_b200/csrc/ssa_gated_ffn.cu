@@ -287,8 +287,8 @@ int ffn_check(const ssa_gated_ffn_t* p) {
                      p->rows, p->hidden, p->ffn);
   if (p->hidden % 8)
     return abi_error(SSA_ERR_BAD_SHAPE, "gated_ffn: hidden=%d must be a multiple of 8", p->hidden);
-  if (p->rows > (1 << 24) || p->ffn > (1 << 24))
-    return abi_error(SSA_ERR_BAD_SHAPE, "gated_ffn: rows and ffn must not exceed 2^24");
+  if (p->rows > (1 << 24) || p->hidden > (1 << 24) || p->ffn > (1 << 24))
+    return abi_error(SSA_ERR_BAD_SHAPE, "gated_ffn: rows, hidden and ffn must not exceed 2^24");
   if (!p->x || !p->w) return abi_error(SSA_ERR_NULL, "gated_ffn: x or w is NULL");
   if (((uintptr_t)p->x | (uintptr_t)p->w) % 16 || p->x_stride % 8 || p->w_stride % 8 ||
       p->x_stride < p->hidden || p->w_stride < p->hidden)

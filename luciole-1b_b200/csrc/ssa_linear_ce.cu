@@ -503,8 +503,8 @@ int ce_check(const ssa_linear_ce_t* p) {
                      p->rows, p->hidden, p->vocab);
   if (p->hidden % 8)
     return abi_error(SSA_ERR_BAD_SHAPE, "linear_ce: hidden=%d must be a multiple of 8", p->hidden);
-  if (p->rows > (1 << 24) || p->vocab > (1 << 24))
-    return abi_error(SSA_ERR_BAD_SHAPE, "linear_ce: rows and vocab must not exceed 2^24");
+  if (p->rows > (1 << 24) || p->hidden > (1 << 24) || p->vocab > (1 << 24))
+    return abi_error(SSA_ERR_BAD_SHAPE, "linear_ce: rows, hidden and vocab must not exceed 2^24");
   if (p->reduction < 0 || p->reduction > 2)
     return abi_error(SSA_ERR_UNSUPPORTED, "linear_ce: reduction %d (0 none, 1 mean, 2 sum)",
                      p->reduction);

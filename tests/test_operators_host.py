@@ -68,6 +68,19 @@ def test_linear_ce_arguments(lib):
     assert lib.ssa_linear_ce_bwd_workspace_size(ctypes.byref(big)) < 2 * 65536 * 131072 // 10
 
 
+def test_sizes_beyond_2_to_the_24(lib):
+    from SSA import _lib
+    big = (1 << 24) + 8
+    for kw in (dict(rows=big), dict(hidden=big, x_stride=big, w_stride=big), dict(vocab=big)):
+        p = ctypes.byref(_ce(**kw))
+        assert lib.ssa_linear_ce_fwd(p, 256, 256, 256, 256, 1 << 40, None) == _lib.SSA_ERR_BAD_SHAPE
+        assert lib.ssa_linear_ce_bwd_workspace_size(p) == 0
+    for kw in (dict(rows=big), dict(hidden=big, x_stride=big, w_stride=big), dict(ffn=big)):
+        p = ctypes.byref(_ffn(**kw))
+        assert lib.ssa_gated_ffn_fwd(p, 256, 1 << 30, None) == _lib.SSA_ERR_BAD_SHAPE
+        assert lib.ssa_gated_ffn_bwd_workspace_size(p) == 0
+
+
 def test_gated_ffn_arguments(lib):
     from SSA import _lib
     for kw, code in ((dict(dtype=0), _lib.SSA_ERR_UNSUPPORTED), (dict(ffn=0), _lib.SSA_ERR_BAD_SHAPE),
