@@ -11,7 +11,6 @@ the call a user makes of the framework's kernel.
                fp32 buffer (or, with "norm_only", the norm alone)
 """
 
-import functools
 import math
 import random
 import sys
@@ -25,7 +24,6 @@ _DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 _EPS = 1e-5
 
 
-@functools.lru_cache(maxsize=None)
 def _framework():
     root = str(Path(__file__).resolve().parent.parent / "luciole-1b_b200")
     if root not in sys.path:
