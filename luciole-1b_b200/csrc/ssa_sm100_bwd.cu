@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(512, 1)
       }
     };
     // delta comes from the preprocess kernel, which may still be running (programmatic launch);
-    // the K / V loads above do not depend on it.
+    // the K / V loads above do not depend on it, and what came before it has completed.
     griddep_wait();
     fetch_stats(0);
     for (int t = 0; t < T; ++t) {
@@ -786,10 +786,12 @@ __global__ void __launch_bounds__(256) bwd_preprocess_sm100_kernel(Problem p, Te
                                                                    int sem_per_zh, T* dom,
                                                                    const float* lse,
                                                                    float* lse_shifted) {
-  griddep_launch_dependents();  // the backward's setup may overlap this pass
-  // Launched programmatically behind the forward (which wrote `o`): nothing global is touched
-  // before that grid has completed.
+  // Launched programmatically: nothing global is touched before the kernel ahead has completed.
+  // Only then may the backward start to overlap this pass: before its own wait, which is for this
+  // grid, it reads K and V, which the kernel ahead may have written, and writes parts of its
+  // workspace that the kernel ahead may have read.
   griddep_wait();
+  griddep_launch_dependents();
   if (sem && blockIdx.x == 0) {
     const int nz = p.cu_seqlens ? p.B : 1;  // packed: grid row = q-head, every document
     for (int zz = 0; zz < nz; ++zz) {
