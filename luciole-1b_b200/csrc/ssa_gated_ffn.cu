@@ -35,21 +35,24 @@ struct EpiFfnFwd {
                                               const EpiCtx& e) {
     const int off = e.half * (BN / 4);  // a warp's gate columns; the up projection's are BN / 2 on
     uint16_t* base = reinterpret_cast<uint16_t*>(a.h) + (int64_t)e.row0 * a.ldh;
+    // Only columns that exist are fetched: every read of TMEM is waited for before the tile is handed
+    // back to the MMAs.
+    const int col0 = w.nt * (BN / 2) + off, n = min(BN / 4, a.ffn - col0);
+    if (n <= 0) return;
     uint32_t xg[32], xu[32];
     e.fetch(off, xg);
     e.fetch(BN / 2 + off, xu);
 #pragma unroll 1
-    for (int c = 0; c < BN / 4; c += 32) {
-      const int col = w.nt * (BN / 2) + off + c;
+    for (int c = 0; c < n; c += 32) {
+      const int col = col0 + c;
       float g[32], u[32];
       e.settle();
       e.values(xg, g);
       e.values(xu, u);
-      if (c + 32 < BN / 4) {
+      if (c + 32 < n) {
         e.fetch(off + c + 32, xg);
         e.fetch(BN / 2 + off + c + 32, xu);
       }
-      if (col >= a.ffn) break;
 #pragma unroll
       for (int i = 0; i < 32; ++i) g[i] = g[i] * sigmoid_approx(g[i]) * u[i];
       store_block16<BF16>(e, g, base, a.ldh, a.rows - e.row0, col, a.ffn, a.vec);
