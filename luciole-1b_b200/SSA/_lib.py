@@ -13,6 +13,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 _PKG_ROOT = Path(__file__).resolve().parent.parent
@@ -210,6 +211,21 @@ def table(t: torch.Tensor) -> torch.Tensor:
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
+def has_tangent(tensors) -> bool:
+    """Whether one of the tensors (or None) carries a forward-mode tangent. requires_grad does not show
+    it, and the kernels read the primal alone."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no dual level is open
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def differentiated(*tensors) -> bool:
+    """Whether a call on these tensors (or None) is autograd's business: a gradient is asked for, or
+    there is a tangent, which the operators' Functions refuse (they have no jvp)."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) \
+        or has_tangent(tensors)
+
+
 def first_order(backward):
     """A Function's backward that runs kernels autograd cannot see through: differentiating it again
     raises (torch's once_differentiable, whose wrapper is entered only where a graph of the
@@ -217,6 +233,8 @@ def first_order(backward):
     guarded = once_differentiable(backward)
 
     def run(ctx, *grads):
+        if has_tangent(grads):
+            raise NotImplementedError("gradients that carry forward-mode tangents are not followed")
         return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
     return run
 

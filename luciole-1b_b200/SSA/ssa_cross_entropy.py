@@ -118,6 +118,6 @@ def ssa_linear_cross_entropy(hidden, weight, targets, ignore_index=-100, reducti
         raise ValueError(f"targets must be int64 or int32, got {targets.dtype}")
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+    if _lib.differentiated(hidden, weight):
         return SSALinearCrossEntropyFunc.apply(hidden, weight, targets, int(ignore_index), reduction)
     return _forward(hidden, weight, targets, int(ignore_index), _REDUCTIONS[reduction])[0]

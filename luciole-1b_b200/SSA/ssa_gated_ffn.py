@@ -97,6 +97,6 @@ def ssa_gated_ffn(x, weight_gate_up):
                          f"{tuple(x.shape)}")
     if x.shape[-1] < 8 or x.shape[-1] % 8:
         raise ValueError(f"hidden size {x.shape[-1]} must be a positive multiple of 8")
-    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+    if _lib.differentiated(x, w):
         return SSAGatedFFNFunc.apply(x, w)
     return _forward(x, w)[0]

@@ -34,6 +34,8 @@ def _check_list(ts, what, device=None):
         raise ValueError(f"{what} must be CUDA tensors (there is no CPU path)")
     if ts and ts[0].dtype not in _lib.DTYPE_CODES:
         raise ValueError(f"{what} must be fp32, fp16 or bf16, got {ts[0].dtype}")
+    if _lib.has_tangent(ts):
+        raise NotImplementedError(f"{what} carry forward-mode tangents, which are not followed")
     return ts
 
 

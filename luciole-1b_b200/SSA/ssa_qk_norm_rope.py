@@ -154,8 +154,7 @@ def ssa_qk_norm_rope(qkv, num_heads, num_kv_heads, cos, sin, q_weight=None, k_we
             raise ValueError(f"positions {tuple(positions.shape)} do not fit rows {tuple(lead)}")
         if cos.shape[0] < 1:
             raise ValueError("empty cos / sin tables")
-    if torch.is_grad_enabled() and (qkv.requires_grad or (
-            q_weight is not None and (q_weight.requires_grad or k_weight.requires_grad))):
+    if _lib.differentiated(qkv, q_weight, k_weight) or _lib.has_tangent((cos, sin)):
         return SSAQKNormRopeFunc.apply(qkv, q_weight, k_weight, cos, sin, positions, hq, hkv,
                                        float(eps))
     return _forward(qkv, q_weight, k_weight, cos, sin, positions, hq, hkv, float(eps))[0]
