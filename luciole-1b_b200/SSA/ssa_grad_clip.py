@@ -75,8 +75,14 @@ def _contiguous(grads):
 def ssa_grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
     """The 2-norm over all elements of a list of tensors (fp32, fp16 or bf16, one dtype, one CUDA
     device), as an fp32 scalar on their device. Squares are summed in 64 bits in a fixed order;
-    infinities and NaN in a gradient come through. An empty list gives 0 on the current device."""
+    infinities and NaN in a gradient come through. An empty list gives 0 on the current device.
+
+    The norm takes no part in autograd: gradients that have a graph of their own (create_graph=True) are
+    refused unless detached or under torch.no_grad()."""
     grads = _check_list(grads, "grads")
+    if torch.is_grad_enabled() and any([t.grad_fn is not None for t in grads]):
+        raise ValueError("the norm is not differentiable: detach gradients made with create_graph, or "
+                         "call it under torch.no_grad()")
     return _run(grads, _contiguous(grads)) if grads else torch.zeros((), device="cuda")
 
 
@@ -88,7 +94,8 @@ def ssa_clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float,
     Every element is multiplied by ``min(1, max_norm / (norm + 1e-6))`` in fp32 and rounded once: in
     place, or, with ``out``, into contiguous tensors of the same sizes that are fp32 or of the
     gradients' dtype (``grads`` then stay as they are). As with torch's clipping, a NaN norm makes
-    every gradient NaN and an infinite one makes the finite ones 0. grads: one dtype (fp32, fp16,
+    every gradient NaN and an infinite one makes the finite ones 0, and autograd does not record the
+    scaling: the norm and ``out`` are without a graph. grads: one dtype (fp32, fp16,
     bf16), one CUDA device; tensors that are written must not share memory, with one another or
     with gradients that are read."""
     grads = _check_list(grads, "grads")

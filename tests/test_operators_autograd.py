@@ -67,3 +67,16 @@ def test_tangents_of_incoming_gradients_are_refused(fake, monkeypatch, name):
             grads[i] = fwAD.make_dual(grads[i], torch.ones_like(grads[i]))
             with pytest.raises(NotImplementedError):
                 fn.backward(None, *grads)  # before anything of the context is read
+
+
+def test_the_norm_refuses_gradients_with_a_graph(fake, monkeypatch):
+    from SSA import ssa_grad_clip
+    monkeypatch.setattr(ssa_grad_clip, "_run", lambda *a, **k: fake(dtype=torch.float32))
+    leaf = fake(4, 64).requires_grad_(True)
+    made = leaf * 2  # as torch.autograd.grad(..., create_graph=True) returns them
+    with pytest.raises(ValueError, match="create_graph"):
+        ssa_grad_clip.ssa_grad_norm([fake(3), made])
+    ssa_grad_clip.ssa_grad_norm([fake(3), made.detach()])
+    with torch.no_grad():
+        ssa_grad_clip.ssa_grad_norm([fake(3), made])
+    ssa_grad_clip.ssa_grad_norm([leaf])
