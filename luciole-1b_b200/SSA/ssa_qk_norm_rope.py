@@ -111,7 +111,8 @@ def ssa_qk_norm_rope(qkv, num_heads, num_kv_heads, cos, sin, q_weight=None, k_we
     (or ``n = x`` without weights), in fp32 with one rounding.
 
     qkv: [B, S, (Hq + 2 Hkv) D] or packed [T, (Hq + 2 Hkv) D], fp32, fp16 or bf16 on CUDA, queries'
-    heads first, then keys', then values'; D 16, 32, 64 or 128. cos, sin: fp32 [P, D] (``rope_tables``).
+    heads first, then keys', then values'; D 16, 32, 64 or 128. cos, sin: fp32 [P, D] (``rope_tables``), which
+    get no gradient.
     q_weight, k_weight: [D], both or neither, fp32 or of qkv's dtype. positions: None (row s of a
     sequence has position s), or int32 / int64 of shape [S], [B, S] or [T], an index into the tables;
     one outside them gives NaN (nothing is read out of range). Returns q [..., Hq, D], k [..., Hkv, D]
@@ -131,6 +132,8 @@ def ssa_qk_norm_rope(qkv, num_heads, num_kv_heads, cos, sin, q_weight=None, k_we
     if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 \
             or sin.dtype != torch.float32:
         raise ValueError("cos and sin must be fp32 [P, D] tables of one shape")
+    if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
+        raise ValueError("cos and sin are tables without a gradient: detach them")
     d = cos.shape[1]
     if d not in (16, 32, 64, 128):
         raise ValueError(f"head dim D={d} not supported (16, 32, 64, 128)")

@@ -80,3 +80,14 @@ def test_the_norm_refuses_gradients_with_a_graph(fake, monkeypatch):
     with torch.no_grad():
         ssa_grad_clip.ssa_grad_norm([fake(3), made])
     ssa_grad_clip.ssa_grad_norm([leaf])
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_rotation_tables_with_a_gradient_are_refused(fake, monkeypatch, which):
+    call, inputs = _calls(fake, monkeypatch)["tables"]
+    args = [fake(*s, dtype=d) for s, d in inputs]
+    args[which].requires_grad_(True)
+    with pytest.raises(ValueError, match="without a gradient"):
+        call(*args)
+    with torch.no_grad():
+        call(*args)
