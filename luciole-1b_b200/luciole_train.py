@@ -233,14 +233,19 @@ def train_step(model: nn.Module, opt: MasterWeightAdamW, tokens: torch.Tensor,
                targets: torch.Tensor, max_grad_norm: Optional[float] = None) -> torch.Tensor:
     """One optimizer step on one micro-batch: forward, loss, backward (DDP all-reduces the
     gradients when `model` is wrapped), AdamW on the fp32 masters, with max_grad_norm on gradients
-    clipped to that global norm. Returns the loss (device)."""
-    if getattr(model, "module", model).cfg.fused:
+    clipped to that global norm. Returns the loss (device). `model` may be any module that maps
+    tokens to logits; a LucioleDecoder with cfg.fused returns the loss itself."""
+    cfg = getattr(getattr(model, "module", model), "cfg", None)
+    if isinstance(cfg, LucioleConfig) and cfg.fused:
         loss = model(tokens, targets)
     else:
         logits = model(tokens)
         loss = F.cross_entropy(logits.float().view(-1, logits.shape[-1]), targets.reshape(-1))
     loss.backward()
-    opt.step(max_grad_norm)
+    if max_grad_norm is None:
+        opt.step()
+    else:
+        opt.step(max_grad_norm)
     opt.zero_grad()
     return loss.detach()
 
