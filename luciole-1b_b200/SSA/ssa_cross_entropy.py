@@ -2,8 +2,11 @@
 
 ``ssa_linear_cross_entropy(hidden, weight, targets)`` is
 ``cross_entropy(hidden @ weight.T, targets)``: the logits stay on the chip in fp32, the backward
-forms them again per piece of the vocabulary, and neither pass holds a [tokens, vocab] matrix (the
-backward's workspace is one 16-bit piece of at most about 256 MiB).
+forms them again per piece of the vocabulary, and neither pass holds a [tokens, vocab] matrix.
+
+The backward's workspace: one 16-bit piece of the logits' gradient (with reduction "none" two), up to
+256 MiB or 1024 columns, whichever is more; a 16-bit copy of the hidden states; and where there are
+several pieces, or dx's contraction is split, their fp32 gradient once per split.
 """
 
 from __future__ import annotations

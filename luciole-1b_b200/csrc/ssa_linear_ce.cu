@@ -6,8 +6,9 @@
 // Forward: one tensor-core product whose epilogue reduces each row of a tile to a running maximum
 // and sum of exponentials (and picks the target's logit); a second kernel joins the tiles' pairs.
 // Backward: the vocabulary is walked in pieces that fit the workspace. Per piece the logits are
-// formed again and leave as d in 16 bits, then two products read that piece: dx is summed over the
-// pieces in fp32, dW's rows of the piece are final. Bound: the tensor cores, 8 rows hidden vocab
+// formed again and leave as d in 16 bits (the products' operands; the rounding, with that of the
+// result, puts both gradients 0.02% off in fp16 and 0.17% in bf16, as the inputs' type allows), then
+// two products read that piece: dx is summed over the pieces in fp32, dW's rows of the piece are final. Bound: the tensor cores, 8 rows hidden vocab
 // operations for forward and backward against the 6 that a kept logit matrix would need.
 #include <cmath>
 
@@ -290,33 +291,27 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// A gradient as +- 2^e times the rest in [0.5, 1); one that is 0 or not finite is its own factor.
-__device__ __forceinline__ float split_power(float g, float& rest) {
-  rest = 1.f;
-  if (g == 0.f || !(fabsf(g) < INFINITY)) return g;
-  int e;
-  rest = fabsf(frexpf(g, &e));
-  return copysignf(ldexpf(1.f, min(e, 127)), g) * (e > 127 ? 2.f : 1.f);
-}
-
 // What the backward multiplies (p - [v = t]) by before it is rounded to 16 bits: a power of two, so that
 // the target's p - 1, which weighs most, is rounded as a number just below a power of two and not
 // times an arbitrary factor that would put one error, up to 2^-8 in bf16, on a whole row (0.4% of the
-// gradients of 8192 rows before). The rest of each gradient enters elsewhere:
-//   one for all rows (mean, sum): the power is 2^14, `inv` = grad / count 2^-14 in the epilogues;
-//   one per row: grad_r = +- 2^e rest_r. The powers are brought to at most 2^14 by another that `inv`
-//   undoes; rest_r multiplies row r of dx in its epilogue, and row r of the copy of x for dW.
-// 2^14 keeps the small probabilities of a large vocabulary normal numbers in fp16. Ignored rows: 0.
+// gradients of 8192 rows before). The power is 2^14, which keeps the small probabilities of a large
+// vocabulary normal numbers in fp16; ignored rows and gradients of 0 have 0. The gradients enter in fp32:
+//   one for all rows (mean, sum): grad / count 2^-14 in both products' epilogues (inv);
+//   one per row: dx_r = grad_r 2^-14 (d W)_r, in the epilogue, so that a row's gradient depends on its
+//   own factor alone. dW sums over rows, so there d has to carry the factors: a second matrix, d times
+//   grad_r / top (top: the largest), rounded once, with top 2^-14 in the epilogue. Equal gradients,
+//   as of a sum or a mean taken outside, give the factor 1. (One matrix for both products, with the
+//   powers of two of grad_r in d and the rest rounded into x: 3-5% faster at 4096 and 8192 rows, dW's
+//   terms rounded twice, and in fp16 the small probabilities of a row lost once another row's
+//   gradient was 10^5 times as large.)
 //
-// Blocks after the first make that copy of x, with ignored rows as zeros, for the product that sums over
-// rows: what an ignored row holds (padding, an infinity) must not reach dW as 0 times it.
-template <bool BF16>
+// Blocks after the first copy x, with ignored rows as zeros, for the product that sums over rows: what
+// an ignored row holds (padding, an infinity) must not reach dW as 0 times it.
 __global__ void __launch_bounds__(1024)
     ce_row_weights_kernel(const float* grad, int per_row, const int64_t* targets,
                           int64_t ignore_index, int rows, int vocab, const float* count, int mean,
-                          float* weight, float* rest, float* inv, const uint16_t* x, int64_t ldx,
-                          int hidden, uint16_t* x_kept) {
-  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+                          float* weight, float* scale_x, float* factor, float* inv, const uint16_t* x,
+                          int64_t ldx, int hidden, uint16_t* x_kept) {
   __shared__ float red[32];
   griddep_wait();
   griddep_launch_dependents();
@@ -325,22 +320,15 @@ __global__ void __launch_bounds__(1024)
     const int64_t total = (int64_t)rows * chunks, step = (int64_t)(gridDim.x - 1) * 1024;
     for (int64_t i = (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x; i < total; i += step) {
       const int row = (int)(i / chunks), c = (int)(i - (int64_t)row * chunks);
-      uint4 v = __ldg(reinterpret_cast<const uint4*>(x + (int64_t)row * ldx) + c);
-      if (per_row) {
-        float r;
-        split_power(__ldg(grad + row), r);
-        T* t = reinterpret_cast<T*>(&v);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) t[k] = from_f32<T>(to_f32<T>(t[k]) * r);
-      }
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(x + (int64_t)row * ldx) + c);
       reinterpret_cast<uint4*>(x_kept)[i] =
           __ldg(targets + row) == ignore_index ? make_uint4(0u, 0u, 0u, 0u) : v;
     }
     return;
   }
-  float up = 16384.f;
+  constexpr float kUp = 16384.f, kDown = 1.f / 16384.f;
+  float top = 0.f;
   if (per_row) {
-    float top = 0.f;
     for (int i = threadIdx.x; i < rows; i += 1024)
       if (targets[i] != ignore_index) top = fmaxf(top, fabsf(grad[i]));
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -348,13 +336,11 @@ __global__ void __launch_bounds__(1024)
     __syncthreads();
     top = red[threadIdx.x & 31];
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    int e = 0;
-    if (top > 0.f && top < INFINITY) e = max(-126, min(126, 13 - ilogbf(top)));
-    up = ldexpf(1.f, e);
-    if (threadIdx.x == 0) *inv = ldexpf(1.f, -e);
+    if (!(top > 0.f && top < INFINITY)) top = 1.f;
+    if (threadIdx.x == 0) inv[0] = kDown, inv[1] = top * kDown;
   } else if (threadIdx.x == 0) {
     const float n = mean ? *count : 1.f;  // no row counts: nothing to divide, gradients of 0
-    *inv = n > 0.f ? grad[0] / n * (1.f / 16384.f) : 0.f;
+    inv[0] = inv[1] = n > 0.f ? grad[0] / n * kDown : 0.f;
   }
   for (int i = threadIdx.x; i < rows; i += 4096) {
     int64_t t[4];
@@ -364,12 +350,10 @@ __global__ void __launch_bounds__(1024)
     for (int k = 0; k < 4; ++k) {
       const int at = i + 1024 * k;
       if (at >= rows) break;
-      float g = up, r = 1.f;
-      if (per_row) g = split_power(grad[at], r) * up;
-      if (per_row) rest[at] = r;
-      if (t[k] == ignore_index) g = 0.f;
-      else if (t[k] < 0 || t[k] >= vocab) g = nan_f32();
-      weight[at] = g;
+      const bool skip = t[k] == ignore_index;
+      const float g = skip ? 0.f : per_row ? grad[at] : 1.f;
+      weight[at] = !skip && (t[k] < 0 || t[k] >= vocab) ? nan_f32() : g == 0.f ? 0.f : kUp;
+      if (per_row) scale_x[at] = g, factor[at] = g / top;
     }
   }
 }
@@ -378,27 +362,29 @@ struct CeBwdArgs {
   const int64_t* targets;
   const float* lse;
   const float* weight;
+  const float* factor;  // one gradient per row: what d2 has above d
   void* d;         // 16-bit [rows][ldd], this piece's columns; columns past the vocabulary are 0
+  void* d2;        // one gradient per row: d for dW; either may be nullptr
   int64_t ldd;
   int rows, piece0, vocab;
 };
 
-template <int BN, bool BF16>
+template <int BN, bool BF16, bool PER_ROW>
 struct EpiCeBwd {
   using Args = CeBwdArgs;
   struct Row {
-    float g, b;
+    float g, b, f;
     int t;
   };
   __device__ static __forceinline__ Row row(const Args& a, int row) {
     const bool ok = row < a.rows;
     return Row{ok ? __ldg(a.weight + row) : 0.f, ok ? -__ldg(a.lse + row) * kLog2e : 0.f,
-               ce_target(a.targets, row, a.rows, a.vocab)};
+               PER_ROW && ok ? __ldg(a.factor + row) : 0.f, ce_target(a.targets, row, a.rows, a.vocab)};
   }
   __device__ static __forceinline__ void tile(const Args& a, const GemmUnit& w, const Row& rw,
                                               const EpiCtx& e) {
     const int off = e.half * (BN / 2);
-    uint16_t* base = reinterpret_cast<uint16_t*>(a.d) + (int64_t)e.row0 * a.ldd + w.nt * BN + off;
+    const int64_t first = (int64_t)e.row0 * a.ldd + w.nt * BN + off;
     const float g = rw.g, b = rw.b;
     const uint32_t mask = g == 0.f ? 0u : 0xffffffffu;  // an ignored row adds nothing, whatever it holds
     uint32_t x[32];
@@ -422,7 +408,15 @@ struct EpiCeBwd {
         for (int i = 0; i < 32; ++i)
           if (col + i >= a.vocab) v[i] = 0.f;
       }
-      store_block16<BF16>(e, v, base, a.ldd, a.rows - e.row0, c, BN / 2, true, mask);
+      if (!PER_ROW || a.d)
+        store_block16<BF16>(e, v, reinterpret_cast<uint16_t*>(a.d) + first, a.ldd, a.rows - e.row0, c,
+                            BN / 2, true, mask);
+      if (PER_ROW && a.d2) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] *= rw.f;
+        store_block16<BF16>(e, v, reinterpret_cast<uint16_t*>(a.d2) + first, a.ldd, a.rows - e.row0, c,
+                            BN / 2, true, mask);
+      }
     }
   }
 };
@@ -433,7 +427,7 @@ namespace {
 
 using namespace sm100;
 
-// d of one piece; the larger, the fewer passes over the fp32 sums of dx
+// d of one piece (each of two matrices with one gradient per row); the larger, the fewer passes over the fp32 sums of dx
 constexpr int64_t kPieceBytes = (int64_t)256 << 20;
 
 // Warps per contraction: as few as take it with one batch of loads each, but a row's columns must
@@ -457,7 +451,7 @@ struct CePlan {
   int pieces;
   int dx_splits;
   size_t off_target, off_rows, fwd_bytes;
-  size_t off_rest, off_inv, off_x, off_d, off_sum, bwd_bytes;
+  size_t off_scale, off_factor, off_inv, off_x, off_d, off_d2, off_sum, bwd_bytes;
 };
 
 CePlan ce_plan(const ssa_linear_ce_t* p) {
@@ -471,6 +465,7 @@ CePlan ce_plan(const ssa_linear_ce_t* p) {
   q.off_rows = q.off_target + up256(sizeof(float) * rows);
   q.fwd_bytes = q.off_rows + up256(sizeof(float) * rows);
 
+  const int matrices = p->reduction ? 1 : 2;  // one gradient per row: d for dx and d for dW
   int64_t cols = kPieceBytes / (2 * rows) / 256 * 256;
   if (cols < 1024) cols = 1024;
   const int64_t all = (int64_t)cdiv(p->vocab, 256) * 256;
@@ -483,11 +478,13 @@ CePlan ce_plan(const ssa_linear_ce_t* p) {
   const int64_t dw_tiles = (int64_t)cdiv(q.ldd, q.bwd.bm) * cdiv(p->hidden, q.bwd.bn);
   q.dx_splits = split_count(dx_tiles, (int)(q.ldd / 64), dw_tiles * (cdiv(rows, 64) + kTileCost),
                             q.bwd.workers);
-  q.off_rest = up256(sizeof(float) * rows);
-  q.off_inv = 2 * q.off_rest;
+  q.off_scale = up256(sizeof(float) * rows);
+  q.off_factor = 2 * q.off_scale;
+  q.off_inv = 3 * q.off_scale;
   q.off_x = q.off_inv + 256;
   q.off_d = q.off_x + up256(2 * (size_t)rows * p->hidden);
-  q.off_sum = q.off_d + up256(2 * (size_t)rows * q.ldd);
+  q.off_d2 = q.off_d + up256(2 * (size_t)rows * q.ldd);
+  q.off_sum = matrices == 1 ? q.off_d2 : 2 * q.off_d2 - q.off_d;
   q.bwd_bytes = q.off_sum;
   if (q.pieces > 1 || q.dx_splits > 1)
     q.bwd_bytes += up256(sizeof(float) * (size_t)q.dx_splits * rows * p->hidden);
@@ -577,19 +574,21 @@ template <bool BF16>
 int ce_bwd(const ssa_linear_ce_t* p, const CePlan& q, const float* lse, const float* count,
            const float* grad, void* dx, void* dw, uint8_t* ws, cudaStream_t st) {
   float* weight = reinterpret_cast<float*>(ws);
-  float* rest = reinterpret_cast<float*>(ws + q.off_rest);
+  float* scale_x = reinterpret_cast<float*>(ws + q.off_scale);
+  float* factor = reinterpret_cast<float*>(ws + q.off_factor);
   float* inv = reinterpret_cast<float*>(ws + q.off_inv);
   const bool per_row = p->reduction == 0;
   uint8_t* d = ws + q.off_d;
+  uint8_t* d_w = per_row ? ws + q.off_d2 : d;  // what dW reads
   float* sum = reinterpret_cast<float*>(ws + q.off_sum);
   uint16_t* x_kept = reinterpret_cast<uint16_t*>(ws + q.off_x);
   int copies = dw ? cdiv((int64_t)p->rows * (p->hidden / 8), 4 * 1024) : 0;
   if (copies > 2 * device_sm_count()) copies = 2 * device_sm_count();
   const cudaError_t e =
-      launch_pdl(ce_row_weights_kernel<BF16>, dim3((unsigned)(1 + copies)), dim3(1024), 0, st, grad,
+      launch_pdl(ce_row_weights_kernel, dim3((unsigned)(1 + copies)), dim3(1024), 0, st, grad,
                  (int)per_row, p->targets, p->ignore_index, p->rows, p->vocab, count,
-                 (int)(p->reduction == 1), weight, rest, inv, static_cast<const uint16_t*>(p->x),
-                 p->x_stride, p->hidden, x_kept);
+                 (int)(p->reduction == 1), weight, scale_x, factor, inv,
+                 static_cast<const uint16_t*>(p->x), p->x_stride, p->hidden, x_kept);
   if (e != cudaSuccess) return abi_error(SSA_ERR_LAUNCH, "ce_row_weights: %s", cudaGetErrorString(e));
   note_launches(1);
   for (int i = 0; i < q.pieces; ++i) {
@@ -597,17 +596,22 @@ int ce_bwd(const ssa_linear_ce_t* p, const CePlan& q, const float* lse, const fl
     const int64_t cols = p->vocab - v0 < q.ldd ? p->vocab - v0 : q.ldd;  // of the vocabulary
     const int64_t wide = (int64_t)cdiv(cols, 256) * 256;                 // written to d
     const uint8_t* w0 = static_cast<const uint8_t*>(p->w) + 2 * v0 * p->w_stride;
-    const CeBwdArgs a{p->targets, lse, weight, d, q.ldd, p->rows, (int)v0, p->vocab};
+    const CeBwdArgs a{p->targets, lse, weight, factor, per_row && !dx ? nullptr : d,
+                      per_row && dw ? d_w : nullptr, q.ldd, p->rows, (int)v0, p->vocab};
     const GemmForm form = gemm_form(p->rows, wide);
-    int rc = ce_logits<EpiCeBwd<256, BF16>, EpiCeBwd<128, BF16>, BF16>(
-        p, form, w0, cols, (int)(wide / form.bn), a, st);
+    const int tiles_n = (int)(wide / form.bn);
+    int rc = per_row ? ce_logits<EpiCeBwd<256, BF16, true>, EpiCeBwd<128, BF16, true>, BF16>(
+                           p, form, w0, cols, tiles_n, a, st)
+                     : ce_logits<EpiCeBwd<256, BF16, false>, EpiCeBwd<128, BF16, false>, BF16>(
+                           p, form, w0, cols, tiles_n, a, st);
     if (rc != SSA_OK) return rc;
 
     StoreArgs sx{}, sw{};
     sx.out = q.dx_splits == 1 && q.pieces == 1 ? dx : nullptr;
     sx.sum = sum;
-    sx.scale = sw.scale = inv;
-    sx.row_scale = per_row ? rest : nullptr;
+    sx.scale = inv;
+    sw.scale = inv + 1;
+    sx.row_scale = per_row ? scale_x : nullptr;
     sx.rows = p->rows;
     sx.ldo = sx.cols = sw.ldo = sw.cols = p->hidden;
     sx.add_prev = i > 0;
@@ -620,7 +624,7 @@ int ce_bwd(const ssa_linear_ce_t* p, const CePlan& q, const float* lse, const fl
     sw.rows = (int)cols;
     const GemmShape gw = plain_shape(cdiv(cols, q.bwd.bm), tiles_h, cdiv(p->rows, 64),
                                      2 * (int64_t)p->rows * q.ldd);
-    const GemmOperand dk{d, p->rows, wide, q.ldd, "d"}, dmn{d, wide, p->rows, q.ldd, "d"};
+    const GemmOperand dk{d, p->rows, wide, q.ldd, "d"}, dmn{d_w, wide, p->rows, q.ldd, "d"};
     const GemmOperand wb{w0, p->hidden, cols, p->w_stride, "w"};
     const GemmOperand xb{x_kept, p->hidden, p->rows, p->hidden, "x"};
     const StoreProduct px{dk, wb, gx, sx}, pw{dmn, xb, gw, sw};
@@ -628,7 +632,7 @@ int ce_bwd(const ssa_linear_ce_t* p, const CePlan& q, const float* lse, const fl
     if (rc != SSA_OK) return rc;
   }
   if (dx && (q.dx_splits > 1 || q.pieces > 1))
-    return launch_sum_splits(BF16, sum, dx, inv, per_row ? rest : nullptr, p->rows, p->hidden,
+    return launch_sum_splits(BF16, sum, dx, inv, per_row ? scale_x : nullptr, p->rows, p->hidden,
                              p->hidden, q.dx_splits, st);
   return SSA_OK;
 }
