@@ -205,6 +205,13 @@ def row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def int32(n: int) -> int:
+    """A size for a 32-bit field of the C structs; ctypes would wrap a larger one without a word."""
+    if not 0 <= n < 1 << 31:
+        raise ValueError(f"size {n} does not fit 32 bits")
+    return n
+
+
 def table(t: torch.Tensor) -> torch.Tensor:
     """A contiguous, 16-byte aligned table: `t` itself, or a copy in fresh storage."""
     ok = t.is_contiguous() and t.data_ptr() % 16 == 0

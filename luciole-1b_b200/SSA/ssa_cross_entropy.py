@@ -24,9 +24,9 @@ _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
 def _problem(x, w, t, ignore_index, reduction):
-    return _lib.SsaLinearCe(_lib.DTYPE_CODES[x.dtype], x.shape[0], x.shape[1], w.shape[0],
-                            x.data_ptr(), _lib.row_stride(x), w.data_ptr(), _lib.row_stride(w),
-                            t.data_ptr(), ignore_index, reduction)
+    return _lib.SsaLinearCe(_lib.DTYPE_CODES[x.dtype], _lib.int32(x.shape[0]),
+                            _lib.int32(x.shape[1]), _lib.int32(w.shape[0]), x.data_ptr(),
+                            _lib.row_stride(x), w.data_ptr(), _lib.row_stride(w), t.data_ptr(), ignore_index, reduction)
 
 
 def _forward(hidden, weight, targets, ignore_index, code):
@@ -119,6 +119,8 @@ def ssa_linear_cross_entropy(hidden, weight, targets, ignore_index=-100, reducti
                          f"{tuple(hidden.shape[:-1])}")
     if targets.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"targets must be int64 or int32, got {targets.dtype}")
+    if not -(1 << 63) <= int(ignore_index) < 1 << 63:
+        raise ValueError(f"ignore_index {ignore_index} does not fit 64 bits")
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
     if _lib.differentiated(hidden, weight):

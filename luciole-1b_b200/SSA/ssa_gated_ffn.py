@@ -18,8 +18,9 @@ __all__ = ["SSAGatedFFNFunc", "ssa_gated_ffn"]
 
 
 def _problem(x, w):
-    return _lib.SsaGatedFfn(_lib.DTYPE_CODES[x.dtype], x.shape[0], x.shape[1], w.shape[0] // 2,
-                            x.data_ptr(), _lib.row_stride(x), w.data_ptr(), _lib.row_stride(w))
+    return _lib.SsaGatedFfn(_lib.DTYPE_CODES[x.dtype], _lib.int32(x.shape[0]),
+                            _lib.int32(x.shape[1]), _lib.int32(w.shape[0] // 2), x.data_ptr(),
+                            _lib.row_stride(x), w.data_ptr(), _lib.row_stride(w))
 
 
 def _forward(inp, weight):

@@ -34,8 +34,9 @@ def _tensor(t: torch.Tensor) -> _lib.SsaTensor:
 def _problem(x, hq, hkv, cos, sin, pos, pos_stride, wq, wk, eps):
     """x [B, S, Hq + 2 Hkv, D]."""
     return _lib.SsaQkRope(
-        _lib.DTYPE_CODES[x.dtype], x.shape[0], x.shape[1], hq, hkv, x.shape[3], _tensor(x),
-        cos.data_ptr(), sin.data_ptr(), cos.shape[0], pos.data_ptr() if pos is not None else None,
+        _lib.DTYPE_CODES[x.dtype], _lib.int32(x.shape[0]), _lib.int32(x.shape[1]), _lib.int32(hq),
+        _lib.int32(hkv), x.shape[3], _tensor(x), cos.data_ptr(), sin.data_ptr(),
+        _lib.int32(cos.shape[0]), pos.data_ptr() if pos is not None else None,
         1 if pos is not None and pos.dtype == torch.int64 else 0, pos_stride,
         wq.data_ptr() if wq is not None else None, wk.data_ptr() if wk is not None else None,
         _lib.DTYPE_CODES[wq.dtype if wq is not None else x.dtype], eps)
