@@ -9,8 +9,8 @@
 // rotate with, so the rotation needs no exchange and the norm a few shuffles. A lane walks kHeads
 // heads of one token with that token's cos and sin in registers (a table row is 4 to 8 times as wide
 // as a 16-bit head), all heads' loads issued before the first is used: 8 heads forward (65,536
-// tokens of 32 + 8 heads of 64, no norm: 2 heads 159 us, 4 heads 127 us, 8 heads 111 us), 4
-// backward, where more registers leave too few warps. Few tokens: one head each. What is read is
+// tokens of 32 + 8 heads of 64, no norm: 4 heads 114 us, 8 heads 110 us; heads_per_lane has more),
+// 4 backward, where more registers leave too few warps. Few tokens: one head each. What is read is
 // not read again here (streaming loads); what is written is left in L2 for the attention, unless it
 // is larger than that (streaming stores: 115 us without, 105 us with, 6.4 TB/s).
 //
@@ -351,10 +351,13 @@ struct RopePlan {
 };
 
 // Several heads per lane once that still leaves every multiprocessor several blocks: 4 from 2.4
-// million elements on, 8 forward from 78 million on (at 21 million 4 are 2 us faster).
+// million elements on, 8 forward from 19 million on. Forward, 32 + 8 heads of 64, inputs from memory,
+// 4 against 8: 5 million elements 5.7 and 6.7 us (with norm 7.9 and 6.6), 10 million 9.2 and 9.7 (12.2
+// and 10.9), 21 million 17.1 and 17.1 (22.2 and 19.1), 78 million 54.6 and 51.8 (69.9 and 62.9), 168
+// million 114 and 110 (145 and 130); fp32 within 1% everywhere.
 int64_t elements(const ssa_qk_rope_t* p) { return (int64_t)p->B * p->S * (p->Hq + p->Hkv) * p->D; }
 int heads_per_lane(const ssa_qk_rope_t* p) {
-  return elements(p) >= 148 * 16384 * 32 ? 8 : elements(p) >= 148 * 16384 ? 4 : 1;
+  return elements(p) >= 148 * 16384 * 8 ? 8 : elements(p) >= 148 * 16384 ? 4 : 1;
 }
 
 RopePlan rope_plan(const ssa_qk_rope_t* p) {

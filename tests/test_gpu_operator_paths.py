@@ -14,8 +14,8 @@ pytestmark = pytest.mark.gpu
                                         (True, torch.float32)])
 @pytest.mark.parametrize("lead,hq,hkv", [((76001,), 13, 3), ((3, 22003), 17, 1)])
 def test_rotation_of_many_tokens(cuda_device, norm, dtype, lead, hq, hkv):
-    """78 and 76 million query and key elements: eight and four heads a lane forward, head counts that
-    neither divides, results that do not stay in L2."""
+    """78 and 76 million query and key elements: eight heads a lane forward, four backward, head counts
+    that neither divides, results that do not stay in L2."""
     from test_gpu_qk_norm_rope import _check
     _check(lead, hq, hkv, 64, dtype, cuda_device, norm, seed=hq)
 
