@@ -229,8 +229,11 @@ def has_tangent(tensors) -> bool:
 def differentiated(*tensors) -> bool:
     """Whether a call on these tensors (or None) is autograd's business: a gradient is asked for, or
     there is a tangent, which the operators' Functions refuse (they have no jvp)."""
-    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) \
-        or has_tangent(tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return has_tangent(tensors)
 
 
 def first_order(backward):

@@ -26,7 +26,8 @@ _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 def _problem(x, w, t, ignore_index, reduction):
     return _lib.SsaLinearCe(_lib.DTYPE_CODES[x.dtype], _lib.int32(x.shape[0]),
                             _lib.int32(x.shape[1]), _lib.int32(w.shape[0]), x.data_ptr(),
-                            _lib.row_stride(x), w.data_ptr(), _lib.row_stride(w), t.data_ptr(), ignore_index, reduction)
+                            _lib.row_stride(x), w.data_ptr(), _lib.row_stride(w), t.data_ptr(),
+                            ignore_index, reduction)
 
 
 def _forward(hidden, weight, targets, ignore_index, code):
