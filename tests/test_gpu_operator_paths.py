@@ -27,6 +27,13 @@ def test_pieces_of_the_vocabulary_with_split_contractions(cuda_device, reduction
     _check(*_data(4100, 1024, 128001, torch.bfloat16, 33, 0.1, cuda_device), reduction)
 
 
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_more_rows_than_a_piece_of_256_mib_takes(cuda_device, reduction):
+    """140,001 rows: pieces of the least width, 1024 columns, are larger than that."""
+    from test_gpu_linear_ce import _check, _data
+    _check(*_data(140001, 64, 2101, torch.bfloat16, 35, 0.1, cuda_device), reduction)
+
+
 def _ffn(seed, dev):
     from SSA.ssa_gated_ffn import ssa_gated_ffn
     from test_gpu_gated_ffn import _data
