@@ -7,7 +7,10 @@
 // leaves directly. Nothing but x and the weights is kept for the backward, which forms the
 // pre-activations again (fp32: the derivative sees no rounding) and writes
 //     dg = dh u s (1 + g (1 - s)),  du = dh g s,  s = sigmoid(g)
-// as one 16-bit matrix d = [dg | du]; then dx = d W and dW = d^T x are two plain products. Bound:
+// as one 16-bit matrix d = [dg | du]; then dx = d W and dW = d^T x are two plain products. d is
+// rounded to 16 bits because it is their operand: with the rounding of the results both are 0.029% off
+// in fp16 and 0.23% in bf16, where the results' rounding alone is 0.021% and 0.17%; an fp32 d would take
+// two or three products for each. In fp16 d has that type's range too, as dh has: 6e-8 to 65,504. Bound:
 // the tensor cores, 16 rows hidden ffn operations for forward and backward against the 12 that
 // kept pre-activations would need (at 8 bytes of memory per row and ffn column, held over the whole
 // forward). A forward of few rows has a kernel of its own, bound by memory.

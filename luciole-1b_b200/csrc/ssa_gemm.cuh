@@ -3,7 +3,7 @@
 // gated feed-forward (ssa_gated_ffn.cu).
 //
 // A tile is 128 CG rows by BN columns, made by a cluster of CG CTAs. Each CTA holds 128 rows of A and
-// BN / CG = 128 rows of B per 64-wide K block in shared memory (32 KB a stage, 6 stages) and the
+// BN / CG = 128 rows of B per 64-wide K block in shared memory (32 KB a stage, 6 stages; 48 KB and 4 with NH = 2) and the
 // fp32 accumulator of its 128 rows in BN TMEM columns, twice, so that the epilogue of one tile runs
 // under the MMAs of the next. CG = 2, BN = 256 is the form for large products: the pair's MMA reads
 // both halves of B, so a CTA fetches 32 KB per 4.2 MFLOP where a lone 128 x 256 tile fetches 48 KB.
